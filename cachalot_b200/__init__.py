@@ -17,8 +17,9 @@ _OPS = (
     "affine_expert_forward_batched", "SlabExperts", "shared_expert_forward", "shared_expert_forward_fused",
     "shared_expert_forward_batched", "fp8_linear_rows", "bf16_gemv_f32", "fused_qr_kv_linear", "moe_layer_forward", "validate_routing", "self_check", "requantize_fp4_to_affine", "requantize_bank",
 )
+_PAGED = ("PagePlan", "plan_pages")
 _LOADER = ("load_bank", "detect_expert_bank", "build_expert_index", "build_stacked_expert_index")
-__all__ = [*_BANK, *_OPS, *_LOADER, "NUMERICS_VERSION"]
+__all__ = [*_BANK, *_OPS, *_PAGED, *_LOADER, "NUMERICS_VERSION"]
 
 
 def __getattr__(name):
@@ -28,6 +29,8 @@ def __getattr__(name):
         return getattr(importlib.import_module(".bank", __name__), name)
     if name in _OPS:
         return getattr(importlib.import_module(".ops", __name__), name)
+    if name in _PAGED:
+        return getattr(importlib.import_module(".paged", __name__), name)
     if name in _LOADER:
         return getattr(importlib.import_module(".loader", __name__), name)
     raise AttributeError(f"module {__name__!r} has no attribute {name!r}")

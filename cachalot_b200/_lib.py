@@ -15,11 +15,13 @@ LIB_PATH = Path(os.environ.get("CACHALOT_B200_LIB", _PKG / "libcachalot_b200.so"
 OK, EINVAL, EALIGN, EUNSUPPORTED, ECUDA, ESCRATCH = 0, -1, -2, -3, -4, -5
 BANK_FP4, BANK_AFFINE = 0, 1
 F16, BF16, F32 = 0, 1, 2
+E4M3 = 3  # paged caches only
 NUMERICS_F32, NUMERICS_BF16, NUMERICS_BF16_H32 = 0, 1, 2
 DECODE_ONLY_GATE_UP, DECODE_ONLY_DOWN, DECODE_SIMPLE, DECODE_UNFUSED = 0x100, 0x200, 0x400, 0x800
 ROUTER_SQRT_SOFTPLUS, ROUTER_SIGMOID = 0, 1
 SCALE_E8M0, SCALE_F32 = 0, 1
 STATUS_SLOT_RANGE, STATUS_ID_RANGE, STATUS_SCALE_RANGE, STATUS_WAIT_EXPIRED, STATUS_BAD_WEIGHT = 1, 2, 4, 8, 16
+STATUS_LENGTH, STATUS_NO_PAGE = 32, 64
 
 
 class BankDesc(C.Structure):
@@ -45,7 +47,17 @@ class PeerCtx(C.Structure):
     _fields_ = [("inbox", C.c_void_p * 8), ("epoch", C.c_void_p), ("world", C.c_int32), ("rank", C.c_int32)]
 
 
+class PagedKV(C.Structure):
+    """Mirror of `cachalot_paged_kv`."""
+
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
+                ("k_page_stride", C.c_int64), ("k_head_stride", C.c_int64), ("k_token_stride", C.c_int64),
+                ("v_page_stride", C.c_int64), ("v_head_stride", C.c_int64), ("v_token_stride", C.c_int64),
+                ("n_pages", C.c_int32), ("page_size", C.c_int32), ("kv_heads", C.c_int32), ("head_dim", C.c_int32), ("dtype", C.c_int32)]
+
+
 _vp, _i, _f, _sz = C.c_void_p, C.c_int, C.c_float, C.c_size_t
+_i64 = C.c_int64
 _desc = C.POINTER(BankDesc)
 
 # name -> (restype, argtypes); the list is also what the symbol-export test walks
@@ -84,6 +96,7 @@ SIGNATURES = {
     "cachalot_peer_layer_inbox_bytes": (_sz, [_i, _i]),
     "cachalot_moe_layer_decode_peer": (_i, [_vp, _desc, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _f, _f, _i, _i, _f, _i, _vp, _sz, _vp, _i,
                                             _vp, _vp, _vp, _vp, _vp]),
+    "cachalot_plan_pages": (_i, [_vp, _vp, _i, _vp, _i64, _i, _vp, _i, _vp, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
     "cachalot_moe_prefill": (_i, [_vp, _desc, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _f, _i, _vp, _sz, _vp, _vp, _vp]),
 }
 

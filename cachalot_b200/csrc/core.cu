@@ -13,4 +13,5 @@ void set_error(const char* fmt, ...) {
 
 extern "C" const char* cachalot_last_error(void) { return cachalot::g_error; }
 // 2: cachalot_group_rows takes cachalot_group_rows_scratch_ints() of scratch; rows-level prefill, combine and peer sum added
-extern "C" int cachalot_version(void) { return 2; }
+// 3: paged cache, attention and log probabilities of a decode step
+extern "C" int cachalot_version(void) { return 3; }

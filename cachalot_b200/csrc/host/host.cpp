@@ -29,7 +29,8 @@ using at::ScalarType;
 #define ENTRIES(X) \
   X(cachalot_bf16_gemv_f32) X(cachalot_fp8_linear) X(cachalot_group_rows) X(cachalot_group_rows_scratch_ints) \
   X(cachalot_last_error) X(cachalot_moe_decode) X(cachalot_moe_decode_workspace_bytes) X(cachalot_moe_layer_decode) \
-  X(cachalot_moe_layer_decode_workspace_bytes) X(cachalot_moe_prefill) X(cachalot_moe_prefill_experts_workspace_bytes) X(cachalot_route_topk) \
+  X(cachalot_moe_layer_decode_workspace_bytes) X(cachalot_moe_prefill) X(cachalot_moe_prefill_experts_workspace_bytes) X(cachalot_plan_pages) \
+  X(cachalot_route_topk) \
   X(cachalot_router_logits) X(cachalot_shared_expert) X(cachalot_shared_expert_workspace_bytes)
 struct Lib {
 #define X(name) decltype(&::name) name = nullptr;
@@ -402,9 +403,47 @@ PyObject* moe_block(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   END_HANDLE_TH_ERRORS
 }
 
+// ---- the decode step around the experts ----
+
+// int32 [n], contiguous
+bool plain_ints(const at::Tensor* t, int64_t n, int device) { return plain(t, ScalarType::Int, device) && t->dim() == 1 && t->size(0) == n; }
+// int32 [rows, width] with contiguous rows that do not overlap
+bool table_of(const at::Tensor* t, int64_t rows, int device) {
+  return t && t->is_cuda() && t->scalar_type() == ScalarType::Int && t->get_device() == device && t->dim() == 2 && t->size(0) == rows && t->size(1) > 0 &&
+         t->size(1) < (1 << 30) && t->stride(1) == 1 && t->stride(0) >= t->size(1);
+}
+int32_t* ints(const at::Tensor& t) { return static_cast<int32_t*>(t.data_ptr()); }
+
+// (context_lens, new_lens, block_table, free_pages, free_count, page_size, tokens, status | None)
+//  -> (starts, requests, positions, slots, lens, free_count)
+PyObject* plan_pages(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+  HANDLE_TH_ERRORS
+  PLAIN_OR_NONE(bound && n_args == 8);
+  Args p{a};
+  const at::Tensor* ctx = tensor_of(a[0]);
+  PLAIN_OR_NONE(ctx && ctx->is_cuda());  // before the device is asked for: without a GPU the general form refuses the tensors
+  const int dev = current_device(), page = (int)p.i(5), tokens = (int)p.i(6);
+  const at::Tensor *fresh = tensor_of(a[1]), *table = tensor_of(a[2]), *pages = tensor_of(a[3]), *count = tensor_of(a[4]);
+  PLAIN_OR_NONE(!p.bad && page > 0 && tokens > 0 && ctx->dim() == 1 && none_or_plain(a[7], ScalarType::Int, dev));
+  const int64_t r = ctx->size(0);
+  PLAIN_OR_NONE(r > 0 && plain_ints(ctx, r, dev) && plain_ints(fresh, r, dev) && table_of(table, r, dev) && pages && pages->dim() == 1);
+  PLAIN_OR_NONE(pages->size(0) < (1LL << 31) && plain_ints(pages, pages->size(0), dev) && plain_ints(count, 1, dev));
+  PLAIN_OR_NONE(a[7] == Py_None || tensor_of(a[7])->numel() > 0);
+  at::Tensor out[6];
+  const int64_t sizes[6] = {r + 1, tokens, tokens, tokens, r, 1};
+  for (int i = 0; i < 6; ++i) out[i] = empty({sizes[i]}, ScalarType::Int, dev);
+  const int rc = UNLOCKED(lib.cachalot_plan_pages(ints(*ctx), ints(*fresh), (int)r, ints(*table), table->stride(0), (int)table->size(1), ints(*pages),
+                                                  (int)pages->size(0), ints(*count), page, tokens, ints(out[0]), ints(out[1]), ints(out[2]),
+                                                  ints(out[3]), ints(out[4]), ints(out[5]), static_cast<int*>(ptr_or_null(a[7])), current_stream(dev)));
+  if (rc) return raise(rc);
+  return Py_BuildValue("(NNNNNN)", THPVariable_Wrap(std::move(out[0])), THPVariable_Wrap(std::move(out[1])), THPVariable_Wrap(std::move(out[2])),
+                       THPVariable_Wrap(std::move(out[3])), THPVariable_Wrap(std::move(out[4])), THPVariable_Wrap(std::move(out[5])));
+  END_HANDLE_TH_ERRORS
+}
+
 #define FAST(name) {#name, (PyCFunction)(void (*)(void))name, METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {FAST(entries), FAST(bind), FAST(fp8_linear), FAST(bf16_gemv_f32), FAST(shared_expert), FAST(moe_forward), FAST(layer_decode),
-                         FAST(prefill_grouped), FAST(moe_block), {nullptr, nullptr, 0, nullptr}};
+                         FAST(prefill_grouped), FAST(moe_block), FAST(plan_pages), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", "Native call path of the operators (see host.cpp).", -1, methods};
 
 }  // namespace

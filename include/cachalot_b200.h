@@ -44,11 +44,14 @@ enum {
   CACHALOT_STATUS_ID_RANGE = 2,   /* an expert id outside [0, E) was seen and dropped */
   CACHALOT_STATUS_SCALE_RANGE = 4, /* an FP4 block scale outside the window around fp4_scale_centre was clamped */
   CACHALOT_STATUS_WAIT_EXPIRED = 8, /* a bounded device-side wait ran out (the result of that call is not valid) */
-  CACHALOT_STATUS_BAD_WEIGHT = 16 /* a router weight was NaN or infinite (it was used as it is) */
+  CACHALOT_STATUS_BAD_WEIGHT = 16, /* a router weight was NaN or infinite (it was used as it is) */
+  CACHALOT_STATUS_LENGTH = 32, /* a length was negative, or more than its block table or output has room for (it was cut) */
+  CACHALOT_STATUS_NO_PAGE = 64 /* the free pages ran out: the tokens that got none have slot -1 */
 };
 
 enum { CACHALOT_BANK_FP4 = 0, CACHALOT_BANK_AFFINE = 1 };
 enum { CACHALOT_F16 = 0, CACHALOT_BF16 = 1, CACHALOT_F32 = 2 };
+enum { CACHALOT_E4M3 = 3 }; /* paged caches only */
 /* rounding points of the expert FFN */
 enum {
   CACHALOT_NUMERICS_F32 = 0, /* decode FP4 op: fp32 everywhere (model/moe_fused_metal.py:101-179) */
@@ -96,7 +99,7 @@ typedef struct {
 } cachalot_bank_desc;
 
 CACHALOT_API const char* cachalot_last_error(void);
-CACHALOT_API int cachalot_version(void); /* ABI revision, 2 for this header */
+CACHALOT_API int cachalot_version(void); /* ABI revision, 3 for this header */
 
 /* ---- dequantisation (bit-exact against the reference's numpy path) ------------------------ */
 
@@ -355,6 +358,39 @@ CACHALOT_API int cachalot_moe_layer_decode_peer(const void* bank, const cachalot
                                    size_t workspace_bytes, void* out, int out_dtype, int32_t* indices_out,
                                    float* weights_out, const cachalot_peer_ctx* peer /* host */, int* status,
                                    cachalot_stream_t stream);
+
+/* ---- the decode step around the experts: paged key-value cache, attention, log probabilities --- */
+
+/* A paged key-value cache of one layer: n_pages pages of page_size tokens.  Element (page, head, token, d) of the keys is
+ * k[page * k_page_stride + head * k_head_stride + token * k_token_stride + d] (strides in elements, multiples of 16 bytes;
+ * the values likewise), so pages may hold their heads or their tokens outermost.  dtype CACHALOT_F16, CACHALOT_BF16 or
+ * CACHALOT_E4M3; an E4M3 cache stands for code * scale with one scale per head (NULL: 1).  A slot names a token of the
+ * cache: page * page_size + token within the page.  n_pages * page_size < 2^31. */
+typedef struct {
+  void* k;
+  void* v;
+  const float* k_scale; /* f32 [kv_heads] or NULL */
+  const float* v_scale;
+  int64_t k_page_stride, k_head_stride, k_token_stride;
+  int64_t v_page_stride, v_head_stride, v_token_stride;
+  int32_t n_pages, page_size, kv_heads, head_dim;
+  int32_t dtype;
+} cachalot_paged_kv;
+
+/* No counterpart in the reference (one request, contiguous caches).  Places a step's new tokens: request r holds
+ * context_lens[r] tokens and gets new_lens[r] more (both i32 [requests]).  The new tokens are numbered request by request,
+ * those past `tokens` are left out (CACHALOT_STATUS_LENGTH) as if they had not been asked for; pages that a request needs
+ * beyond the ceil(context / page_size) it has come from the end of free_pages[0 .. *free_count), request by request and
+ * page by page, and are written into block_table (i32 [requests, width], rows table_stride apart); nothing else of the
+ * table is written.  Outputs: starts i32 [requests+1] (first token of every request), request_of, positions, slots
+ * i32 [tokens] (past the last token: -1, 0, -1), lens i32 [requests] = context + new, free_count_out i32 [1] = pages left.
+ * A token without a page (none left: CACHALOT_STATUS_NO_PAGE; past the table's width: CACHALOT_STATUS_LENGTH; a negative
+ * table entry) has slot -1.  No output may overlap an input, block_table apart.  requests <= 8192; n_free = the length of
+ * free_pages; status (or NULL) gets the bits OR-ed in. */
+CACHALOT_API int cachalot_plan_pages(const int32_t* context_lens, const int32_t* new_lens, int requests, int32_t* block_table,
+                        int64_t table_stride, int width, const int32_t* free_pages, int n_free, const int32_t* free_count,
+                        int page_size, int tokens, int32_t* starts, int32_t* request_of, int32_t* positions, int32_t* slots,
+                        int32_t* lens, int32_t* free_count_out, int* status, cachalot_stream_t stream);
 
 #ifdef __cplusplus
 }
