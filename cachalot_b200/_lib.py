@@ -97,6 +97,8 @@ SIGNATURES = {
     "cachalot_moe_layer_decode_peer": (_i, [_vp, _desc, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _f, _f, _i, _i, _f, _i, _vp, _sz, _vp, _i,
                                             _vp, _vp, _vp, _vp, _vp]),
     "cachalot_plan_pages": (_i, [_vp, _vp, _i, _vp, _i64, _i, _vp, _i, _vp, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "cachalot_qk_norm_rope": (_i, [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _i, _i, _i, _i, _i, _vp, _vp, _i, _f, _vp, _vp, _i, _i, _f,
+                                   _vp, _vp, C.POINTER(PagedKV), _vp, _vp, _vp]),
     "cachalot_moe_prefill": (_i, [_vp, _desc, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _f, _i, _vp, _sz, _vp, _vp, _vp]),
 }
 

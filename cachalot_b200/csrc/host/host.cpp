@@ -30,6 +30,7 @@ using at::ScalarType;
   X(cachalot_bf16_gemv_f32) X(cachalot_fp8_linear) X(cachalot_group_rows) X(cachalot_group_rows_scratch_ints) \
   X(cachalot_last_error) X(cachalot_moe_decode) X(cachalot_moe_decode_workspace_bytes) X(cachalot_moe_layer_decode) \
   X(cachalot_moe_layer_decode_workspace_bytes) X(cachalot_moe_prefill) X(cachalot_moe_prefill_experts_workspace_bytes) X(cachalot_plan_pages) \
+  X(cachalot_qk_norm_rope) \
   X(cachalot_route_topk) \
   X(cachalot_router_logits) X(cachalot_shared_expert) X(cachalot_shared_expert_workspace_bytes)
 struct Lib {
@@ -441,9 +442,84 @@ PyObject* plan_pages(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   END_HANDLE_TH_ERRORS
 }
 
+int element_code(ScalarType t) { return t == ScalarType::Half ? CACHALOT_F16 : t == ScalarType::BFloat16 ? CACHALOT_BF16 : t == ScalarType::Float8_e4m3fn ? CACHALOT_E4M3 : -1; }
+bool none_or_scales(PyObject* o, int64_t heads, int device) {
+  return o == Py_None || (plain(tensor_of(o), ScalarType::Float, device) && tensor_of(o)->dim() == 1 && tensor_of(o)->size(0) == heads);
+}
+// a cache of one layer: k_cache, v_cache [pages, heads, page_size, dim] with contiguous rows, and the scales of an E4M3 one
+bool cache_from(const at::Tensor* k, const at::Tensor* v, PyObject* k_scale, PyObject* v_scale, int device, cachalot_paged_kv* c) {
+  if (!k || !v || !k->is_cuda() || !v->is_cuda() || k->get_device() != device || v->get_device() != device) return false;
+  if (k->dim() != 4 || k->sizes() != v->sizes() || k->scalar_type() != v->scalar_type() || k->stride(3) != 1 || v->stride(3) != 1) return false;
+  c->dtype = element_code(k->scalar_type());
+  for (int i = 0; i < 4; ++i)
+    if (k->size(i) <= 0 || k->size(i) >= (1LL << 31)) return false;
+  if (c->dtype < 0 || !none_or_scales(k_scale, k->size(1), device) || !none_or_scales(v_scale, k->size(1), device)) return false;
+  if (c->dtype != CACHALOT_E4M3 && (k_scale != Py_None || v_scale != Py_None)) return false;
+  c->k = k->data_ptr(), c->v = v->data_ptr();
+  c->k_scale = static_cast<const float*>(ptr_or_null(k_scale)), c->v_scale = static_cast<const float*>(ptr_or_null(v_scale));
+  c->k_page_stride = k->stride(0), c->k_head_stride = k->stride(1), c->k_token_stride = k->stride(2);
+  c->v_page_stride = v->stride(0), c->v_head_stride = v->stride(1), c->v_token_stride = v->stride(2);
+  c->n_pages = (int32_t)k->size(0), c->kv_heads = (int32_t)k->size(1), c->page_size = (int32_t)k->size(2), c->head_dim = (int32_t)k->size(3);
+  return true;
+}
+// [tokens, heads, dim] of this type whose heads are 16-byte rows
+bool head_rows(const at::Tensor* t, ScalarType dt, int device) {
+  return t && t->is_cuda() && t->scalar_type() == dt && t->get_device() == device && t->dim() == 3 && t->stride(2) == 1 && t->stride(0) % 8 == 0 &&
+         t->stride(1) % 8 == 0 && reinterpret_cast<uintptr_t>(t->data_ptr()) % 16 == 0;
+}
+
+// (q, k, positions, inv_freq, q_weight | None, k_weight | None, eps, interleaved, magnitude, v | None, k_cache | None, v_cache | None, slots | None,
+//  k_scale | None, v_scale | None, status | None) -> (q_out, k_out | None)
+PyObject* qk_norm_rope(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+  HANDLE_TH_ERRORS
+  PLAIN_OR_NONE(bound && n_args == 16);
+  Args p{a};
+  const at::Tensor *q = tensor_of(a[0]), *k = tensor_of(a[1]), *pos = tensor_of(a[2]), *freq = tensor_of(a[3]);
+  PLAIN_OR_NONE(q && q->is_cuda());
+  const int dev = current_device();
+  const ScalarType dt = q->scalar_type();
+  const double eps = p.f(6), magnitude = p.f(8);
+  const int interleaved = PyObject_IsTrue(a[7]);
+  PLAIN_OR_NONE(!p.bad && interleaved >= 0 && (dt == ScalarType::Half || dt == ScalarType::BFloat16) && head_rows(q, dt, dev) && head_rows(k, dt, dev));
+  const int64_t tokens = q->size(0), heads = q->size(1), dim = q->size(2), kv_heads = k->size(1);
+  PLAIN_OR_NONE(tokens > 0 && tokens < (1LL << 31) && heads > 0 && heads < (1 << 20) && kv_heads > 0 && kv_heads < (1 << 20) && dim > 0 && dim <= 4096);
+  PLAIN_OR_NONE(k->size(0) == tokens && k->size(2) == dim && plain_ints(pos, tokens, dev) && plain(freq, ScalarType::Double, dev) && freq->dim() == 1 && freq->size(0) <= dim);
+  ScalarType wt = dt;
+  for (int i = 4; i < 6; ++i) {
+    const at::Tensor* w = a[i] == Py_None ? nullptr : tensor_of(a[i]);
+    PLAIN_OR_NONE(a[i] == Py_None || (w && (plain(w, dt, dev) || plain(w, ScalarType::Float, dev)) && w->dim() == 1 && w->size(0) == dim));
+    if (!w) continue;
+    PLAIN_OR_NONE(i == 4 || a[4] == Py_None || wt == w->scalar_type());
+    PLAIN_OR_NONE(reinterpret_cast<uintptr_t>(w->data_ptr()) % 16 == 0);
+    wt = w->scalar_type();
+  }
+  PLAIN_OR_NONE(none_or_plain(a[15], ScalarType::Int, dev) && (a[15] == Py_None || tensor_of(a[15])->numel() > 0));
+  const bool stored = a[10] != Py_None;
+  cachalot_paged_kv cache;
+  const at::Tensor* v = nullptr;
+  if (stored) {
+    v = tensor_of(a[9]);
+    PLAIN_OR_NONE(a[11] != Py_None && cache_from(tensor_of(a[10]), tensor_of(a[11]), a[13], a[14], dev, &cache));
+    PLAIN_OR_NONE(head_rows(v, dt, dev) && v->sizes() == k->sizes() && plain_ints(tensor_of(a[12]), tokens, dev));
+  } else {
+    PLAIN_OR_NONE(a[9] == Py_None && a[11] == Py_None && a[12] == Py_None && a[13] == Py_None && a[14] == Py_None);
+  }
+  at::Tensor y = empty({tokens, heads, dim}, dt, dev), ko;
+  if (!stored) ko = empty({tokens, kv_heads, dim}, dt, dev);
+  const int rc = UNLOCKED(lib.cachalot_qk_norm_rope(
+      q->data_ptr(), q->stride(0), q->stride(1), k->data_ptr(), k->stride(0), k->stride(1), stored ? v->data_ptr() : nullptr, stored ? v->stride(0) : 0,
+      stored ? v->stride(1) : 0, element_code(dt), (int)tokens, (int)heads, (int)kv_heads, (int)dim, ptr_or_null(a[4]), ptr_or_null(a[5]),
+      wt == ScalarType::Float ? CACHALOT_F32 : element_code(dt), (float)eps, ints(*pos), static_cast<const double*>(freq->data_ptr()),
+      2 * (int)freq->size(0), interleaved, (float)magnitude, y.data_ptr(), stored ? nullptr : ko.data_ptr(), stored ? &cache : nullptr,
+      stored ? ints(*tensor_of(a[12])) : nullptr, static_cast<int*>(ptr_or_null(a[15])), current_stream(dev)));
+  if (rc) return raise(rc);
+  return Py_BuildValue("(NN)", THPVariable_Wrap(std::move(y)), stored ? Py_NewRef(Py_None) : THPVariable_Wrap(std::move(ko)));
+  END_HANDLE_TH_ERRORS
+}
+
 #define FAST(name) {#name, (PyCFunction)(void (*)(void))name, METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {FAST(entries), FAST(bind), FAST(fp8_linear), FAST(bf16_gemv_f32), FAST(shared_expert), FAST(moe_forward), FAST(layer_decode),
-                         FAST(prefill_grouped), FAST(moe_block), FAST(plan_pages), {nullptr, nullptr, 0, nullptr}};
+                         FAST(prefill_grouped), FAST(moe_block), FAST(plan_pages), FAST(qk_norm_rope), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", "Native call path of the operators (see host.cpp).", -1, methods};
 
 }  // namespace

@@ -10,6 +10,8 @@ go through the native call path, and none has a PyTorch or CPU fallback.
 """
 from __future__ import annotations
 
+import ctypes as C
+import math
 from typing import NamedTuple
 
 import torch
@@ -50,6 +52,31 @@ def _block_table(t: torch.Tensor, rows: int) -> None:
         raise ValueError(f"block_table must be int32 [{rows}, width], got {t.dtype} {tuple(t.shape)}")
     if t.shape[1] > 1 and t.stride(1) != 1 or rows > 1 and t.stride(0) < t.shape[1]:
         raise ValueError("block_table rows must be contiguous")
+
+
+_DT = {torch.float16: _lib.F16, torch.bfloat16: _lib.BF16, torch.float32: _lib.F32, torch.float8_e4m3fn: _lib.E4M3}
+
+
+def _cache(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale, v_scale) -> _lib.PagedKV:
+    """The descriptor of a cache of one layer."""
+    if k_cache.dim() != 4 or k_cache.shape != v_cache.shape:
+        raise ValueError(f"k_cache and v_cache must both be [pages, kv_heads, page_size, head_dim], got {tuple(k_cache.shape)} and {tuple(v_cache.shape)}")
+    if k_cache.dtype != v_cache.dtype or k_cache.dtype not in (torch.float16, torch.bfloat16, torch.float8_e4m3fn):
+        raise ValueError(f"a cache holds float16, bfloat16 or float8_e4m3fn, got {k_cache.dtype} and {v_cache.dtype}")
+    pages, heads, page, dim = k_cache.shape
+    for t in (k_cache, v_cache):
+        if t.stride(3) != 1 and dim > 1:
+            raise ValueError("the last axis of a cache must be contiguous")
+    scaled = k_cache.dtype == torch.float8_e4m3fn
+    for t in (k_scale, v_scale):
+        if t is not None and (not scaled or t.dtype != torch.float32 or tuple(t.shape) != (heads,) or not t.is_contiguous()):
+            raise ValueError(f"scales are float32 [{heads}] and belong to a float8_e4m3fn cache")
+    d = _lib.PagedKV()
+    d.k, d.v, d.k_scale, d.v_scale = _ptr(k_cache), _ptr(v_cache), _ptr(k_scale), _ptr(v_scale)
+    d.k_page_stride, d.k_head_stride, d.k_token_stride = k_cache.stride()[:3]
+    d.v_page_stride, d.v_head_stride, d.v_token_stride = v_cache.stride()[:3]
+    d.n_pages, d.page_size, d.kv_heads, d.head_dim, d.dtype = pages, page, heads, dim, _DT[k_cache.dtype]
+    return d
 
 
 # ---- page plan --------------------------------------------------------------------------------
@@ -97,3 +124,97 @@ def plan_pages(context_lens: torch.Tensor, new_lens: torch.Tensor, block_table: 
                                       _ptr(count), page_size, tokens, _ptr(starts), _ptr(requests), _ptr(positions), _ptr(slots), _ptr(lens),
                                       _ptr(left), _ptr(status), _stream(dev)))
     return PagePlan(starts, requests, positions, slots, lens, left)
+
+
+# ---- queries and keys -------------------------------------------------------------------------
+
+def rope_frequencies(rotary_dim: int, *, base: float = 10000.0, scaling: str | None = None, factor: float = 1.0, trained_len: int = 0,
+                     beta_fast: float = 32.0, beta_slow: float = 1.0, device="cuda") -> tuple[torch.Tensor, float]:
+    """(inv_freq float64 [rotary_dim/2] in radians per position, magnitude) for `qk_norm_rope`, computed once on the host.
+    f_i = base ** (-2i / rotary_dim).  For contexts `factor` times as long as the trained one: "linear" stretches every
+    frequency, "ntk" raises the base so that the slowest one is stretched and the fastest kept, "yarn" (Peng et al. 2023)
+    stretches those that turn less than beta_slow times over `trained_len` positions, keeps those that turn more than
+    beta_fast times, blends in between and lengthens the rotated vector by 0.1 ln(factor) + 1."""
+    if rotary_dim <= 0 or rotary_dim % 2:
+        raise ValueError(f"rotary_dim must be positive and even, got {rotary_dim}")
+    if scaling not in (None, "linear", "ntk", "yarn"):
+        raise ValueError(f"unknown scaling {scaling!r}")
+    if factor < 1.0 or base <= 1.0:
+        raise ValueError(f"factor must be at least 1 and base above 1, got {factor} and {base}")
+    magnitude = 1.0
+    if scaling == "ntk" and rotary_dim > 2:
+        base *= factor ** (rotary_dim / (rotary_dim - 2))
+    f = [base ** (-2.0 * i / rotary_dim) for i in range(rotary_dim // 2)]
+    if scaling == "linear":
+        f = [x / factor for x in f]
+    if scaling == "yarn":
+        if trained_len <= 0:
+            raise ValueError("yarn needs trained_len")
+        pair = lambda turns: rotary_dim * math.log(trained_len / (turns * 2 * math.pi)) / (2 * math.log(base))  # noqa: E731
+        lo, hi = max(math.floor(pair(beta_fast)), 0), min(math.ceil(pair(beta_slow)), rotary_dim - 1)
+        stretched = [min(max((i - lo) / max(hi - lo, 1e-3), 0.0), 1.0) for i in range(rotary_dim // 2)]
+        f = [x * (1.0 - s) + x / factor * s for x, s in zip(f, stretched)]
+        magnitude = 0.1 * math.log(factor) + 1.0
+    return torch.tensor(f, dtype=torch.float64, device=device), magnitude
+
+
+def _rows16(t: torch.Tensor) -> torch.Tensor:
+    """The tensor itself if its heads are 16-byte rows, else a contiguous copy."""
+    ok = t.stride(2) == 1 and t.stride(0) % 8 == 0 and t.stride(1) % 8 == 0 and t.data_ptr() % 16 == 0
+    return t if ok else t.clone(memory_format=torch.contiguous_format)
+
+
+def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, *, q_weight: torch.Tensor | None = None,
+                 k_weight: torch.Tensor | None = None, eps: float = 1e-6, interleaved: bool = False, magnitude: float = 1.0,
+                 v: torch.Tensor | None = None, k_cache: torch.Tensor | None = None, v_cache: torch.Tensor | None = None,
+                 slots: torch.Tensor | None = None, k_scale: torch.Tensor | None = None, v_scale: torch.Tensor | None = None,
+                 status: torch.Tensor | None = None):
+    """Norm of every query and key head, position rotation and cache write of new tokens in one launch
+    (model/norm_rope_mlx.py, model/decode_fused_metal.py:43): q [tokens, heads, dim], k and v [tokens, kv_heads, dim]
+    float16 or bfloat16 (views of the projection's rows as they are), positions int32 [tokens].
+
+    q_weight, k_weight [dim] (None: no norm); `inv_freq` and `magnitude` from `rope_frequencies`, the first
+    2 * len(inv_freq) elements of a head are rotated, as pairs (i, i + half) or, `interleaved`, (2i, 2i + 1).  Everything
+    in fp32 (angles in 64 bits), rounded once.  With a cache, keys and values go to `slots` int32 [tokens] (-1: not
+    stored; a slot named twice in a call: undefined) and (q_out, None) is returned, else (q_out, k_out)."""
+    r = _host.qk_norm_rope(q, k, positions, inv_freq, q_weight, k_weight, eps, interleaved, magnitude, v, k_cache, v_cache, slots, k_scale, v_scale, status)
+    if r is not None:
+        return r
+    dev = _same_device(q, k, positions, inv_freq, q_weight, k_weight, v, k_cache, v_cache, slots, k_scale, v_scale, status)
+    if q.dim() != 3 or k.dim() != 3 or q.shape[0] != k.shape[0] or q.shape[2] != k.shape[2]:
+        raise ValueError(f"q and k must be [tokens, heads, dim], got {tuple(q.shape)} and {tuple(k.shape)}")
+    if q.dtype not in (torch.float16, torch.bfloat16) or k.dtype != q.dtype:
+        raise ValueError(f"q and k must both be float16 or both bfloat16, got {q.dtype} and {k.dtype}")
+    tokens, heads, dim = q.shape
+    kv_heads = k.shape[1]
+    pos = _ints(positions, "positions", (tokens,))
+    if inv_freq.dtype != torch.float64 or inv_freq.dim() != 1:
+        raise ValueError(f"inv_freq must be float64 [rotary_dim / 2], got {inv_freq.dtype} {tuple(inv_freq.shape)}")
+    w_dtype = None
+    for w, name in ((q_weight, "q_weight"), (k_weight, "k_weight")):
+        if w is not None:
+            if tuple(w.shape) != (dim,) or w.dtype not in (q.dtype, torch.float32) or w_dtype not in (None, w.dtype):
+                raise ValueError(f"{name} must be [{dim}] in {q.dtype} or float32 (both weights alike), got {w.dtype} {tuple(w.shape)}")
+            w_dtype = w.dtype
+    _status(status)
+    desc = None
+    with torch.cuda.device(dev):
+        if k_cache is not None or v_cache is not None:
+            if k_cache is None or v_cache is None or v is None or slots is None:
+                raise ValueError("a cache write needs v, k_cache, v_cache and slots")
+            if v.dtype != q.dtype or v.shape != k.shape:
+                raise ValueError(f"v must be {q.dtype} {tuple(k.shape)}, got {v.dtype} {tuple(v.shape)}")
+            desc = _cache(k_cache, v_cache, k_scale, v_scale)
+            slots, v = _ints(slots, "slots", (tokens,)), _rows16(v)
+        elif v is not None or slots is not None or k_scale is not None or v_scale is not None:
+            raise ValueError("v, slots and scales go with k_cache and v_cache")
+        q, k, inv_freq = _rows16(q), _rows16(k), inv_freq.contiguous()
+        q_weight, k_weight = (None if w is None else w.contiguous().clone() if w.data_ptr() % 16 else w.contiguous() for w in (q_weight, k_weight))
+        q_out = torch.empty((tokens, heads, dim), dtype=q.dtype, device=dev)
+        k_out = torch.empty((tokens, kv_heads, dim), dtype=q.dtype, device=dev) if desc is None else None
+        check(lib.cachalot_qk_norm_rope(_ptr(q), q.stride(0), q.stride(1), _ptr(k), k.stride(0), k.stride(1), _ptr(v), v.stride(0) if v is not None else 0,
+                                        v.stride(1) if v is not None else 0, _DT[q.dtype], tokens, heads, kv_heads, dim, _ptr(q_weight), _ptr(k_weight),
+                                        _DT[w_dtype] if w_dtype is not None else _DT[q.dtype], eps, _ptr(pos), _ptr(inv_freq), 2 * inv_freq.numel(),
+                                        int(interleaved), magnitude, _ptr(q_out), _ptr(k_out), None if desc is None else C.byref(desc), _ptr(slots),
+                                        _ptr(status), _stream(dev)))
+    return q_out, k_out

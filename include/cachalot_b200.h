@@ -392,6 +392,24 @@ CACHALOT_API int cachalot_plan_pages(const int32_t* context_lens, const int32_t*
                         int page_size, int tokens, int32_t* starts, int32_t* request_of, int32_t* positions, int32_t* slots,
                         int32_t* lens, int32_t* free_count_out, int* status, cachalot_stream_t stream);
 
+/* Replaces model/norm_rope_mlx.py and the rope_1d kernels of model/decode_fused_metal.py:43 (one token, then a cache
+ * append): for every new token, RMS norm of each query and key head (q_weight, k_weight [head_dim] in `dtype` or f32; NULL:
+ * no norm), rotation of the first rotary_dim elements by the token's position, rounding, and the write of keys and values
+ * to slots[token] of the cache.  q [tokens, heads, head_dim], k and v [tokens, kv_heads, head_dim] in `dtype` (CACHALOT_F16
+ * or CACHALOT_BF16), rows 16-byte aligned, strides in elements; inv_freq f64 [rotary_dim/2], radians per position;
+ * interleaved: pairs (2i, 2i+1), else (i, i + rotary_dim/2); magnitude: factor of the rotated elements (1; more where
+ * long-context scaling asks for it).  q_out [tokens, heads, head_dim] and, if not NULL, k_out [tokens, kv_heads, head_dim]
+ * are contiguous and may not overlap an input.  cache NULL: v and slots are not read.  A negative slot (padding) is not stored, one past the
+ * cache neither (CACHALOT_STATUS_SLOT_RANGE); two tokens of a call must not share one.  E4M3 caches get value / scale,
+ * saturated at +-448.  head_dim a multiple of 8 up to 256. */
+CACHALOT_API int cachalot_qk_norm_rope(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k,
+                          int64_t k_token_stride, int64_t k_head_stride, const void* v, int64_t v_token_stride,
+                          int64_t v_head_stride, int dtype, int tokens, int heads, int kv_heads, int head_dim,
+                          const void* q_weight, const void* k_weight, int w_dtype, float eps, const int32_t* positions,
+                          const double* inv_freq, int rotary_dim, int interleaved, float magnitude, void* q_out, void* k_out,
+                          const cachalot_paged_kv* cache /* host, or NULL */, const int32_t* slots, int* status,
+                          cachalot_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

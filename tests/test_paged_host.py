@@ -33,3 +33,56 @@ def test_cpu_tensors_are_refused():
     t = torch.zeros(2, dtype=torch.int32)
     with pytest.raises(ValueError, match="CUDA tensors"):
         cb.plan_pages(t, t, t.reshape(2, 1), t, t[:1], page_size=16, tokens=2)
+
+
+def test_rope_frequencies():
+    import cachalot_b200 as cb
+
+    f, m = cb.rope_frequencies(64, device="cpu")
+    assert m == 1.0 and f.dtype == torch.float64 and f.tolist() == [10000.0 ** (-2 * i / 64) for i in range(32)]
+    assert torch.allclose(cb.rope_frequencies(64, scaling="linear", factor=4.0, device="cpu")[0], f / 4, rtol=1e-15)
+    g, _ = cb.rope_frequencies(64, scaling="ntk", factor=4.0, device="cpu")
+    assert g[0] == 1.0 and abs(float(g[-1] / f[-1]) - 0.25) < 1e-12
+    y, m = cb.rope_frequencies(64, scaling="yarn", factor=32.0, trained_len=4096, device="cpu")
+    assert abs(m - (0.1 * 3.4657359027997265 + 1)) < 1e-12
+    turns = f * 4096 / (2 * 3.141592653589793)
+    assert torch.equal(y[turns > 33], f[turns > 33]) and torch.allclose(y[turns < 0.75], f[turns < 0.75] / 32, rtol=1e-12)
+    assert (y <= f).all() and (y >= f / 32 * (1 - 1e-12)).all()
+    for kw in (dict(rotary_dim=3), dict(rotary_dim=0), dict(rotary_dim=8, scaling="other"), dict(rotary_dim=8, factor=0.5), dict(rotary_dim=8, scaling="yarn", factor=2.0)):
+        with pytest.raises(ValueError):
+            cb.rope_frequencies(**kw, device="cpu")
+
+
+def test_qk_norm_rope_refusals():
+    from cachalot_b200 import _lib
+
+    buf = (C.c_int32 * 4096)()
+    base = C.addressof(buf) + (-C.addressof(buf)) % 16
+    lib, p = _lib.lib, C.c_void_p(base)
+
+    def cache(**kw):
+        d = _lib.PagedKV()
+        d.k = d.v = base
+        d.k_page_stride = d.v_page_stride = 256
+        d.k_head_stride, d.v_head_stride = 128, 128
+        d.k_token_stride, d.v_token_stride = 64, 64
+        d.n_pages, d.page_size, d.kv_heads, d.head_dim, d.dtype = 2, 2, 2, 64, _lib.BF16
+        for k, v in kw.items():
+            setattr(d, k, v)
+        return d
+
+    def call(q=p, qs=128, dtype=_lib.BF16, tokens=1, heads=2, kv=2, dim=64, w=None, wdt=_lib.BF16, pos=p, rot=64, out=p, ko=None, d=None, slots=p, none=False):
+        d = None if none else C.byref(d or cache())
+        return lib.cachalot_qk_norm_rope(q, qs, 64, p, 128, 64, p, 128, 64, dtype, tokens, heads, kv, dim, w, w, wdt, 1e-6, pos, p, rot, 0, 1.0, out, ko, d, slots,
+                                         None, None)
+
+    odd = C.c_void_p(base + 8)
+    for kw, rc, word in ((dict(tokens=-1), _lib.EINVAL, "shape"), (dict(dtype=_lib.F32), _lib.EINVAL, "float16"), (dict(dim=264), _lib.EUNSUPPORTED, "264"),
+                         (dict(rot=3), _lib.EINVAL, "rotary"), (dict(rot=66), _lib.EINVAL, "rotary"), (dict(w=p, wdt=_lib.F16), _lib.EINVAL, "weights"),
+                         (dict(none=True), _lib.EINVAL, "nowhere"), (dict(pos=None), _lib.EINVAL, "null"), (dict(q=odd), _lib.EALIGN, "16-byte"),
+                         (dict(qs=12), _lib.EALIGN, "16-byte"), (dict(out=odd), _lib.EALIGN, "16-byte"), (dict(slots=None), _lib.EINVAL, "slots"),
+                         (dict(d=cache(k=None)), _lib.EINVAL, "null"), (dict(d=cache(dtype=_lib.F32)), _lib.EINVAL, "cache"),
+                         (dict(d=cache(dtype=_lib.F16)), _lib.EINVAL, "differ"), (dict(d=cache(kv_heads=1)), _lib.EINVAL, "holds"),
+                         (dict(d=cache(k_token_stride=63)), _lib.EALIGN, "strides"), (dict(d=cache(v_page_stride=-64)), _lib.EALIGN, "strides"),
+                         (dict(d=cache(n_pages=2 ** 30)), _lib.EUNSUPPORTED, "slots"), (dict(d=cache(n_pages=0)), _lib.EINVAL, "empty")):
+        assert call(**kw) == rc and word in _lib.last_error(), (kw, _lib.last_error())
