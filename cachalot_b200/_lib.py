@@ -99,6 +99,8 @@ SIGNATURES = {
     "cachalot_plan_pages": (_i, [_vp, _vp, _i, _vp, _i64, _i, _vp, _i, _vp, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
     "cachalot_qk_norm_rope": (_i, [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _i, _i, _i, _i, _i, _vp, _vp, _i, _f, _vp, _vp, _i, _i, _f,
                                    _vp, _vp, C.POINTER(PagedKV), _vp, _vp, _vp]),
+    "cachalot_paged_attention_workspace_bytes": (_sz, [_i, _i, _i, _i]),
+    "cachalot_paged_attention": (_i, [_vp, _i64, _i64, _i, _i, _i, C.POINTER(PagedKV), _vp, _i64, _i, _vp, _f, _i, _f, _vp, _sz, _vp, _i, _vp, _vp, _vp]),
     "cachalot_moe_prefill": (_i, [_vp, _desc, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _f, _i, _vp, _sz, _vp, _vp, _vp]),
 }
 

@@ -29,7 +29,8 @@ using at::ScalarType;
 #define ENTRIES(X) \
   X(cachalot_bf16_gemv_f32) X(cachalot_fp8_linear) X(cachalot_group_rows) X(cachalot_group_rows_scratch_ints) \
   X(cachalot_last_error) X(cachalot_moe_decode) X(cachalot_moe_decode_workspace_bytes) X(cachalot_moe_layer_decode) \
-  X(cachalot_moe_layer_decode_workspace_bytes) X(cachalot_moe_prefill) X(cachalot_moe_prefill_experts_workspace_bytes) X(cachalot_plan_pages) \
+  X(cachalot_moe_layer_decode_workspace_bytes) X(cachalot_moe_prefill) X(cachalot_moe_prefill_experts_workspace_bytes) X(cachalot_paged_attention) \
+  X(cachalot_paged_attention_workspace_bytes) X(cachalot_plan_pages) \
   X(cachalot_qk_norm_rope) \
   X(cachalot_route_topk) \
   X(cachalot_router_logits) X(cachalot_shared_expert) X(cachalot_shared_expert_workspace_bytes)
@@ -517,9 +518,44 @@ PyObject* qk_norm_rope(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   END_HANDLE_TH_ERRORS
 }
 
+// (q, k_cache, v_cache, block_table, lens, scale, window, softcap, k_scale | None, v_scale | None, out dtype, want_lse, status | None)
+//  -> out, or (out, lse)
+PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+  HANDLE_TH_ERRORS
+  PLAIN_OR_NONE(bound && n_args == 13);
+  Args p{a};
+  const at::Tensor *q = tensor_of(a[0]), *table = tensor_of(a[3]), *lens = tensor_of(a[4]);
+  PLAIN_OR_NONE(q && q->is_cuda());
+  const int dev = current_device();
+  const double scale = p.f(5), softcap = p.f(7);
+  const int window = (int)p.i(6), odt = (int)p.i(10), want = PyObject_IsTrue(a[11]);
+  const ScalarType dt = q->scalar_type();
+  PLAIN_OR_NONE(!p.bad && want >= 0 && (dt == ScalarType::Half || dt == ScalarType::BFloat16) && q->get_device() == dev && q->dim() == 3 && q->stride(2) == 1);
+  PLAIN_OR_NONE(q->stride(0) % 2 == 0 && q->stride(1) % 2 == 0 && reinterpret_cast<uintptr_t>(q->data_ptr()) % 4 == 0);
+  const int64_t requests = q->size(0), heads = q->size(1), dim = q->size(2);
+  PLAIN_OR_NONE(requests > 0 && requests < (1LL << 30) && heads > 0 && heads < (1 << 20) && odt >= CACHALOT_F16 && odt <= CACHALOT_F32 && window >= 0);
+  cachalot_paged_kv cache;
+  PLAIN_OR_NONE(cache_from(tensor_of(a[1]), tensor_of(a[2]), a[8], a[9], dev, &cache) && cache.head_dim == dim && heads % cache.kv_heads == 0);
+  PLAIN_OR_NONE(table_of(table, requests, dev) && plain_ints(lens, requests, dev));
+  PLAIN_OR_NONE(none_or_plain(a[12], ScalarType::Int, dev) && (a[12] == Py_None || tensor_of(a[12])->numel() > 0));
+  const size_t need = lib.cachalot_paged_attention_workspace_bytes((int)heads, cache.kv_heads, (int)dim, cache.dtype);
+  PLAIN_OR_NONE(need > 0);
+  const at::Tensor ws = scratch(need, dev);
+  at::Tensor y = empty({requests, heads, dim}, odt == CACHALOT_F16 ? ScalarType::Half : out_type(odt), dev), lse;
+  if (want) lse = empty({requests, heads}, ScalarType::Float, dev);
+  const int rc = UNLOCKED(lib.cachalot_paged_attention(
+      q->data_ptr(), q->stride(0), q->stride(1), element_code(dt), (int)requests, (int)heads, &cache, ints(*table), table->stride(0), (int)table->size(1),
+      ints(*lens), (float)scale, window, (float)softcap, ws.data_ptr(), need, y.data_ptr(), odt, want ? static_cast<float*>(lse.data_ptr()) : nullptr,
+      static_cast<int*>(ptr_or_null(a[12])), current_stream(dev)));
+  if (rc) return raise(rc);
+  if (!want) return THPVariable_Wrap(std::move(y));
+  return Py_BuildValue("(NN)", THPVariable_Wrap(std::move(y)), THPVariable_Wrap(std::move(lse)));
+  END_HANDLE_TH_ERRORS
+}
+
 #define FAST(name) {#name, (PyCFunction)(void (*)(void))name, METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {FAST(entries), FAST(bind), FAST(fp8_linear), FAST(bf16_gemv_f32), FAST(shared_expert), FAST(moe_forward), FAST(layer_decode),
-                         FAST(prefill_grouped), FAST(moe_block), FAST(plan_pages), FAST(qk_norm_rope), {nullptr, nullptr, 0, nullptr}};
+                         FAST(prefill_grouped), FAST(moe_block), FAST(plan_pages), FAST(qk_norm_rope), FAST(paged_attention), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", "Native call path of the operators (see host.cpp).", -1, methods};
 
 }  // namespace

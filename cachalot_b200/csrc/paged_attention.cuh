@@ -1,0 +1,608 @@
+// Attention of one new token per request over a paged key-value cache: the kernel, instantiated per cache type in
+// paged_attention_{bf16,f16,e4m3}.cu.
+//
+//   s_j = scale * q . k_j   (cap * tanh(s / cap) with a soft cap),  j in [max(0, len - window), len)
+//   out = sum_j 2^(s_j log2 e - m) v_j / sum_j 2^(s_j log2 e - m),  m a running maximum
+//
+// HBM-bound: every visible key and value is read once for the G query heads that share it, 2 G FLOP per byte of a 16-bit
+// cache.  On CUDA cores G = 8 would already need the whole fp32 rate; the legacy warp MMA (m16n8k16) has ten times the
+// arithmetic this needs and, unlike tcgen05, takes its operands from registers, so nothing is staged:
+//   * a warp works on tiles of 16 tokens.  S^T = K Q^T has the tokens as MMA rows and 8 query heads as columns, O^T = V^T P^T
+//     the head's elements as rows and the 8 heads as columns: no row of an MMA is spent on padding for G = 8.
+//   * the order of the reduction index is free, so a lane's 16-byte loads of a key row ARE its operand fragments; for the
+//     values, whose fragments pair two tokens, one byte permute per register pairs the words of two rows.
+//   * keys of the next tile are requested when the scores are done, its values when the products are: 4 to 8 KB in
+//     flight per warp, 12 to 16 warps per SM.
+//   * S^T fragments become P^T fragments by one movmatrix each.
+//   * the running maximum moves only when a score exceeds it by more than 2^8 (one vote per tile instead of six shuffles
+//     and a rescaling); P stays below 2^8 in bf16, and is shifted by 2^7 in f16 to use that type's range.
+// Work is cut on the device, where the lengths are: the steps (64 tokens of one request and key-value head) of the whole
+// batch are numbered through and every CTA takes an equal run of them, so a batch of very different lengths is balanced
+// and one long request fills the GPU.  A CTA merges its four warps in shared memory; a unit (request, head) that lies in
+// one CTA is finished there, a unit that crosses CTAs leaves (m, l, O) of each part for the join kernel.
+#pragma once
+#include "paged.cuh"
+
+namespace cachalot {
+
+constexpr int PA_THREADS = 128, PA_WARPS = 4, PA_STEP = 64, PA_TILE = 16;
+
+struct AttendArgs {
+  const void* q;
+  long long q_row, q_head;  // elements
+  int q_bf16;
+  PagedView c;
+  const int32_t* table;
+  long long table_stride;
+  int width;
+  const int32_t* lens;
+  int requests, heads, group;      // group: query heads per key-value head
+  int tiles, head_blocks;          // head tiles (of 8 NT heads) a CTA's warps are split over; units per key-value head
+  int page_shift;                  // log2(page_size / 8) or -1; tokens one by one where the page size is no multiple of 8
+  int min_steps;
+  float scale, softcap;
+  int window;
+  float* part_o;                   // [ctas][2][heads of a unit][dim]
+  float2* part_ml;                 // [ctas][2][heads of a unit]
+  int4* parts;                     // [ctas][2]: request, key-value head * head_blocks + block, first CTA, CTAs (0: none)
+  void* out;
+  int out_dtype;
+  float* lse;
+  int* status;
+};
+
+constexpr float PA_LOG2E = 1.4426950408889634f, PA_LN2 = 0.6931471805599453f;
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+template <typename M>
+__device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  if constexpr (std::is_same<M, __half>::value)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+template <typename M>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  if constexpr (std::is_same<M, __half>::value) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  } else {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+}
+__device__ __forceinline__ uint32_t movmatrix(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+// two E4M3 codes (low half of `x`) -> two f16
+__device__ __forceinline__ uint32_t e4m3x2_f16x2(uint32_t x) {
+  uint32_t y;
+  asm("{\n.reg .b16 l, h;\nmov.b32 {l, h}, %1;\ncvt.rn.f16x2.e4m3x2 %0, l;\n}" : "=r"(y) : "r"(x));
+  return y;
+}
+
+// B bytes per load (16, 8 or 4), W words in all, loads STRIDE bytes apart
+template <int B, int W, int STRIDE, bool KEEP>
+__device__ __forceinline__ void load_words(uint32_t (&r)[W], const uint8_t* p) {
+#pragma unroll
+  for (int c = 0; c < W * 4 / B; ++c) {
+    const uint8_t* at = p + c * STRIDE;
+    if constexpr (B == 16) {
+      const uint4 v = KEEP ? __ldg(reinterpret_cast<const uint4*>(at)) : ld_stream_u4(at);
+      r[c * 4] = v.x, r[c * 4 + 1] = v.y, r[c * 4 + 2] = v.z, r[c * 4 + 3] = v.w;
+    } else if constexpr (B == 8) {
+      const uint2 v = KEEP ? __ldg(reinterpret_cast<const uint2*>(at)) : ld_stream_u2(at);
+      r[c * 2] = v.x, r[c * 2 + 1] = v.y;
+    } else {
+      r[c] = KEEP ? __ldg(reinterpret_cast<const uint32_t*>(at)) : ld_stream_u32(at);
+    }
+  }
+}
+
+// Geometry of one instantiation: what a lane holds of a key row (a quarter of it) and of a value row (an eighth).
+template <bool F8, int D, int NT>
+struct AttendShape {
+  static constexpr int ES = F8 ? 1 : 2;
+  static constexpr int KBYTES = D * ES / 4, VBYTES = D * ES / 8;
+  static constexpr int KB = KBYTES % 16 == 0 ? 16 : 8;
+  static constexpr int VB = VBYTES % 16 == 0 ? 16 : VBYTES % 8 == 0 ? 8 : 4;
+  static constexpr int KW = KBYTES / 4, VW = VBYTES / 4;
+  static constexpr int KSTEPS = D / 16;                 // MMAs over the head's elements = MMA row tiles of O^T
+  static constexpr int TILE_HEADS = 8 * NT;
+  static constexpr int O_PITCH = D + 4;
+  // element of the head at which lane quad t's key word w starts / lane row g's value word w
+  static constexpr __host__ __device__ int k_dim(int w, int t) { return (w / (KB / 4) * (4 * KB) + t * KB + w % (KB / 4) * 4) / ES; }
+  static constexpr __host__ __device__ int v_dim(int w, int g) { return (w / (VB / 4) * (8 * VB) + g * VB + w % (VB / 4) * 4) / ES; }
+  static constexpr int Q_BYTES(int tiles) { return tiles * NT * KSTEPS * 32 * 8; }
+  static constexpr int SMEM(int tiles) { return Q_BYTES(tiles) + PA_WARPS * TILE_HEADS * (O_PITCH * 4 + 8) + 4 * TILE_HEADS * 4; }
+  static constexpr int MAX_TILES = 4;
+  // CTAs per SM that the registers are cut for
+  static constexpr int CTAS = D * NT <= 64 ? 4 : D * NT <= 128 ? 3 : 2;
+};
+
+struct Span {  // what is visible of a request
+  int lo, len, first_tile, steps;
+};
+__device__ __forceinline__ Span span_of(const AttendArgs& a, int r) {
+  const long long room = (long long)a.width * a.c.page_size;
+  const int n = a.lens[r];
+  Span s;
+  s.len = (int)min((long long)max(n, 0), room);
+  s.lo = a.window > 0 ? max(0, s.len - a.window) : 0;
+  s.first_tile = s.lo / PA_TILE;
+  s.steps = s.len > 0 ? (s.len - s.first_tile * PA_TILE + PA_STEP - 1) / PA_STEP : 0;
+  return s;
+}
+
+__device__ __forceinline__ void store_out(void* out, int dtype, long long at, float v) {
+  if (dtype == CACHALOT_F32) static_cast<float*>(out)[at] = v;
+  else if (dtype == CACHALOT_BF16) static_cast<__nv_bfloat16*>(out)[at] = __float2bfloat16_rn(v);
+  else static_cast<__half*>(out)[at] = __float2half_rn(v);
+}
+
+template <typename M, bool F8, int D, int NT, bool PAGE8, bool KEEP>
+__global__ void __launch_bounds__(PA_THREADS, AttendShape<F8, D, NT>::CTAS) attend_kernel(const AttendArgs a) {
+  using S = AttendShape<F8, D, NT>;
+  constexpr bool HALF = std::is_same<M, __half>::value;
+  constexpr float SHIFT = HALF ? 7.f : 0.f, SLACK = 8.f;
+  extern __shared__ __align__(16) uint8_t smem[];
+  uint2* sq = reinterpret_cast<uint2*>(smem);                                        // [tiles * NT][KSTEPS][32]
+  float* so = reinterpret_cast<float*>(smem + S::Q_BYTES(a.tiles));                  // [warps][TILE_HEADS][O_PITCH]
+  float2* sml = reinterpret_cast<float2*>(so + PA_WARPS * S::TILE_HEADS * S::O_PITCH);  // [warps][TILE_HEADS]
+  float* sexp = reinterpret_cast<float*>(sml + PA_WARPS * S::TILE_HEADS);            // [tiles * TILE_HEADS] scale of the query
+  __shared__ long long sums[PA_WARPS];
+  __shared__ long long found_at;
+  __shared__ int found;
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
+  const int per_request = a.c.kv_heads * a.head_blocks;
+  int flags = 0;
+
+  // ---- which steps are this CTA's ----
+  long long mine = 0;
+  for (int r = tid; r < a.requests; r += PA_THREADS) {
+    mine += span_of(a, r).steps;
+    const int n = a.lens[r];
+    if (n < 0 || n > (long long)a.width * a.c.page_size) flags |= CACHALOT_STATUS_LENGTH;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
+  if (lane == 0) sums[warp] = mine;
+  if (tid == 0) found = -1;
+  __syncthreads();
+  long long total = 0;
+#pragma unroll
+  for (int w = 0; w < PA_WARPS; ++w) total += sums[w];
+  total *= per_request;
+  long long per = (total + gridDim.x - 1) / gridDim.x;
+  if (per < a.min_steps) per = a.min_steps;
+  const long long begin = per * blockIdx.x, end = min(begin + per, total);
+  long long before = 0;
+  if (begin < end) {
+    for (int r0 = 0; r0 < a.requests; r0 += PA_THREADS) {
+      const int r = r0 + tid;
+      const long long own = r < a.requests ? (long long)span_of(a, r).steps * per_request : 0;
+      long long v = own;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const long long u = __shfl_up_sync(0xffffffffu, v, o);
+        if (lane >= o) v += u;
+      }
+      __syncthreads();
+      if (lane == 31) sums[warp] = v;
+      __syncthreads();
+#pragma unroll
+      for (int w = 0; w < PA_WARPS; ++w) v += w < warp ? sums[w] : 0;
+      v += before;
+      if (begin >= v - own && begin < v) found = r, found_at = v - own;
+#pragma unroll
+      for (int w = 0; w < PA_WARPS; ++w) before += sums[w];
+      __syncthreads();
+      if (found >= 0) break;
+    }
+  }
+
+  // ---- rows without a visible key ----
+  for (int r = blockIdx.x; r < a.requests; r += gridDim.x) {
+    if (span_of(a, r).steps) continue;
+    for (int i = tid; i < a.heads * D; i += PA_THREADS) store_out(a.out, a.out_dtype, (long long)r * a.heads * D + i, 0.f);
+    if (a.lse)
+      for (int i = tid; i < a.heads; i += PA_THREADS) a.lse[(long long)r * a.heads + i] = -INFINITY;
+  }
+  if (tid < 2) a.parts[blockIdx.x * 2 + tid] = make_int4(0, 0, 0, 0);
+  __syncthreads();
+  if (begin >= end || found < 0) {
+    if (a.status && flags) atomicOr(a.status, flags);
+    return;
+  }
+
+  int r = found;
+  Span sp = span_of(a, r);
+  int unit = (int)((begin - found_at) / sp.steps), step0 = (int)((begin - found_at) % sp.steps);
+  const int mt = warp % a.tiles, slice = warp / a.tiles, slices = PA_WARPS / a.tiles;
+  const int unit_heads = a.tiles * S::TILE_HEADS;
+
+  for (long long at = begin; at < end;) {
+    const int steps = (int)min((long long)(sp.steps - step0), end - at);
+    const int h = unit / a.head_blocks, block = unit % a.head_blocks;
+    const int head0 = block * unit_heads, heads = min(unit_heads, a.group - head0);  // within the group
+    const long long row0 = (long long)r * a.heads + (long long)h * a.group + head0;  // first output row of the unit
+
+    // ---- the query heads as MMA fragments ----
+    if constexpr (F8) {  // f16 from here on: a bf16 head is brought into range by a power of two
+      for (int i = warp; i < unit_heads; i += PA_WARPS) {
+        float top = 0.f;
+        if (i < heads && a.q_bf16) {
+          const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(a.q) + r * a.q_row + (long long)(h * a.group + head0 + i) * a.q_head;
+          for (int d = lane; d < D; d += 32) top = fmaxf(top, fabsf(__bfloat162float(q[d])));
+          top = warp_max(top);
+        }
+        const int e = (int)((__float_as_uint(top) >> 23) & 255) - 127;
+        if (lane == 0) sexp[i] = top > 0.f ? pow2f(max(-126, min(126, e))) : 1.f;
+      }
+      __syncthreads();
+    }
+    for (int i = tid; i < a.tiles * NT * S::KSTEPS * 32; i += PA_THREADS) {
+      const int l = i & 31, ks = (i >> 5) % S::KSTEPS, head = (i >> 5) / S::KSTEPS * 8 + (l >> 2);
+      const int d0 = F8 ? S::k_dim(ks, l & 3) : S::k_dim(2 * ks, l & 3), d1 = F8 ? d0 + 2 : S::k_dim(2 * ks + 1, l & 3);
+      uint2 f = make_uint2(0, 0);
+      if (head < heads) {
+        const uint16_t* q = static_cast<const uint16_t*>(a.q) + r * a.q_row + (long long)(h * a.group + head0 + head) * a.q_head;
+        f.x = *reinterpret_cast<const uint32_t*>(q + d0), f.y = *reinterpret_cast<const uint32_t*>(q + d1);
+        if (F8 && a.q_bf16) {
+          const float inv = 1.f / sexp[head];  // a power of two
+          f.x = pack2<__half>(__uint_as_float(f.x << 16) * inv, __uint_as_float(f.x & 0xffff0000u) * inv);
+          f.y = pack2<__half>(__uint_as_float(f.y << 16) * inv, __uint_as_float(f.y & 0xffff0000u) * inv);
+        }
+      }
+      sq[i] = f;
+    }
+    __syncthreads();
+
+    // scores in units of log2: s * f, or cap' - 2 cap' / (1 + 2^(s * f)) = cap' * tanh
+    float hs[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        float f = a.softcap > 0.f ? a.scale / a.softcap * (2.f * PA_LOG2E) : a.scale * PA_LOG2E;
+        if constexpr (F8) f *= sexp[(mt * NT + n) * 8 + 2 * t4 + c] * (a.c.k_scale ? a.c.k_scale[h] : 1.f);
+        hs[n][c] = f;
+      }
+    const float cap = a.softcap * PA_LOG2E;
+
+    // ---- this warp's tiles ----
+    const uint8_t* kbase = a.c.k + h * a.c.k_head + t4 * S::KB;
+    const uint8_t* vbase = a.c.v + h * a.c.v_head + g * S::VB;
+    const int32_t* pages = a.table + r * a.table_stride;
+    const int tile_end = min(sp.first_tile + (step0 + steps) * (PA_STEP / PA_TILE), (sp.len + PA_TILE - 1) / PA_TILE);
+    float o[S::KSTEPS][NT][4];
+    float m[NT][2], base[NT][2], l[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+      for (int c = 0; c < 2; ++c) m[n][c] = -INFINITY, base[n][c] = 0.f, l[n][c] = 0.f;
+#pragma unroll
+      for (int k = 0; k < S::KSTEPS; ++k)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) o[k][n][c] = 0.f;
+    }
+    uint32_t kr[2][S::KW], vr[4][S::VW];
+
+    // page of a token, -1 where the table names none of the cache's
+    auto page_of = [&](int token, int index) {
+      if (token >= sp.len) return -1;
+      const int p = pages[index];
+      if ((unsigned)p < (unsigned)a.c.n_pages) return p;
+      flags |= CACHALOT_STATUS_SLOT_RANGE;
+      return -1;
+    };
+    struct Place {  // where a tile lies: page and place in it of its two halves of 8 tokens (pages of 8 k tokens)
+      int tile, page[2], off[2];
+      bool full;
+    };
+    auto locate = [&](int tile) {
+      Place p;
+      p.tile = tile;
+      p.full = tile * PA_TILE >= sp.lo && (tile + 1) * PA_TILE <= sp.len;
+      if constexpr (PAGE8) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int token = tile * PA_TILE + 8 * i;
+          const int index = a.page_shift >= 0 ? (token >> 3) >> a.page_shift : token / a.c.page_size;
+          p.off[i] = token - index * a.c.page_size;
+          p.page[i] = token + 8 <= sp.lo ? -1 : page_of(token, index);
+          p.full = p.full && p.page[i] >= 0;
+        }
+      } else {
+        p.full = false;
+      }
+      return p;
+    };
+    // place of token `half * 8 + i` of a tile: true and its page and offset if it is visible
+    auto token_at = [&](const Place& p, int half, int i, int& page, int& off) {
+      const int token = p.tile * PA_TILE + half * 8 + i;
+      bool ok = token >= sp.lo && token < sp.len;
+      if constexpr (PAGE8) {
+        page = p.page[half], off = p.off[half] + i;
+        return ok && page >= 0;
+      } else {
+        if (!ok) return false;
+        const int index = token / a.c.page_size;
+        page = page_of(token, index), off = token - index * a.c.page_size;
+        return page >= 0;
+      }
+    };
+    int seen = 0;  // bit i: key row g + 8 i of the tile in `kr` is visible
+    auto load_k = [&](const Place& p) {
+      seen = 3;
+      if (p.full) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          load_words<S::KB, S::KW, 4 * S::KB, KEEP>(kr[i], kbase + p.page[i] * a.c.k_page + (p.off[i] + g) * a.c.k_token);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          int page, off;
+          if (token_at(p, i, g, page, off)) {
+            load_words<S::KB, S::KW, 4 * S::KB, KEEP>(kr[i], kbase + page * a.c.k_page + off * a.c.k_token);
+          } else {
+            seen &= ~(1 << i);
+#pragma unroll
+            for (int w = 0; w < S::KW; ++w) kr[i][w] = 0;
+          }
+        }
+      }
+    };
+    auto load_v = [&](const Place& p) {  // rows 2 t4, 2 t4 + 1 of either half; what is hidden must be zero, 0 * NaN is not
+      if (p.full) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          load_words<S::VB, S::VW, 8 * S::VB, KEEP>(vr[i], vbase + p.page[i >> 1] * a.c.v_page + (p.off[i >> 1] + 2 * t4 + (i & 1)) * a.c.v_token);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          int page, off;
+          if (token_at(p, i >> 1, 2 * t4 + (i & 1), page, off)) {
+            load_words<S::VB, S::VW, 8 * S::VB, KEEP>(vr[i], vbase + page * a.c.v_page + off * a.c.v_token);
+          } else {
+#pragma unroll
+            for (int w = 0; w < S::VW; ++w) vr[i][w] = 0;
+          }
+        }
+      }
+    };
+
+    int tile = sp.first_tile + step0 * (PA_STEP / PA_TILE) + slice;
+    Place next;
+    if (tile < tile_end) {
+      const Place p = locate(tile);
+      load_k(p), load_v(p);
+      if (tile + slices < tile_end) next = locate(tile + slices);
+    }
+    const uint2* q = sq + mt * NT * S::KSTEPS * 32 + lane;
+    for (; tile < tile_end; tile += slices) {
+      const bool more = tile + slices < tile_end;
+      float s[NT][4];
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) s[n][c] = 0.f;
+#pragma unroll
+      for (int k = 0; k < S::KSTEPS; ++k) {
+        uint32_t a0, a1, a2, a3;
+        if constexpr (F8) {
+          a0 = e4m3x2_f16x2(kr[0][k]), a1 = e4m3x2_f16x2(kr[1][k]);
+          a2 = e4m3x2_f16x2(kr[0][k] >> 16), a3 = e4m3x2_f16x2(kr[1][k] >> 16);
+        } else {
+          a0 = kr[0][2 * k], a1 = kr[1][2 * k], a2 = kr[0][2 * k + 1], a3 = kr[1][2 * k + 1];
+        }
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          const uint2 b = q[(n * S::KSTEPS + k) * 32];
+          mma16816<M>(s[n], a0, a1, a2, a3, b.x, b.y);
+        }
+      }
+      const int visible = seen;
+      if (more) load_k(next);
+      bool higher = false;
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          float x = s[n][c] * hs[n][c & 1];
+          if (a.softcap > 0.f) x = cap - __fdividef(2.f * cap, 1.f + ex2(x));
+          s[n][c] = visible >> (c >> 1) & 1 ? x : -INFINITY;
+        }
+        higher = higher || fmaxf(s[n][0], s[n][2]) > m[n][0] + SLACK || fmaxf(s[n][1], s[n][3]) > m[n][1] + SLACK;
+      }
+      if (__any_sync(0xffffffffu, higher)) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            float top = fmaxf(s[n][c], s[n][c + 2]);
+#pragma unroll
+            for (int x = 4; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+            const float now = fmaxf(m[n][c], top);
+            const float keep = now == -INFINITY ? 1.f : ex2(m[n][c] - now);  // m still -inf: 0
+            m[n][c] = now, base[n][c] = now == -INFINITY ? 0.f : now - SHIFT;
+            l[n][c] *= keep;
+#pragma unroll
+            for (int k = 0; k < S::KSTEPS; ++k) o[k][n][c] *= keep, o[k][n][c + 2] *= keep;
+          }
+      }
+      uint32_t pb[NT][2];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        float p[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) p[c] = ex2(s[n][c] - base[n][c & 1]);
+        l[n][0] += p[0] + p[2], l[n][1] += p[1] + p[3];
+        pb[n][0] = movmatrix(pack2<M>(p[0], p[1])), pb[n][1] = movmatrix(pack2<M>(p[2], p[3]));
+      }
+#pragma unroll
+      for (int w = 0; w < S::VW; ++w) {
+        if constexpr (F8) {
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const uint32_t x = __byte_perm(vr[0][w], vr[1][w], i ? 0x7362 : 0x5140), y = __byte_perm(vr[2][w], vr[3][w], i ? 0x7362 : 0x5140);
+            const uint32_t a0 = e4m3x2_f16x2(x), a1 = e4m3x2_f16x2(x >> 16), a2 = e4m3x2_f16x2(y), a3 = e4m3x2_f16x2(y >> 16);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) mma16816<M>(o[2 * w + i][n], a0, a1, a2, a3, pb[n][0], pb[n][1]);
+          }
+        } else {
+          const uint32_t a0 = __byte_perm(vr[0][w], vr[1][w], 0x5410), a1 = __byte_perm(vr[0][w], vr[1][w], 0x7632);
+          const uint32_t a2 = __byte_perm(vr[2][w], vr[3][w], 0x5410), a3 = __byte_perm(vr[2][w], vr[3][w], 0x7632);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) mma16816<M>(o[w][n], a0, a1, a2, a3, pb[n][0], pb[n][1]);
+        }
+      }
+      if (more) {
+        load_v(next);
+        if (tile + 2 * slices < tile_end) next = locate(tile + 2 * slices);
+      }
+    }
+
+    // ---- the four warps' parts of this run ----
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+#pragma unroll
+        for (int x = 4; x < 32; x <<= 1) l[n][c] += __shfl_xor_sync(0xffffffffu, l[n][c], x);
+        if (g == 0) sml[warp * S::TILE_HEADS + n * 8 + 2 * t4 + c] = make_float2(m[n][c], l[n][c]);
+      }
+    __syncthreads();
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const int row = n * 8 + 2 * t4 + c;
+        float top = -INFINITY;
+        for (int w = mt; w < PA_WARPS; w += a.tiles) top = fmaxf(top, sml[w * S::TILE_HEADS + row].x);
+        const float f = m[n][c] == -INFINITY ? 0.f : ex2(m[n][c] - top);
+        float* dst = so + (warp * S::TILE_HEADS + row) * S::O_PITCH;
+#pragma unroll
+        for (int w = 0; w < S::VW; ++w) {
+          if constexpr (F8)
+            *reinterpret_cast<float4*>(dst + S::v_dim(w, g)) =
+                make_float4(o[2 * w][n][c] * f, o[2 * w][n][c + 2] * f, o[2 * w + 1][n][c] * f, o[2 * w + 1][n][c + 2] * f);
+          else
+            *reinterpret_cast<float2*>(dst + S::v_dim(w, g)) = make_float2(o[w][n][c] * f, o[w][n][c + 2] * f);
+        }
+      }
+    __syncthreads();
+    const bool whole = step0 == 0 && steps == sp.steps;
+    const int which = step0 > 0 ? 0 : 1;
+    const long long slot = (long long)blockIdx.x * 2 + which;
+    const float v_scale = F8 && a.c.v_scale ? a.c.v_scale[h] : 1.f;
+    for (int i = tid; i < heads * (D / 4); i += PA_THREADS) {
+      const int head = i / (D / 4), d = i % (D / 4) * 4;
+      const int row = head % S::TILE_HEADS, from = head / S::TILE_HEADS;
+      float top = -INFINITY, sum = 0.f;
+      for (int w = from; w < PA_WARPS; w += a.tiles) top = fmaxf(top, sml[w * S::TILE_HEADS + row].x);
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int w = from; w < PA_WARPS; w += a.tiles) {
+        const float2 ml = sml[w * S::TILE_HEADS + row];
+        sum += ml.x == -INFINITY ? 0.f : ml.y * ex2(ml.x - top);
+        const float4 x = *reinterpret_cast<const float4*>(so + (w * S::TILE_HEADS + row) * S::O_PITCH + d);
+        v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
+      }
+      if (whole) {
+        const float inv = sum == 0.f ? 0.f : v_scale / sum;
+        const long long to = (row0 + head) * D + d;
+        store_out(a.out, a.out_dtype, to, v.x * inv), store_out(a.out, a.out_dtype, to + 1, v.y * inv);
+        store_out(a.out, a.out_dtype, to + 2, v.z * inv), store_out(a.out, a.out_dtype, to + 3, v.w * inv);
+        if (d == 0 && a.lse) a.lse[row0 + head] = sum == 0.f ? -INFINITY : (top - SHIFT + log2f(sum)) * PA_LN2;
+      } else {
+        *reinterpret_cast<float4*>(a.part_o + (slot * unit_heads + head) * D + d) = v;
+        if (d == 0) a.part_ml[slot * unit_heads + head] = make_float2(top, sum);
+      }
+    }
+    if (!whole && tid == 0) {
+      const long long first = at - step0;  // the unit's first step
+      const int c0 = (int)(first / per), c1 = (int)((first + sp.steps - 1) / per);
+      a.parts[slot] = make_int4(r, unit, c0, c1 - c0 + 1);
+    }
+    __syncthreads();
+    at += steps, step0 = 0;
+    if (at < end && ++unit == per_request) {
+      unit = 0;
+      do {
+        if (++r >= a.requests) return;  // not with lengths that stay as they are during the call
+        sp = span_of(a, r);
+      } while (sp.steps == 0);
+    }
+  }
+  if (a.status && flags) atomicOr(a.status, flags);
+}
+
+struct AttendLaunch {
+  int unit_heads, tiles, head_blocks, ctas_per_sm;
+};
+// head tiles and units of a group of query heads
+template <bool F8, int D, int NT>
+AttendLaunch attend_shape(int group) {
+  AttendLaunch l;
+  const int need = (group + 8 * NT - 1) / (8 * NT);
+  l.tiles = need >= 3 ? 4 : need;
+  l.unit_heads = l.tiles * 8 * NT;
+  l.head_blocks = (group + l.unit_heads - 1) / l.unit_heads;
+  l.ctas_per_sm = AttendShape<F8, D, NT>::CTAS;
+  return l;
+}
+// Up to 8 query heads per key-value head take one MMA column tile per warp, more take two where the registers hold them.
+template <bool F8, typename Fn>
+bool attend_dispatch(int dim, int group, Fn&& fn) {
+  auto go = [&](auto d, auto nt) { fn(d, nt, attend_shape<F8, decltype(d)::value, decltype(nt)::value>(group)); };
+  using std::integral_constant;
+  auto nt = [&](auto d) {
+    if constexpr (decltype(d)::value <= 128) {
+      if (group > 8) return go(d, integral_constant<int, 2>{});
+    }
+    go(d, integral_constant<int, 1>{});
+  };
+  switch (dim) {
+    case 64: nt(integral_constant<int, 64>{}); return true;
+    case 96: nt(integral_constant<int, 96>{}); return true;
+    case 128: nt(integral_constant<int, 128>{}); return true;
+    case 192: nt(integral_constant<int, 192>{}); return true;
+    case 256: nt(integral_constant<int, 256>{}); return true;
+    default: return false;
+  }
+}
+
+template <typename M, bool F8>
+int launch_attend(AttendArgs& a, int dim, int ctas, cudaStream_t stream) {
+  cudaError_t e = cudaSuccess;
+  attend_dispatch<F8>(dim, a.group, [&](auto d, auto nt, const AttendLaunch& l) {
+    constexpr int D = decltype(d)::value, NT = decltype(nt)::value;
+    using S = AttendShape<F8, D, NT>;
+    auto run = [&](auto kern) {
+      e = smem_optin_once(kern, S::SMEM(S::MAX_TILES));
+      if (e == cudaSuccess) kern<<<ctas, PA_THREADS, S::SMEM(l.tiles), stream>>>(a);
+    };
+    const bool page8 = a.c.page_size % 8 == 0;
+    if (page8 && l.tiles == 1) run(attend_kernel<M, F8, D, NT, true, false>);
+    else if (page8) run(attend_kernel<M, F8, D, NT, true, true>);
+    else run(attend_kernel<M, F8, D, NT, false, true>);
+  });
+  if (e != cudaSuccess) return fail(CACHALOT_ECUDA, "paged_attention: %s", cudaGetErrorString(e));
+  return check_launch("paged_attention");
+}
+
+int launch_attend_bf16(AttendArgs& a, int dim, int ctas, cudaStream_t stream);
+int launch_attend_f16(AttendArgs& a, int dim, int ctas, cudaStream_t stream);
+int launch_attend_e4m3(AttendArgs& a, int dim, int ctas, cudaStream_t stream);
+
+}  // namespace cachalot

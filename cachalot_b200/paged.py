@@ -54,7 +54,7 @@ def _block_table(t: torch.Tensor, rows: int) -> None:
         raise ValueError("block_table rows must be contiguous")
 
 
-_DT = {torch.float16: _lib.F16, torch.bfloat16: _lib.BF16, torch.float32: _lib.F32, torch.float8_e4m3fn: _lib.E4M3}
+_DT = {torch.float16: _lib.F16, torch.bfloat16: _lib.BF16, torch.float32: _lib.F32, torch.float8_e4m3fn: _lib.E4M3}  # of the C ABI
 
 
 def _cache(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale, v_scale) -> _lib.PagedKV:
@@ -218,3 +218,53 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_
                                         int(interleaved), magnitude, _ptr(q_out), _ptr(k_out), None if desc is None else C.byref(desc), _ptr(slots),
                                         _ptr(status), _stream(dev)))
     return q_out, k_out
+
+
+# ---- attention --------------------------------------------------------------------------------
+
+def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor, lens: torch.Tensor, *,
+                    scale: float | None = None, window: int = 0, softcap: float = 0.0, k_scale: torch.Tensor | None = None,
+                    v_scale: torch.Tensor | None = None, out_dtype: torch.dtype | None = None, want_lse: bool = False,
+                    status: torch.Tensor | None = None):
+    """One new token per request over its pages (grouped-query decode attention, minimax/gqa_decode.py:180-187):
+    q [requests, heads, dim] float16 or bfloat16, caches as `qk_norm_rope` fills them, block_table int32 [requests, width],
+    lens int32 [requests] = visible tokens, the new one among them.  Query head i reads key-value head
+    i // (heads // kv_heads); `scale` defaults to dim ** -0.5; softcap > 0: scores softcap * tanh(s / softcap); window > 0:
+    only the last `window` tokens.  Returns out [requests, heads, dim] in `out_dtype` (default: q's), with `want_lse` also
+    float32 [requests, heads] log sum exp of the scores.  A request of length 0 gives zeros and -inf; tokens whose table
+    entry is no page of the cache are hidden, lengths past the table cut (bits in `status`).  The lengths are read on the
+    device: nothing waits for them, and a captured call replays with new ones."""
+    if scale is None:
+        scale = q.shape[-1] ** -0.5
+    r = _host.paged_attention(q, k_cache, v_cache, block_table, lens, scale, window, softcap, k_scale, v_scale,
+                              _DT.get(q.dtype if out_dtype is None else out_dtype, -1), want_lse, status)
+    if r is not None:
+        return r
+    dev = _same_device(q, k_cache, v_cache, block_table, lens, k_scale, v_scale, status)
+    if q.dim() != 3:
+        raise ValueError(f"q must be [requests, heads, dim], got {tuple(q.shape)}")
+    if q.dtype not in (torch.float16, torch.bfloat16):
+        raise ValueError(f"q must be float16 or bfloat16, got {q.dtype}")
+    out_dtype = q.dtype if out_dtype is None else out_dtype
+    if out_dtype not in (torch.float16, torch.bfloat16, torch.float32):
+        raise ValueError(f"out_dtype must be float16, bfloat16 or float32, got {out_dtype}")
+    requests, heads, dim = q.shape
+    desc = _cache(k_cache, v_cache, k_scale, v_scale)
+    if desc.head_dim != dim:
+        raise ValueError(f"q has heads of {dim}, the cache of {desc.head_dim}")
+    _block_table(block_table, requests)
+    n = _ints(lens, "lens", (requests,))
+    _status(status)
+    if not 0 <= window < 2 ** 31:
+        raise ValueError(f"window must be in [0, 2**31), got {window}")
+    with torch.cuda.device(dev):
+        if q.stride(2) != 1 or q.stride(0) % 2 or q.stride(1) % 2 or q.data_ptr() % 4:
+            q = q.clone(memory_format=torch.contiguous_format)
+        out = torch.empty((requests, heads, dim), dtype=out_dtype, device=dev)
+        lse = torch.empty((requests, heads), dtype=torch.float32, device=dev) if want_lse else None
+        need = lib.cachalot_paged_attention_workspace_bytes(heads, desc.kv_heads, dim, desc.dtype)
+        ws = torch.empty(need, dtype=torch.uint8, device=dev)  # of this call: a captured graph keeps its own
+        check(lib.cachalot_paged_attention(_ptr(q), q.stride(0), q.stride(1), _DT[q.dtype], requests, heads, C.byref(desc), _ptr(block_table),
+                                           block_table.stride(0), block_table.shape[1], _ptr(n), scale, window, softcap, _ptr(ws), need, _ptr(out),
+                                           _DT[out_dtype], _ptr(lse), _ptr(status), _stream(dev)))
+    return (out, lse) if want_lse else out

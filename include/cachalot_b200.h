@@ -410,6 +410,24 @@ CACHALOT_API int cachalot_qk_norm_rope(const void* q, int64_t q_token_stride, in
                           const cachalot_paged_kv* cache /* host, or NULL */, const int32_t* slots, int* status,
                           cachalot_stream_t stream);
 
+/* Replaces minimax/gqa_decode.py:180-187 (grouped-query attention of one decode token over a contiguous cache): one new
+ * token per request against the tokens of its pages,
+ *   s_j = scale * q . k_j  (softcap > 0: softcap * tanh(s_j / softcap)),  out = softmax(s) V,  lse = log sum_j exp(s_j)
+ * over j < lens[r], with window > 0 only the last `window` of them (the new token is one of them and already in the cache).
+ * q [requests, heads, head_dim] F16 or BF16 (strides in elements, 4-byte aligned), out [requests, heads, head_dim]
+ * contiguous in out_dtype, lse f32 [requests, heads] or NULL; query head i reads key-value head i / (heads / kv_heads).  The cache holds q's type or
+ * E4M3.  block_table i32 [requests, width], rows table_stride apart; lens i32 [requests].  A request without a visible
+ * key gets zeros and -inf.  A length past its table is cut, a negative one counts as 0 (CACHALOT_STATUS_LENGTH); tokens on
+ * a page outside [0, n_pages) are hidden (CACHALOT_STATUS_SLOT_RANGE); pages that no visible token lies on are not looked at.
+ * head_dim 64, 96, 128, 192 or 256.  workspace: cachalot_paged_attention_workspace_bytes() bytes, 256-byte aligned, not
+ * shared by calls that may overlap; its content does not matter. */
+CACHALOT_API size_t cachalot_paged_attention_workspace_bytes(int heads, int kv_heads, int head_dim, int cache_dtype);
+CACHALOT_API int cachalot_paged_attention(const void* q, int64_t q_row_stride, int64_t q_head_stride, int q_dtype, int requests,
+                             int heads, const cachalot_paged_kv* cache /* host */, const int32_t* block_table,
+                             int64_t table_stride, int width, const int32_t* lens, float scale, int window, float softcap,
+                             void* workspace, size_t workspace_bytes, void* out, int out_dtype, float* lse, int* status,
+                             cachalot_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

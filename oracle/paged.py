@@ -60,35 +60,42 @@ def rotate(x, positions, inv_freq, interleaved=False, magnitude=1.0):
 
 
 def attend(q, keys, values, scale, softcap=0.0):
-    """One head: q [dim], keys and values [n, dim] (the visible ones) -> (out [dim], lse)."""
+    """One head: q [dim], keys and values [n, dim] (the visible ones) -> (out [dim], lse, spread [dim], reach, floor [dim]) with
+    what error bounds need: spread = sum p |v| / sum p, reach = largest |scale| * sum |q_i k_i|, floor = sum |v| / sum p for
+    p relative to the largest."""
     q, keys, values = (np.asarray(t, np.float64) for t in (q, keys, values))
+    zero = np.zeros(values.shape[1])
     if not len(keys):
-        return np.zeros(values.shape[1]), -np.inf
+        return zero, -np.inf, zero, 0.0, zero
     s = keys @ q * scale
     if softcap:
         s = softcap * np.tanh(s / softcap)
     m = s.max()
     if m == -np.inf:
-        return np.zeros(values.shape[1]), -np.inf
+        return zero, -np.inf, zero, 0.0, zero
     p = np.exp(s - m)
-    return p @ values / p.sum(), m + np.log(p.sum())
+    return (p @ values / p.sum(), m + np.log(p.sum()), p @ np.abs(values) / p.sum(), abs(scale) * (np.abs(keys) @ np.abs(q)).max(),
+            np.abs(values).sum(0) / p.sum())
 
 
 def paged_attention(q, keys, values, table, lens, page_size, scale, window=0, softcap=0.0):
-    """q [requests, heads, dim]; keys, values float64 [pages, kv_heads, page_size, dim] -> (out, lse).  A page outside the
-    cache hides its tokens; a length past the table is cut to it."""
+    """q [requests, heads, dim]; keys, values float64 [pages, kv_heads, page_size, dim] -> (out, lse, spread, reach, floor) as
+    `attend`, per request and head.  A page outside the cache hides its tokens; a length past the table is cut to it."""
     q = np.asarray(q, np.float64)
     pages, kv_heads = keys.shape[:2]
     group = q.shape[1] // kv_heads
-    out, lse = np.zeros(q.shape), np.full(q.shape[:2], -np.inf)
+    out, lse, spread, reach, floor = np.zeros(q.shape), np.full(q.shape[:2], -np.inf), np.zeros(q.shape), np.zeros(q.shape[:2]), np.zeros(q.shape)
     for r in range(q.shape[0]):
         n = min(max(int(lens[r]), 0), table.shape[1] * page_size)
-        where = [(int(table[r, j // page_size]), j % page_size) for j in range(max(0, n - window) if window else 0, n)]
-        where = [(p, o) for p, o in where if 0 <= p < pages]
-        p, o = (np.array([w[i] for w in where], dtype=np.int64) for i in (0, 1))
-        for h in range(q.shape[1]):
-            out[r, h], lse[r, h] = attend(q[r, h], keys[p, h // group, o], values[p, h // group, o], scale, softcap)
-    return out, lse
+        j = np.arange(max(0, n - window) if window else 0, n)
+        p, o = np.asarray(table[r])[j // page_size], j % page_size
+        live = (p >= 0) & (p < pages)
+        p, o = p[live], o[live]
+        for g in range(kv_heads):
+            k, v = keys[p, g, o], values[p, g, o]
+            for h in range(g * group, (g + 1) * group):
+                out[r, h], lse[r, h], spread[r, h], reach[r, h], floor[r, h] = attend(q[r, h], k, v, scale, softcap)
+    return out, lse, spread, reach, floor
 
 
 def token_logprobs(logits, tokens, top):

@@ -86,3 +86,34 @@ def test_qk_norm_rope_refusals():
                          (dict(d=cache(k_token_stride=63)), _lib.EALIGN, "strides"), (dict(d=cache(v_page_stride=-64)), _lib.EALIGN, "strides"),
                          (dict(d=cache(n_pages=2 ** 30)), _lib.EUNSUPPORTED, "slots"), (dict(d=cache(n_pages=0)), _lib.EINVAL, "empty")):
         assert call(**kw) == rc and word in _lib.last_error(), (kw, _lib.last_error())
+
+
+def test_paged_attention_refusals():
+    from cachalot_b200 import _lib
+
+    buf = (C.c_int32 * 4096)()
+    base = C.addressof(buf) + (-C.addressof(buf)) % 256
+    lib, p = _lib.lib, C.c_void_p(base)
+
+    def call(qs=256, dtype=_lib.BF16, requests=1, heads=4, kv=2, dim=64, cdt=_lib.BF16, table=p, stride=4, width=4, lens=p, window=0, cap=0.0, ws=p, room=1 << 40,
+             odt=_lib.BF16, q=p):
+        d = _lib.PagedKV()
+        d.k = d.v = base
+        d.k_page_stride = d.v_page_stride = 16 * kv * dim
+        d.k_head_stride = d.v_head_stride = 16 * dim
+        d.k_token_stride = d.v_token_stride = dim
+        d.n_pages, d.page_size, d.kv_heads, d.head_dim, d.dtype = 2, 16, kv, dim, cdt
+        return lib.cachalot_paged_attention(q, qs, dim, dtype, requests, heads, C.byref(d), table, stride, width, lens, 0.125, window, cap, ws, room, p, odt, None,
+                                            None, None)
+
+    for kw, rc, word in ((dict(requests=-1), _lib.EINVAL, "shape"), (dict(dtype=_lib.F32), _lib.EINVAL, "queries"), (dict(odt=_lib.E4M3), _lib.EINVAL, "output"),
+                         (dict(heads=5), _lib.EINVAL, "heads"), (dict(cdt=_lib.F16), _lib.EINVAL, "differ"), (dict(window=-1), _lib.EINVAL, "window"),
+                         (dict(cap=-1.0), _lib.EINVAL, "softcap"), (dict(cap=float("nan")), _lib.EINVAL, "softcap"), (dict(dim=80), _lib.EUNSUPPORTED, "80"),
+                         (dict(table=None), _lib.EINVAL, "null"), (dict(lens=None), _lib.EINVAL, "null"), (dict(ws=None), _lib.EINVAL, "null"),
+                         (dict(q=C.c_void_p(base + 2)), _lib.EALIGN, "4-byte"), (dict(qs=255), _lib.EALIGN, "4-byte"),
+                         (dict(requests=2, stride=3), _lib.EINVAL, "overlap"), (dict(ws=C.c_void_p(base + 16)), _lib.EALIGN, "256"),
+                         (dict(room=1000), _lib.ESCRATCH, "workspace")):
+        assert call(**kw) == rc and word in _lib.last_error(), (kw, _lib.last_error())
+    assert call(requests=0, lens=None) == _lib.OK
+    size = lib.cachalot_paged_attention_workspace_bytes
+    assert size(64, 8, 128, _lib.BF16) > 0 and size(64, 8, 80, _lib.BF16) == 0 and size(64, 7, 128, _lib.BF16) == 0 and size(64, 0, 128, _lib.E4M3) == 0
