@@ -17,7 +17,7 @@ _OPS = (
     "affine_expert_forward_batched", "SlabExperts", "shared_expert_forward", "shared_expert_forward_fused",
     "shared_expert_forward_batched", "fp8_linear_rows", "bf16_gemv_f32", "fused_qr_kv_linear", "moe_layer_forward", "validate_routing", "self_check", "requantize_fp4_to_affine", "requantize_bank",
 )
-_PAGED = ("PagePlan", "paged_attention", "plan_pages", "qk_norm_rope", "rope_frequencies")
+_PAGED = ("PagePlan", "TokenLogprobs", "paged_attention", "plan_pages", "qk_norm_rope", "rope_frequencies", "token_logprobs")
 _LOADER = ("load_bank", "detect_expert_bank", "build_expert_index", "build_stacked_expert_index")
 __all__ = [*_BANK, *_OPS, *_PAGED, *_LOADER, "NUMERICS_VERSION"]
 

@@ -101,6 +101,7 @@ SIGNATURES = {
                                    _vp, _vp, C.POINTER(PagedKV), _vp, _vp, _vp]),
     "cachalot_paged_attention_workspace_bytes": (_sz, [_i, _i, _i, _i]),
     "cachalot_paged_attention": (_i, [_vp, _i64, _i64, _i, _i, _i, C.POINTER(PagedKV), _vp, _i64, _i, _vp, _f, _i, _f, _vp, _sz, _vp, _i, _vp, _vp, _vp]),
+    "cachalot_token_logprobs": (_i, [_vp, _i, _i64, _i, _i, _vp, _i, _vp, _vp, _vp, _vp, _vp, _vp]),
     "cachalot_moe_prefill": (_i, [_vp, _desc, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _f, _i, _vp, _sz, _vp, _vp, _vp]),
 }
 

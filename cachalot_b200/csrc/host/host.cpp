@@ -33,7 +33,7 @@ using at::ScalarType;
   X(cachalot_paged_attention_workspace_bytes) X(cachalot_plan_pages) \
   X(cachalot_qk_norm_rope) \
   X(cachalot_route_topk) \
-  X(cachalot_router_logits) X(cachalot_shared_expert) X(cachalot_shared_expert_workspace_bytes)
+  X(cachalot_router_logits) X(cachalot_shared_expert) X(cachalot_shared_expert_workspace_bytes) X(cachalot_token_logprobs)
 struct Lib {
 #define X(name) decltype(&::name) name = nullptr;
   ENTRIES(X)
@@ -553,9 +553,33 @@ PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   END_HANDLE_TH_ERRORS
 }
 
+// (logits [rows, vocab], tokens [rows], top, status | None) -> (logprobs, entropy, top_ids, top_logprobs)
+PyObject* token_logprobs(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+  HANDLE_TH_ERRORS
+  PLAIN_OR_NONE(bound && n_args == 4);
+  Args p{a};
+  const at::Tensor *x = tensor_of(a[0]), *ids = tensor_of(a[1]);
+  PLAIN_OR_NONE(x && x->is_cuda());
+  const int dev = current_device(), top = (int)p.i(2);
+  const ScalarType t = x->scalar_type();
+  const int dt = t == ScalarType::Float ? CACHALOT_F32 : t == ScalarType::BFloat16 || t == ScalarType::Half ? element_code(t) : -1;
+  PLAIN_OR_NONE(!p.bad && dt >= 0 && x->get_device() == dev && x->dim() == 2 && x->stride(1) == 1);
+  const int64_t rows = x->size(0), vocab = x->size(1);
+  PLAIN_OR_NONE(rows > 0 && rows < (1LL << 31) && vocab > 0 && vocab < (1LL << 31) && top >= 0 && top <= vocab && plain_ints(ids, rows, dev));
+  PLAIN_OR_NONE(none_or_plain(a[3], ScalarType::Int, dev) && (a[3] == Py_None || tensor_of(a[3])->numel() > 0));
+  at::Tensor lp = empty({rows}, ScalarType::Float, dev), h = empty({rows}, ScalarType::Float, dev);
+  at::Tensor ti = empty({rows, top}, ScalarType::Int, dev), tv = empty({rows, top}, ScalarType::Float, dev);
+  const int rc = UNLOCKED(lib.cachalot_token_logprobs(x->data_ptr(), dt, x->stride(0), (int)rows, (int)vocab, ints(*ids), top, static_cast<float*>(lp.data_ptr()),
+                                                      static_cast<float*>(h.data_ptr()), ints(ti), static_cast<float*>(tv.data_ptr()),
+                                                      static_cast<int*>(ptr_or_null(a[3])), current_stream(dev)));
+  if (rc) return raise(rc);
+  return Py_BuildValue("(NNNN)", THPVariable_Wrap(std::move(lp)), THPVariable_Wrap(std::move(h)), THPVariable_Wrap(std::move(ti)), THPVariable_Wrap(std::move(tv)));
+  END_HANDLE_TH_ERRORS
+}
+
 #define FAST(name) {#name, (PyCFunction)(void (*)(void))name, METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {FAST(entries), FAST(bind), FAST(fp8_linear), FAST(bf16_gemv_f32), FAST(shared_expert), FAST(moe_forward), FAST(layer_decode),
-                         FAST(prefill_grouped), FAST(moe_block), FAST(plan_pages), FAST(qk_norm_rope), FAST(paged_attention), {nullptr, nullptr, 0, nullptr}};
+                         FAST(prefill_grouped), FAST(moe_block), FAST(plan_pages), FAST(qk_norm_rope), FAST(paged_attention), FAST(token_logprobs), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", "Native call path of the operators (see host.cpp).", -1, methods};
 
 }  // namespace

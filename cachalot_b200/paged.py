@@ -1,4 +1,5 @@
-"""The decode step around the experts: page plan, query and key preparation, attention over a paged key-value cache.
+"""The decode step around the experts: page plan, query and key preparation, attention over a paged key-value cache,
+log probabilities of the head's logits.
 
 A cache of one layer is two tensors `k_cache` and `v_cache` [pages, kv_heads, page_size, head_dim] of float16, bfloat16 or
 float8_e4m3fn (with one float32 scale per head: value = code * scale); other orders of the first three axes are views of
@@ -268,3 +269,39 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
                                            block_table.stride(0), block_table.shape[1], _ptr(n), scale, window, softcap, _ptr(ws), need, _ptr(out),
                                            _DT[out_dtype], _ptr(lse), _ptr(status), _stream(dev)))
     return (out, lse) if want_lse else out
+
+
+# ---- log probabilities ------------------------------------------------------------------------
+
+class TokenLogprobs(NamedTuple):
+    """float32 `logprobs` and `entropy` [rows], `top_ids` int32 and `top_logprobs` float32 [rows, top]."""
+
+    logprobs: torch.Tensor
+    entropy: torch.Tensor
+    top_ids: torch.Tensor
+    top_logprobs: torch.Tensor
+
+
+def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, top: int = 0, status: torch.Tensor | None = None) -> TokenLogprobs:
+    """Log probability of tokens int32 [rows] under logits [rows, vocab] (float32 as `bf16_gemv_f32` gives them, bfloat16 or
+    float16), entropy of each row in nats and the `top` <= 32 most likely tokens (ties to the lower index), in one pass over
+    the logits.  A negative id is padding (log probability 0), as is one past the vocabulary (STATUS_ID_RANGE); logits
+    of -inf have no weight, and a row of nothing else gives -inf and entropy 0."""
+    r = _host.token_logprobs(logits, tokens, top, status)
+    if r is not None:
+        return TokenLogprobs(*r)
+    dev = _same_device(logits, tokens, status)
+    if logits.dim() != 2 or logits.dtype not in (torch.float32, torch.bfloat16, torch.float16):
+        raise ValueError(f"logits must be float32, bfloat16 or float16 [rows, vocab], got {logits.dtype} {tuple(logits.shape)}")
+    rows, vocab = logits.shape
+    ids = _ints(tokens, "tokens", (rows,))
+    _status(status)
+    if not 0 <= top < 2 ** 31:
+        raise ValueError(f"top must be in [0, 32], got {top}")
+    with torch.cuda.device(dev):
+        x = logits if logits.stride(1) == 1 else logits.contiguous()
+        logprobs, entropy = (torch.empty(rows, dtype=torch.float32, device=dev) for _ in range(2))
+        top_ids, top_logprobs = (torch.empty((rows, min(top, vocab)), dtype=t, device=dev) for t in (torch.int32, torch.float32))
+        check(lib.cachalot_token_logprobs(_ptr(x), _DT[x.dtype], x.stride(0), rows, vocab, _ptr(ids), top, _ptr(logprobs), _ptr(entropy), _ptr(top_ids),
+                                          _ptr(top_logprobs), _ptr(status), _stream(dev)))
+    return TokenLogprobs(logprobs, entropy, top_ids, top_logprobs)

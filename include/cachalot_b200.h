@@ -428,6 +428,16 @@ CACHALOT_API int cachalot_paged_attention(const void* q, int64_t q_row_stride, i
                              void* workspace, size_t workspace_bytes, void* out, int out_dtype, float* lse, int* status,
                              cachalot_stream_t stream);
 
+/* No counterpart in the reference (its sampling reads the whole logits on the host).  For every row of logits
+ * [rows, vocab] (dtype F32, BF16 or F16, rows row_stride elements apart): logprobs[r] = log softmax of tokens[r] (0 for a
+ * negative id, and for one past the vocabulary: CACHALOT_STATUS_ID_RANGE), entropy[r] = -sum p log p (f32 [rows]), and the
+ * `top` <= 32 most likely tokens, most likely first, ties to the lower index: top_ids i32, top_logprobs f32 [rows, top].
+ * Masked logits (-inf or the type's lowest value) have no weight; a row of -inf alone has log probabilities -inf and entropy 0.  A NaN makes a
+ * row's numbers NaN and is no alternative (missing ones: id -1, -inf). */
+CACHALOT_API int cachalot_token_logprobs(const void* logits, int dtype, int64_t row_stride, int rows, int vocab, const int32_t* tokens,
+                            int top, float* logprobs, float* entropy, int32_t* top_ids, float* top_logprobs, int* status,
+                            cachalot_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -110,7 +110,7 @@ def token_logprobs(logits, tokens, top):
         elif m == -np.inf:
             lp = np.full(vocab, -np.inf)
         else:
-            lp = x[r] - (m + np.log(np.exp(x[r] - m).sum()))
+            lp = (x[r] - m) - np.log(np.exp(x[r] - m).sum())  # m apart: a mask value of 10^38 swallows the sum
         p = np.exp(lp)
         ent[r] = -np.sum(np.where(p > 0, p * np.where(p > 0, lp, 0.0), 0.0)) if not np.isnan(m) else np.nan
         t = int(tokens[r])

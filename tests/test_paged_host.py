@@ -117,3 +117,16 @@ def test_paged_attention_refusals():
     assert call(requests=0, lens=None) == _lib.OK
     size = lib.cachalot_paged_attention_workspace_bytes
     assert size(64, 8, 128, _lib.BF16) > 0 and size(64, 8, 80, _lib.BF16) == 0 and size(64, 7, 128, _lib.BF16) == 0 and size(64, 0, 128, _lib.E4M3) == 0
+
+
+def test_token_logprobs_refusals():
+    from cachalot_b200 import _lib
+
+    lib, p = _lib.lib, _p((C.c_int32 * 64)())
+    call = lambda x=p, dt=_lib.F32, rows=1, vocab=8, ids=p, top=2, tops=p: lib.cachalot_token_logprobs(x, dt, vocab, rows, vocab, ids, top, p, p, tops, tops, None, None)  # noqa: E731
+    for kw, rc, word in ((dict(rows=-1), _lib.EINVAL, "shape"), (dict(vocab=0), _lib.EINVAL, "shape"), (dict(dt=_lib.E4M3), _lib.EINVAL, "float32"),
+                         (dict(top=9), _lib.EINVAL, "9 alternatives"), (dict(top=-1), _lib.EINVAL, "alternatives"), (dict(vocab=50, top=33), _lib.EUNSUPPORTED, "33"),
+                         (dict(x=None), _lib.EINVAL, "null"), (dict(ids=None), _lib.EINVAL, "null"), (dict(tops=None), _lib.EINVAL, "null"),
+                         (dict(x=C.c_void_p(p.value + 2)), _lib.EALIGN, "aligned")):
+        assert call(**kw) == rc and word in _lib.last_error(), (kw, _lib.last_error())
+    assert call(rows=0, x=None) == _lib.OK
