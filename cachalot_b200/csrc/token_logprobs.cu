@@ -3,13 +3,19 @@
 //   m running maximum, S = sum e^(x - m), U = sum e^(x - m) (x - m):
 //   logprob(t) = x_t - m - ln S,  H = ln S - U / S;  when m moves to m': S' = f S, U' = f (U + S (m - m')), f = e^(m - m')
 //
-// HBM-bound: every logit is read once, 4 or 2 bytes, for one exponential and five other instructions.  Each thread keeps
-// (m, S, U) of its own elements, 16-byte loads four deep.  A row is split over a cluster of CTAs where there are few rows,
-// joined through distributed shared memory: one launch, no workspace.
-// The alternatives: every warp keeps its n best so far sorted across its lanes (n <= 32) and only looks closer at loads
-// whose maximum beats its last one and the last one of the CTA's best list; on logits in no particular order that is
-// n (1 + ln(vocabulary / n)) insertions per CTA.  Ties go to the lower index: a warp walks the row upwards, so a later equal value
-// never displaces an earlier one, and insertions and merges compare (value, index).
+// HBM-bound: every logit is read once, 4 or 2 bytes, for one exponential and six other instructions.  Each thread keeps
+// (m, S, U) of its own elements; the 16-byte loads of a round (four per thread) are issued before the round in hand is
+// worked on.  A row is split over a cluster of CTAs where there are few rows, joined through distributed shared memory:
+// one launch, no workspace.
+//
+// The alternatives are kept as 64-bit keys (value mapped to an ordered integer, complement of the index: all distinct,
+// ties to the lower index).  The first round of a CTA finds the n-th largest of its 256 threads' own maxima, a lower
+// bound of the n-th best that only about n of the round's elements reach; from then on a thread looks closer only when its
+// maximum reaches the bar and puts what does into a list in shared memory, about n elements per round on logits in no
+// particular order.  A round that would overflow the list (rising logits) raises the bar first, from the list and the
+// threads' maxima together: at most n threads reach it, so at most 32 n elements.  Selections are bitonic: warps sort 32 keys
+// across their lanes and merge sorted lists.  (Inserting one by one into a list per warp: 335 us for 512 rows of 129280 bf16
+// logits, 8 alternatives; one row, f32, 20 alternatives: 59 us.)
 #include <cfloat>
 #include <cooperative_groups.h>
 
@@ -21,6 +27,8 @@ namespace {
 namespace cg = cooperative_groups;
 
 constexpr int TL_THREADS = 256, TL_WARPS = TL_THREADS / 32, TL_MAX_TOP = 32, TL_LOADS = 4;
+constexpr int TL_CTAS = 3;     // per SM: 48 KB of loads in flight
+constexpr int TL_LIST = 1088;  // 32 kept + 32 threads' 32 elements
 constexpr float TL_LOG2E = 1.4426950408889634f;
 constexpr float TL_FAR = -200.f;  // e^-200 is zero in fp32; stands for -inf, which would make 0 * -inf
 
@@ -52,132 +60,198 @@ struct Sums {  // a maximum that covers the terms (never below -FLT_MAX), sum, s
   }
 };
 
-struct Best {  // lane i holds the i-th best of a warp; empty: (-inf, INT_MAX)
-  float v;
-  int i;
-};
-__device__ __forceinline__ bool before(float av, int ai, float bv, int bi) { return av > bv || (av == bv && ai < bi); }
-// the whole warp inserts one candidate
-__device__ __forceinline__ void insert(Best& b, int lane, float v, int i) {
-  const int at = __popc(__ballot_sync(0xffffffffu, before(b.v, b.i, v, i)));
-  const float uv = __shfl_up_sync(0xffffffffu, b.v, 1);
-  const int ui = __shfl_up_sync(0xffffffffu, b.i, 1);
-  if (lane > at) b.v = uv, b.i = ui;
-  if (lane == at) b.v = v, b.i = i;
+using Key = unsigned long long;  // 0: none
+__device__ __forceinline__ Key key_of(float v, int i) {
+  const unsigned b = __float_as_uint(v + 0.f);  // -0 counts as 0
+  return (Key)(b >> 31 ? ~b : b | 0x80000000u) << 32 | (unsigned)~i;
 }
-// ... the candidates that lanes hold, those that pass `take`
-__device__ __forceinline__ void insert_all(Best& b, int lane, bool take, float v, int i) {
-  for (unsigned hit = __ballot_sync(0xffffffffu, take); hit; hit &= hit - 1) {
-    const int from = __ffs(hit) - 1;
-    insert(b, lane, __shfl_sync(0xffffffffu, v, from), __shfl_sync(0xffffffffu, i, from));
+__device__ __forceinline__ float value_of(Key k) {
+  const unsigned b = (unsigned)(k >> 32);
+  return k ? __uint_as_float(b >> 31 ? b ^ 0x80000000u : ~b) : -INFINITY;
+}
+__device__ __forceinline__ int index_of(Key k) { return k ? (int)~(unsigned)k : -1; }
+
+__device__ __forceinline__ Key swap_step(Key x, int lane, int j, bool down) {
+  const Key y = __shfl_xor_sync(0xffffffffu, x, j);
+  return ((lane & j) == 0) == down ? max(x, y) : min(x, y);
+}
+// 32 keys across the lanes, largest first
+__device__ __forceinline__ Key sort32(Key x, int lane) {
+#pragma unroll
+  for (int k = 2; k <= 32; k <<= 1)
+#pragma unroll
+    for (int j = k >> 1; j > 0; j >>= 1) x = swap_step(x, lane, j, (lane & k) == 0);
+  return x;
+}
+// the 32 largest of two sorted lists, sorted
+__device__ __forceinline__ Key merge32(Key a, Key b, int lane) {
+  Key x = max(a, __shfl_sync(0xffffffffu, b, 31 - lane));
+#pragma unroll
+  for (int j = 16; j > 0; j >>= 1) x = swap_step(x, lane, j, true);
+  return x;
+}
+// ... of the warps' sorted lists, in warp 0 and in lists[0]
+__device__ __forceinline__ Key merge_block(Key x, Key (*lists)[32], int warp, int lane) {
+  lists[warp][lane] = x;
+#pragma unroll
+  for (int step = 1; step < TL_WARPS; step <<= 1) {
+    __syncthreads();
+    if (warp % (2 * step) == 0) lists[warp][lane] = x = merge32(x, lists[warp + step][lane], lane);
   }
+  __syncthreads();
+  return x;
 }
 
-// order-preserving map of floats to unsigned (NaN does not occur here)
-__device__ __forceinline__ unsigned key_of(float v) {
-  const unsigned b = __float_as_uint(v);
-  return b >> 31 ? ~b : b | 0x80000000u;
-}
-__device__ __forceinline__ float value_of(unsigned k) { return __uint_as_float(k >> 31 ? k ^ 0x80000000u : ~k); }
-
+// 16 bytes of logits
 template <typename T>
-__device__ __forceinline__ float widen(T x) {
-  if constexpr (sizeof(T) == 4) return x;
-  else if constexpr (std::is_same<T, __half>::value) return __half2float(x);
-  else return __bfloat162float(x);
-}
+struct Vec {
+  static constexpr int PER = 16 / sizeof(T);
+  uint4 raw;
+  __device__ __forceinline__ float at(int j) const {
+    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+    if constexpr (sizeof(T) == 4) return __uint_as_float(w[j]);
+    else if constexpr (std::is_same<T, __half>::value) return __half2float(reinterpret_cast<const __half*>(w)[j]);
+    else return __uint_as_float(j & 1 ? w[j / 2] & 0xffff0000u : w[j / 2] << 16);
+  }
+  // the largest, NaN left out (-inf or NaN where there is nothing else)
+  __device__ __forceinline__ float top() const {
+    if constexpr (sizeof(T) == 4) {
+      return fmaxf(fmaxf(at(0), at(1)), fmaxf(at(2), at(3)));
+    } else {
+      const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+      using T2 = std::conditional_t<std::is_same<T, __half>::value, __half2, __nv_bfloat162>;
+      const T2* h = reinterpret_cast<const T2*>(w);
+      const T2 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+      return fmaxf(widen(m.x), widen(m.y));
+    }
+  }
+  __device__ static __forceinline__ float widen(T x) {
+    if constexpr (sizeof(T) == 4) return x;
+    else if constexpr (std::is_same<T, __half>::value) return __half2float(x);
+    else return __bfloat162float(x);
+  }
+  __device__ static __forceinline__ uint32_t bits(T x) {
+    if constexpr (sizeof(T) == 4) return __float_as_uint(x);
+    else if constexpr (std::is_same<T, __half>::value) return __half_as_ushort(x);
+    else return __bfloat16_as_ushort(x);
+  }
+  // elements [from, from + PER) of a row, -inf outside [0, vocab)
+  __device__ __forceinline__ void load(const T* row, int from, int vocab) {
+    if (from >= 0 && from + PER <= vocab) {
+      raw = ld_stream_u4(row + from);
+      return;
+    }
+    uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      const int i = from + j;
+      uint32_t b = sizeof(T) == 4 ? 0xff800000u : std::is_same<T, __half>::value ? 0xfc00u : 0xff80u;
+      if (i >= 0 && i < vocab) b = bits(row[i]);
+      w[j * (int)sizeof(T) / 4] |= b << (sizeof(T) == 4 ? 0 : (j & 1) * 16);
+    }
+    raw = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+};
 
 template <typename T, bool TOP>
-__global__ void __launch_bounds__(TL_THREADS) token_logprobs_kernel(const T* __restrict__ logits, long long stride, int vocab,
+__global__ void __launch_bounds__(TL_THREADS, TL_CTAS) token_logprobs_kernel(const T* __restrict__ logits, long long stride, int vocab,
                                                                     const int32_t* __restrict__ tokens, int top, float* __restrict__ logprobs,
                                                                     float* __restrict__ entropy, int32_t* __restrict__ top_ids,
                                                                     float* __restrict__ top_logprobs, int* status) {
-  constexpr int PER = 16 / sizeof(T);
+  using V = Vec<T>;
+  constexpr int PER = V::PER;
   __shared__ Sums parts[TL_WARPS];
-  __shared__ float list_v[TL_WARPS][TL_MAX_TOP];
-  __shared__ int list_i[TL_WARPS][TL_MAX_TOP];
-  __shared__ unsigned bar;  // key of the best n-th value of any of the CTA's warps
+  __shared__ Key lists[TOP ? TL_WARPS : 1][32];
+  __shared__ Key list[TOP ? TL_LIST : 1];
+  __shared__ int added[3];  // by the rounds in turn: one is counted, one still read, one cleared
   cg::cluster_group cluster = cg::this_cluster();
   const int ctas = cluster.num_blocks(), rank = cluster.block_rank();
-  const int row = blockIdx.x / ctas, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int row = blockIdx.x / ctas, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const T* x = logits + row * stride;
-  const int head = min(vocab, (int)((16 - reinterpret_cast<uintptr_t>(x) % 16) % 16 / sizeof(T)));  // elements before the first 16-byte boundary
-  const int vectors = (vocab - head) / PER;
-  const T* body = x + head;
+  // 16-byte vectors of the row, the first and the last may reach over its ends
+  const int shift = (int)(reinterpret_cast<uintptr_t>(x) % 16 / sizeof(T));
+  const int vectors = (vocab + shift + PER - 1) / PER;
+  const int rounds = (vectors + ctas * TL_LOADS * TL_THREADS - 1) / (ctas * TL_LOADS * TL_THREADS);
+  auto vector_of = [&](int round, int k) { return ((round * ctas + rank) * TL_LOADS + k) * TL_THREADS + tid; };
 
   Sums sum{-FLT_MAX, 0.f, 0.f};
-  Best best{-INFINITY, 0x7fffffff};
-  float last = -INFINITY;   // the warp's n-th best
-  bool full = false;
-  if (TOP && threadIdx.x == 0) bar = 0;
-  if (TOP) __syncthreads();
+  int held = 0;          // length of the list
+  Key bar = 0;           // nothing below it is among the best
+  float bar_value = -INFINITY;
+  if (TOP && tid < 3) added[tid] = 0;
 
-  auto settle = [&](int n) {  // after insertions
-    last = __shfl_sync(0xffffffffu, best.v, n - 1);
-    full = __shfl_sync(0xffffffffu, best.i, n - 1) != 0x7fffffff;
-    if (full && lane == 0) atomicMax(&bar, key_of(last));
+  V next[TL_LOADS];
+  auto fetch = [&](int round) {
+#pragma unroll
+    for (int k = 0; k < TL_LOADS; ++k) next[k].load(x, vector_of(round, k) * PER - shift, vocab);
   };
-  auto single = [&](int at, int end) {  // the warp takes up to 32 elements outside the 16-byte body
-    const bool live = at + lane < end;
-    const float v = live ? widen(x[at + lane]) : -INFINITY;
-    if (live) {
-      if (v > sum.m) sum.move(v);
-      sum.add(v);
-    }
-    if (TOP) {
-      insert_all(best, lane, live && v >= last, v, at + lane);
-      settle(top);
-    }
-  };
-
-  if (head && rank == 0 && warp == 0) single(0, head);
-  const int walkers = ctas * TL_WARPS, me = rank * TL_WARPS + warp;
-  for (int v0 = me * TL_LOADS * 32; v0 < vectors; v0 += walkers * TL_LOADS * 32) {
-    float e[TL_LOADS][PER];
+  fetch(0);
+  for (int round = 0; round < rounds; ++round) {
+    V now[TL_LOADS];
     float most = -INFINITY;
-    uint4 raw[TL_LOADS];
 #pragma unroll
-    for (int k = 0; k < TL_LOADS; ++k) {
-      const int at = v0 + k * 32 + lane;
-      if (at < vectors) raw[k] = ld_stream_u4(body + (long long)at * PER);
-    }
-#pragma unroll
-    for (int k = 0; k < TL_LOADS; ++k) {
-      const bool live = v0 + k * 32 + lane < vectors;
-      const uint32_t w[4] = {raw[k].x, raw[k].y, raw[k].z, raw[k].w};
-#pragma unroll
-      for (int j = 0; j < PER; ++j) {
-        float f;
-        if constexpr (sizeof(T) == 4) f = __uint_as_float(w[j]);
-        else if constexpr (std::is_same<T, __half>::value) f = __half2float(reinterpret_cast<const __half*>(w)[j]);
-        else f = __uint_as_float(j & 1 ? w[j / 2] & 0xffff0000u : w[j / 2] << 16);
-        e[k][j] = live ? f : -INFINITY;
-        most = fmaxf(most, e[k][j]);
-      }
-    }
+    for (int k = 0; k < TL_LOADS; ++k) now[k] = next[k], most = fmaxf(most, now[k].top());
+    if (round + 1 < rounds) fetch(round + 1);
     if (most > sum.m) sum.move(most);
 #pragma unroll
     for (int k = 0; k < TL_LOADS; ++k)
 #pragma unroll
-      for (int j = 0; j < PER; ++j) sum.add(e[k][j]);
+      for (int j = 0; j < PER; ++j) sum.add(now[k].at(j));
     if constexpr (TOP) {
-      const unsigned b = *(volatile unsigned*)&bar;
-      const float shared_last = b ? value_of(b) : -INFINITY;
-      // strictly above the warp's own last one (all of its list comes before these), or at least the CTA's
-      const bool look = full ? most > last && most >= shared_last : true;
-      if (__any_sync(0xffffffffu, look)) {
-        const float bound = fmaxf(last, shared_last);
+      int* count = &added[round % 3];
+      if (tid == 0) added[(round + 1) % 3] = 0;
+      auto push = [&](Key k, int base, int limit) {
+        const int at = base + atomicAdd(count, 1);
+        if (at < limit) list[at] = k;
+      };
+      auto offer = [&](int base) {  // this thread's elements that reach the bar
+        if (!(most >= bar_value)) return;
 #pragma unroll
         for (int k = 0; k < TL_LOADS; ++k) {
-          const int at = v0 + k * 32 + lane;
+          if (!(now[k].top() >= bar_value)) continue;
 #pragma unroll
-          for (int j = 0; j < PER; ++j) insert_all(best, lane, at < vectors && e[k][j] >= bound, e[k][j], head + at * PER + j);
+          for (int j = 0; j < PER; ++j) {
+            const float v = now[k].at(j);
+            const int i = vector_of(round, k) * PER - shift + j;
+            if (v >= bar_value && i >= 0 && i < vocab && key_of(v, i) >= bar) push(key_of(v, i), base, TL_LIST);
+          }
         }
-        settle(top);
+      };
+      bool raise = round == 0;
+      if (!raise) {
+        offer(held);
+        __syncthreads();
+        const int n = *count;
+        if (held + n > TL_LIST) raise = true;
+        else held += n;
+      }
+      if (raise) {  // (the round's entries of the list, if any, are given up)
+        Key best = 0;
+#pragma unroll
+        for (int k = TL_LOADS - 1; k >= 0; --k)
+#pragma unroll
+          for (int j = PER - 1; j >= 0; --j) {
+            const int i = vector_of(round, k) * PER - shift + j;
+            if (now[k].at(j) == most && i >= 0 && i < vocab) best = key_of(most, i);
+          }
+        Key mine = sort32(best, lane);
+        for (int at = warp * 32; at < held; at += TL_THREADS) mine = merge32(mine, sort32(at + lane < held ? list[at + lane] : 0, lane), lane);
+        merge_block(mine, lists, warp, lane);
+        bar = lists[0][top - 1], bar_value = value_of(bar);
+        Key kept[(TL_LIST + TL_THREADS - 1) / TL_THREADS];
+#pragma unroll
+        for (int c = 0; c < (TL_LIST + TL_THREADS - 1) / TL_THREADS; ++c) kept[c] = c * TL_THREADS + tid < held ? list[c * TL_THREADS + tid] : 0;
+        if (tid == 0) *count = 0;
+        __syncthreads();
+#pragma unroll
+        for (int c = 0; c < (TL_LIST + TL_THREADS - 1) / TL_THREADS; ++c)
+          if (kept[c] && kept[c] >= bar) push(kept[c], 0, TL_LIST);
+        offer(0);
+        __syncthreads();
+        held = *count;
       }
     }
   }
-  if (rank == ctas - 1 && warp == TL_WARPS - 1 && head + vectors * PER < vocab) single(head + vectors * PER, vocab);
 
   // ---- warps, then CTAs ----
 #pragma unroll
@@ -186,35 +260,24 @@ __global__ void __launch_bounds__(TL_THREADS) token_logprobs_kernel(const T* __r
     sum.join(other);
   }
   if (lane == 0) parts[warp] = sum;
-  if (TOP) list_v[warp][lane] = best.v, list_i[warp][lane] = best.i;
-  __syncthreads();
+  Key best = 0;
+  if constexpr (TOP) {
+    for (int at = warp * 32; at < held; at += TL_THREADS) best = merge32(best, sort32(at + lane < held ? list[at + lane] : 0, lane), lane);
+    best = merge_block(best, lists, warp, lane);
+  } else {
+    __syncthreads();
+  }
   if (warp == 0) {
-    for (int w = 1; w < TL_WARPS; ++w) {
-      sum.join(parts[w]);
-      if (TOP) {
-        const float v = list_v[w][lane];
-        const int i = list_i[w][lane];
-        const float lv = __shfl_sync(0xffffffffu, best.v, top - 1);
-        const int li = __shfl_sync(0xffffffffu, best.i, top - 1);
-        insert_all(best, lane, lane < top && before(v, i, lv, li), v, i);
-      }
-    }
+    for (int w = 1; w < TL_WARPS; ++w) sum.join(parts[w]);
     __syncwarp();
     if (lane == 0) parts[0] = sum;
-    if (TOP) list_v[0][lane] = best.v, list_i[0][lane] = best.i;
   }
   if (ctas > 1) {
     cluster.sync();
     if (rank == 0 && warp == 0) {
       for (int c = 1; c < ctas; ++c) {
         sum.join(*cluster.map_shared_rank(&parts[0], c));
-        if (TOP) {
-          const float v = *cluster.map_shared_rank(&list_v[0][lane], c);
-          const int i = *cluster.map_shared_rank(&list_i[0][lane], c);
-          const float lv = __shfl_sync(0xffffffffu, best.v, top - 1);
-          const int li = __shfl_sync(0xffffffffu, best.i, top - 1);
-          insert_all(best, lane, lane < top && before(v, i, lv, li), v, i);
-        }
+        if (TOP) best = merge32(best, *cluster.map_shared_rank(&lists[0][lane], c), lane);
       }
     }
     cluster.sync();  // nobody leaves before its shared memory has been read
@@ -226,14 +289,13 @@ __global__ void __launch_bounds__(TL_THREADS) token_logprobs_kernel(const T* __r
     if (lane == 0) {
       const int t = tokens[row];
       if (t >= vocab && status) atomicOr(status, CACHALOT_STATUS_ID_RANGE);
-      logprobs[row] = t >= 0 && t < vocab ? logp(widen(x[t])) : 0.f;
+      logprobs[row] = t >= 0 && t < vocab ? logp(V::widen(x[t])) : 0.f;
       const float h = log_s - sum.u / sum.s;
       entropy[row] = none || h < 0.f ? 0.f : h;
     }
     if (TOP && lane < top) {
-      const bool there = best.i != 0x7fffffff;
-      top_ids[(long long)row * top + lane] = there ? best.i : -1;
-      top_logprobs[(long long)row * top + lane] = there ? logp(best.v) : -INFINITY;
+      top_ids[(long long)row * top + lane] = index_of(best);
+      top_logprobs[(long long)row * top + lane] = best ? logp(value_of(best)) : -INFINITY;
     }
   }
 }
@@ -263,7 +325,7 @@ extern "C" int cachalot_token_logprobs(const void* logits, int dtype, int64_t ro
   if (!logits || !tokens || !logprobs || !entropy || (top && (!top_ids || !top_logprobs))) return fail(CACHALOT_EINVAL, "token_logprobs: null pointer");
   const int es = dtype == CACHALOT_F32 ? 4 : 2;
   if (!aligned(logits, es)) return fail(CACHALOT_EALIGN, "token_logprobs: logits are not aligned to their type");
-  if (vocab > 0x7fffffff - 65536) return fail(CACHALOT_EUNSUPPORTED, "token_logprobs: vocabulary of %d", vocab);
+  if (vocab > 0x7fffffff - 131072) return fail(CACHALOT_EUNSUPPORTED, "token_logprobs: vocabulary of %d", vocab);
   // CTAs of a row: enough to fill the GPU with few rows, a power of two up to the portable cluster size
   int ctas = 1;
   while (ctas < 8 && (long long)rows * ctas * 2 <= 1184 && (long long)vocab * es / ctas > 32768) ctas *= 2;

@@ -98,6 +98,18 @@ def test_masks():
         _check(y, [4, 0, 3, 5, 6, 7], 12)
 
 
+def test_zeros_of_either_sign_tie():
+    x = torch.full((2, 3000), -1.0, device="cuda")
+    x[:, 100:2000:3], x[:, 101:2000:3] = -0.0, 0.0
+    _check(x, [100, 101], 32), _check(x.to(F16), [100, 101], 32)
+
+
+def test_too_few_alternatives_that_are_numbers():
+    x = torch.full((2, 40000), float("nan"), device="cuda")
+    x[0, 5::10000], x[1, ::2] = 1.0, -float("inf")
+    _check(x, [5, 6], 32)
+
+
 def test_padding_and_tokens_outside():
     x = torch.randn((4, 300), device="cuda", generator=_gen(3))
     _check(x, [-1, 5, -100, 299], 3)
