@@ -11,11 +11,9 @@
 // The alternatives are kept as 64-bit keys (value mapped to an ordered integer, complement of the index: all distinct,
 // ties to the lower index).  The first round of a CTA finds the n-th largest of its 256 threads' own maxima, a lower
 // bound of the n-th best that only about n of the round's elements reach; from then on a thread looks closer only when its
-// maximum reaches the bar and puts what does into a list in shared memory, about n elements per round on logits in no
-// particular order.  A round that would overflow the list (rising logits) raises the bar first, from the list and the
-// threads' maxima together: at most n threads reach it, so at most 32 n elements.  Selections are bitonic: warps sort 32 keys
-// across their lanes and merge sorted lists.  (Inserting one by one into a list per warp: 335 us for 512 rows of 129280 bf16
-// logits, 8 alternatives; one row, f32, 20 alternatives: 59 us.)
+// maximum reaches that bar and appends what does to a list in shared memory, about n elements per round on logits in no
+// particular order, and no barrier in the loop.  Where the list overflows (rising logits) the share is read once more with
+// the bar raised as needed.  Selections are bitonic: warps sort 32 keys across their lanes and merge sorted lists.
 #include <cfloat>
 #include <cooperative_groups.h>
 
@@ -28,7 +26,7 @@ namespace cg = cooperative_groups;
 
 constexpr int TL_THREADS = 256, TL_WARPS = TL_THREADS / 32, TL_MAX_TOP = 32, TL_LOADS = 4;
 constexpr int TL_CTAS = 3;     // per SM: 48 KB of loads in flight
-constexpr int TL_LIST = 1088;  // 32 kept + 32 threads' 32 elements
+constexpr int TL_LIST = 1088;  // 32 kept + 32 threads of 32 elements
 constexpr float TL_LOG2E = 1.4426950408889634f;
 constexpr float TL_FAR = -200.f;  // e^-200 is zero in fp32; stands for -inf, which would make 0 * -inf
 
@@ -54,9 +52,33 @@ struct Sums {  // a maximum that covers the terms (never below -FLT_MAX), sum, s
     move(to), o.move(to);
     s += o.s, u += o.u;
   }
-  __device__ __forceinline__ void add(float x) {
-    const float d = fmax_nan(x - m, TL_FAR), p = exp_fast(d);
-    s += p, u = fmaf(p, d, u);
+};
+// two fp32 values in one register pair: Blackwell's packed add, multiply and multiply-add halve the issue slots of a sum
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 both(uint64_t p) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(p));
+  return r;
+}
+struct PairSums {  // terms relative to one maximum
+  uint64_t s = 0, u = 0;
+  __device__ __forceinline__ void add(float x, float y, uint64_t minus_m) {
+    uint64_t d, t, p;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(pair(x, y)), "l"(minus_m));
+    const float2 f = both(d);
+    d = pair(fmax_nan(f.x, TL_FAR), fmax_nan(f.y, TL_FAR));
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(t) : "l"(d), "l"(pair(TL_LOG2E, TL_LOG2E)));
+    const float2 e = both(t);
+    float2 v;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(v.x) : "f"(e.x));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(v.y) : "f"(e.y));
+    p = pair(v.x, v.y);
+    asm("add.rn.f32x2 %0, %0, %1;" : "+l"(s) : "l"(p));
+    asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(u) : "l"(p), "l"(d));
   }
 };
 
@@ -153,134 +175,189 @@ struct Vec {
   }
 };
 
+// A CTA's share of a row: 16-byte vectors (the first and the last of the row may reach over its ends), in rounds of
+// TL_LOADS per thread, upwards.
+template <typename T>
+struct Share {
+  const T* row;
+  int vocab, shift, ctas, rank, rounds;
+  __device__ __forceinline__ Share(const T* r, int n, int c, int k) : row(r), vocab(n), ctas(c), rank(k) {
+    shift = (int)(reinterpret_cast<uintptr_t>(r) % 16 / sizeof(T));
+    rounds = ((n + shift + Vec<T>::PER - 1) / Vec<T>::PER + c * TL_LOADS * TL_THREADS - 1) / (c * TL_LOADS * TL_THREADS);
+  }
+  __device__ __forceinline__ int index(int round, int k) const {  // of the first element of a thread's k-th vector
+    return (((round * ctas + rank) * TL_LOADS + k) * TL_THREADS + (int)threadIdx.x) * Vec<T>::PER - shift;
+  }
+  __device__ __forceinline__ void fetch(Vec<T> (&v)[TL_LOADS], int round) const {
+#pragma unroll
+    for (int k = 0; k < TL_LOADS; ++k) v[k].load(row, index(round, k), vocab);
+  }
+};
+
+// The best n of a round in hand: the thread's own best, and its elements that reach a bar, appended to a list.
+template <typename T>
+__device__ __forceinline__ Key best_of(const Share<T>& sh, const Vec<T> (&v)[TL_LOADS], int round, float most) {
+  Key best = 0;
+#pragma unroll
+  for (int k = TL_LOADS - 1; k >= 0; --k)
+#pragma unroll
+    for (int j = Vec<T>::PER - 1; j >= 0; --j) {
+      const int i = sh.index(round, k) + j;
+      if (v[k].at(j) == most && i >= 0 && i < sh.vocab) best = key_of(most, i);
+    }
+  return best;
+}
+template <typename T>
+__device__ __forceinline__ void offer(const Share<T>& sh, const Vec<T>& v, int first, Key bar, float bar_value, Key* list, int base, int* count) {
+#pragma unroll
+  for (int j = 0; j < Vec<T>::PER; ++j) {
+    const float x = v.at(j);
+    const int i = first + j;
+    if (x >= bar_value && i >= 0 && i < sh.vocab && key_of(x, i) >= bar) {
+      const int at = base + atomicAdd(count, 1);
+      if (at < TL_LIST) list[at] = key_of(x, i);
+    }
+  }
+}
+
+// The careful selection, for rows whose list overflowed: over the share once more, the bar raised in every round that would
+// overflow the list, from the list and the threads' own best together (at most n threads reach it, so at most 32 n elements).
+// Returns the length of the list.  `added`: three counters for the rounds in turn (one counted, one still read, one cleared).
+template <typename T>
+__device__ __noinline__ int select_carefully(const Share<T> sh, int top, Key* list, Key (*lists)[32], int* added) {
+  constexpr int CHUNKS = (TL_LIST + TL_THREADS - 1) / TL_THREADS;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  int held = 0;
+  Key bar = 0;
+  float bar_value = -INFINITY;
+  __syncthreads();
+  if (tid < 3) added[tid] = 0;
+  __syncthreads();
+  for (int round = 0; round < sh.rounds; ++round) {
+    Vec<T> v[TL_LOADS];
+    sh.fetch(v, round);
+    float most = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < TL_LOADS; ++k) most = fmaxf(most, v[k].top());
+    int* count = &added[round % 3];
+    if (tid == 0) added[(round + 1) % 3] = 0;
+    auto offer_all = [&](int base) {
+      if (most >= bar_value)
+        for (int k = 0; k < TL_LOADS; ++k) offer(sh, v[k], sh.index(round, k), bar, bar_value, list, base, count);
+    };
+    if (round > 0) {
+      offer_all(held);
+      __syncthreads();
+      const int n = *count;
+      if (held + n <= TL_LIST) {
+        held += n;
+        continue;
+      }
+    }
+    Key mine = sort32(best_of(sh, v, round, most), lane);  // what the round has added to the list is given up
+    for (int at = warp * 32; at < held; at += TL_THREADS) mine = merge32(mine, sort32(at + lane < held ? list[at + lane] : 0, lane), lane);
+    merge_block(mine, lists, warp, lane);
+    bar = lists[0][top - 1], bar_value = value_of(bar);
+    Key kept[CHUNKS];
+#pragma unroll
+    for (int c = 0; c < CHUNKS; ++c) kept[c] = c * TL_THREADS + tid < held ? list[c * TL_THREADS + tid] : 0;
+    if (tid == 0) *count = 0;
+    __syncthreads();
+#pragma unroll
+    for (int c = 0; c < CHUNKS; ++c)
+      if (kept[c] && kept[c] >= bar) list[atomicAdd(count, 1)] = kept[c];
+    offer_all(0);
+    __syncthreads();
+    held = *count;
+  }
+  return held;
+}
+
 template <typename T, bool TOP>
 __global__ void __launch_bounds__(TL_THREADS, TL_CTAS) token_logprobs_kernel(const T* __restrict__ logits, long long stride, int vocab,
-                                                                    const int32_t* __restrict__ tokens, int top, float* __restrict__ logprobs,
-                                                                    float* __restrict__ entropy, int32_t* __restrict__ top_ids,
-                                                                    float* __restrict__ top_logprobs, int* status) {
+                                                                             const int32_t* __restrict__ tokens, int top, float* __restrict__ logprobs,
+                                                                             float* __restrict__ entropy, int32_t* __restrict__ top_ids,
+                                                                             float* __restrict__ top_logprobs, int* status) {
   using V = Vec<T>;
   constexpr int PER = V::PER;
   __shared__ Sums parts[TL_WARPS];
   __shared__ Key lists[TOP ? TL_WARPS : 1][32];
   __shared__ Key list[TOP ? TL_LIST : 1];
-  __shared__ int added[3];  // by the rounds in turn: one is counted, one still read, one cleared
+  __shared__ int added[3];
   cg::cluster_group cluster = cg::this_cluster();
   const int ctas = cluster.num_blocks(), rank = cluster.block_rank();
   const int row = blockIdx.x / ctas, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const T* x = logits + row * stride;
-  // 16-byte vectors of the row, the first and the last may reach over its ends
-  const int shift = (int)(reinterpret_cast<uintptr_t>(x) % 16 / sizeof(T));
-  const int vectors = (vocab + shift + PER - 1) / PER;
-  const int rounds = (vectors + ctas * TL_LOADS * TL_THREADS - 1) / (ctas * TL_LOADS * TL_THREADS);
-  auto vector_of = [&](int round, int k) { return ((round * ctas + rank) * TL_LOADS + k) * TL_THREADS + tid; };
+  const Share<T> sh(x, vocab, ctas, rank);
 
   Sums sum{-FLT_MAX, 0.f, 0.f};
-  int held = 0;          // length of the list
-  Key bar = 0;           // nothing below it is among the best
+  Key bar = 0;  // nothing below it is among the best
   float bar_value = -INFINITY;
-  if (TOP && tid < 3) added[tid] = 0;
-
   V next[TL_LOADS];
-  auto fetch = [&](int round) {
-#pragma unroll
-    for (int k = 0; k < TL_LOADS; ++k) next[k].load(x, vector_of(round, k) * PER - shift, vocab);
-  };
-  fetch(0);
-  for (int round = 0; round < rounds; ++round) {
+  sh.fetch(next, 0);
+  if (TOP && tid == 0) added[0] = 0;
+  for (int round = 0; round < sh.rounds; ++round) {
     V now[TL_LOADS];
-    float most = -INFINITY;
+    float tops[TL_LOADS], most = -INFINITY;
 #pragma unroll
-    for (int k = 0; k < TL_LOADS; ++k) now[k] = next[k], most = fmaxf(most, now[k].top());
-    if (round + 1 < rounds) fetch(round + 1);
+    for (int k = 0; k < TL_LOADS; ++k) now[k] = next[k], tops[k] = now[k].top(), most = fmaxf(most, tops[k]);
+    if (round + 1 < sh.rounds) sh.fetch(next, round + 1);
     if (most > sum.m) sum.move(most);
+    PairSums part;
+    const uint64_t minus_m = pair(-sum.m, -sum.m);
 #pragma unroll
     for (int k = 0; k < TL_LOADS; ++k)
 #pragma unroll
-      for (int j = 0; j < PER; ++j) sum.add(now[k].at(j));
+      for (int j = 0; j < PER; j += 2) part.add(now[k].at(j), now[k].at(j + 1), minus_m);
+    const float2 s2 = both(part.s), u2 = both(part.u);
+    sum.s += s2.x + s2.y, sum.u += u2.x + u2.y;
     if constexpr (TOP) {
-      int* count = &added[round % 3];
-      if (tid == 0) added[(round + 1) % 3] = 0;
-      auto push = [&](Key k, int base, int limit) {
-        const int at = base + atomicAdd(count, 1);
-        if (at < limit) list[at] = k;
-      };
-      auto offer = [&](int base) {  // this thread's elements that reach the bar
-        if (!(most >= bar_value)) return;
-#pragma unroll
-        for (int k = 0; k < TL_LOADS; ++k) {
-          if (!(now[k].top() >= bar_value)) continue;
-#pragma unroll
-          for (int j = 0; j < PER; ++j) {
-            const float v = now[k].at(j);
-            const int i = vector_of(round, k) * PER - shift + j;
-            if (v >= bar_value && i >= 0 && i < vocab && key_of(v, i) >= bar) push(key_of(v, i), base, TL_LIST);
-          }
-        }
-      };
-      bool raise = round == 0;
-      if (!raise) {
-        offer(held);
-        __syncthreads();
-        const int n = *count;
-        if (held + n > TL_LIST) raise = true;
-        else held += n;
-      }
-      if (raise) {  // (the round's entries of the list, if any, are given up)
-        Key best = 0;
-#pragma unroll
-        for (int k = TL_LOADS - 1; k >= 0; --k)
-#pragma unroll
-          for (int j = PER - 1; j >= 0; --j) {
-            const int i = vector_of(round, k) * PER - shift + j;
-            if (now[k].at(j) == most && i >= 0 && i < vocab) best = key_of(most, i);
-          }
-        Key mine = sort32(best, lane);
-        for (int at = warp * 32; at < held; at += TL_THREADS) mine = merge32(mine, sort32(at + lane < held ? list[at + lane] : 0, lane), lane);
-        merge_block(mine, lists, warp, lane);
+      if (round == 0) {
+        merge_block(sort32(best_of(sh, now, 0, most), lane), lists, warp, lane);
         bar = lists[0][top - 1], bar_value = value_of(bar);
-        Key kept[(TL_LIST + TL_THREADS - 1) / TL_THREADS];
+      }
+      if (most >= bar_value) {
 #pragma unroll
-        for (int c = 0; c < (TL_LIST + TL_THREADS - 1) / TL_THREADS; ++c) kept[c] = c * TL_THREADS + tid < held ? list[c * TL_THREADS + tid] : 0;
-        if (tid == 0) *count = 0;
-        __syncthreads();
-#pragma unroll
-        for (int c = 0; c < (TL_LIST + TL_THREADS - 1) / TL_THREADS; ++c)
-          if (kept[c] && kept[c] >= bar) push(kept[c], 0, TL_LIST);
-        offer(0);
-        __syncthreads();
-        held = *count;
+        for (int k = 0; k < TL_LOADS; ++k)
+          if (tops[k] >= bar_value) offer(sh, now[k], sh.index(round, k), bar, bar_value, list, 0, added);
       }
     }
   }
 
   // ---- warps, then CTAs ----
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    Sums other{__shfl_xor_sync(0xffffffffu, sum.m, o), __shfl_xor_sync(0xffffffffu, sum.s, o), __shfl_xor_sync(0xffffffffu, sum.u, o)};
-    sum.join(other);
-  }
+  auto join_lanes = [&](int from) {
+    for (int o = from; o > 0; o >>= 1) {
+      Sums other{__shfl_xor_sync(0xffffffffu, sum.m, o), __shfl_xor_sync(0xffffffffu, sum.s, o), __shfl_xor_sync(0xffffffffu, sum.u, o)};
+      sum.join(other);
+    }
+  };
+  join_lanes(16);
   if (lane == 0) parts[warp] = sum;
   Key best = 0;
+  __syncthreads();
   if constexpr (TOP) {
+    int held = added[0];
+    if (held > TL_LIST) held = select_carefully(sh, top, list, lists, added);
     for (int at = warp * 32; at < held; at += TL_THREADS) best = merge32(best, sort32(at + lane < held ? list[at + lane] : 0, lane), lane);
     best = merge_block(best, lists, warp, lane);
-  } else {
-    __syncthreads();
   }
   if (warp == 0) {
-    for (int w = 1; w < TL_WARPS; ++w) sum.join(parts[w]);
-    __syncwarp();
-    if (lane == 0) parts[0] = sum;
+    sum = parts[lane % TL_WARPS];
+    join_lanes(TL_WARPS / 2);
   }
-  if (ctas > 1) {
+  if (ctas > 1) {  // ctas <= TL_WARPS: a warp for each CTA's list, lanes for their sums
+    __syncthreads();
+    if (tid == 0) parts[0] = sum;
     cluster.sync();
-    if (rank == 0 && warp == 0) {
-      for (int c = 1; c < ctas; ++c) {
-        sum.join(*cluster.map_shared_rank(&parts[0], c));
-        if (TOP) best = merge32(best, *cluster.map_shared_rank(&lists[0][lane], c), lane);
+    if (rank == 0) {
+      if (TOP && warp < ctas) best = *cluster.map_shared_rank(&lists[0][lane], warp);
+      if (warp == 0) {
+        sum = *cluster.map_shared_rank(&parts[0], lane % ctas);
+        join_lanes(ctas / 2);
       }
     }
-    cluster.sync();  // nobody leaves before its shared memory has been read
+    cluster.sync();  // nobody leaves, and no list is written, before all have been read
+    if (TOP && rank == 0) best = merge_block(warp < ctas ? best : 0, lists, warp, lane);
   }
   if (rank == 0 && warp == 0) {
     const float log_s = logf(sum.s);
