@@ -11,10 +11,12 @@
 // The alternatives are kept as 64-bit keys (value mapped to an ordered integer, complement of the index: all distinct,
 // ties to the lower index).  The first round of a CTA finds the n-th largest of its 256 threads' own maxima, a lower
 // bound of the n-th best that only about n of the round's elements reach; from then on a thread looks closer only when its
-// maximum reaches that bar and appends what does to a list in shared memory, about n elements per round on logits in no
-// particular order, and no barrier in the loop.  Where the list overflows (rising logits) the share is read once more with
-// the bar raised as needed.  Selections are bitonic: warps sort 32 keys across their lanes and merge sorted lists.
+// maximum reaches that bar and appends what does to a list in shared memory.  After 2, 4, 8 .. rounds the bar is taken from
+// the list again, so about n elements are appended per doubling on logits in no particular order.  Where the list
+// overflows (rising logits, many equal ones) the share is read once more with the bar raised as needed.
+// Selections are bitonic: warps sort 32 keys across their lanes and merge sorted lists.
 #include <cfloat>
+#include <cmath>
 #include <cooperative_groups.h>
 
 #include "common.cuh"
@@ -25,7 +27,7 @@ namespace {
 namespace cg = cooperative_groups;
 
 constexpr int TL_THREADS = 256, TL_WARPS = TL_THREADS / 32, TL_MAX_TOP = 32, TL_LOADS = 4;
-constexpr int TL_CTAS = 3;     // per SM: 48 KB of loads in flight
+constexpr int TL_CTAS = 4;     // per SM: up to 64 KB of loads in flight
 constexpr int TL_LIST = 1088;  // 32 kept + 32 threads of 32 elements
 constexpr float TL_LOG2E = 1.4426950408889634f;
 constexpr float TL_FAR = -200.f;  // e^-200 is zero in fp32; stands for -inf, which would make 0 * -inf
@@ -83,13 +85,14 @@ struct PairSums {  // terms relative to one maximum
 };
 
 using Key = unsigned long long;  // 0: none
-__device__ __forceinline__ Key key_of(float v, int i) {
+__device__ __forceinline__ unsigned order_of(float v) {
   const unsigned b = __float_as_uint(v + 0.f);  // -0 counts as 0
-  return (Key)(b >> 31 ? ~b : b | 0x80000000u) << 32 | (unsigned)~i;
+  return b >> 31 ? ~b : b | 0x80000000u;
 }
+__device__ __forceinline__ float value_of(unsigned b) { return b ? __uint_as_float(b >> 31 ? b ^ 0x80000000u : ~b) : -INFINITY; }
+__device__ __forceinline__ Key key_of(float v, int i) { return (Key)order_of(v) << 32 | (unsigned)~i; }
 __device__ __forceinline__ float value_of(Key k) {
-  const unsigned b = (unsigned)(k >> 32);
-  return k ? __uint_as_float(b >> 31 ? b ^ 0x80000000u : ~b) : -INFINITY;
+  return value_of((unsigned)(k >> 32));
 }
 __device__ __forceinline__ int index_of(Key k) { return k ? (int)~(unsigned)k : -1; }
 
@@ -112,8 +115,28 @@ __device__ __forceinline__ Key merge32(Key a, Key b, int lane) {
   for (int j = 16; j > 0; j >>= 1) x = swap_step(x, lane, j, true);
   return x;
 }
+// the same of 32-bit keys (values alone), for bars
+__device__ __forceinline__ unsigned swap_step(unsigned x, int lane, int j, bool down) {
+  const unsigned y = __shfl_xor_sync(0xffffffffu, x, j);
+  return ((lane & j) == 0) == down ? max(x, y) : min(x, y);
+}
+__device__ __forceinline__ unsigned sort32(unsigned x, int lane) {
+#pragma unroll
+  for (int k = 2; k <= 32; k <<= 1)
+#pragma unroll
+    for (int j = k >> 1; j > 0; j >>= 1) x = swap_step(x, lane, j, (lane & k) == 0);
+  return x;
+}
+__device__ __forceinline__ unsigned merge32(unsigned a, unsigned b, int lane) {
+  unsigned x = max(a, __shfl_sync(0xffffffffu, b, 31 - lane));
+#pragma unroll
+  for (int j = 16; j > 0; j >>= 1) x = swap_step(x, lane, j, true);
+  return x;
+}
+
 // ... of the warps' sorted lists, in warp 0 and in lists[0]
-__device__ __forceinline__ Key merge_block(Key x, Key (*lists)[32], int warp, int lane) {
+template <typename K>
+__device__ __forceinline__ K merge_block(K x, K (*lists)[32], int warp, int lane) {
   lists[warp][lane] = x;
 #pragma unroll
   for (int step = 1; step < TL_WARPS; step <<= 1) {
@@ -212,10 +235,13 @@ __device__ __forceinline__ void offer(const Share<T>& sh, const Vec<T>& v, int f
 #pragma unroll
   for (int j = 0; j < Vec<T>::PER; ++j) {
     const float x = v.at(j);
-    const int i = first + j;
-    if (x >= bar_value && i >= 0 && i < sh.vocab && key_of(x, i) >= bar) {
-      const int at = base + atomicAdd(count, 1);
-      if (at < TL_LIST) list[at] = key_of(x, i);
+    if (x >= bar_value) {
+      const int i = first + j;
+      const Key key = key_of(x, i);
+      if (i >= 0 && i < sh.vocab && key >= bar) {
+        const int at = base + atomicAdd(count, 1);
+        if (at < TL_LIST) list[at] = key;
+      }
     }
   }
 }
@@ -284,6 +310,7 @@ __global__ void __launch_bounds__(TL_THREADS, TL_CTAS) token_logprobs_kernel(con
   __shared__ Key lists[TOP ? TL_WARPS : 1][32];
   __shared__ Key list[TOP ? TL_LIST : 1];
   __shared__ int added[3];
+  unsigned(*bars)[32] = reinterpret_cast<unsigned(*)[32]>(lists);
   cg::cluster_group cluster = cg::this_cluster();
   const int ctas = cluster.num_blocks(), rank = cluster.block_rank();
   const int row = blockIdx.x / ctas, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -291,11 +318,16 @@ __global__ void __launch_bounds__(TL_THREADS, TL_CTAS) token_logprobs_kernel(con
   const Share<T> sh(x, vocab, ctas, rank);
 
   Sums sum{-FLT_MAX, 0.f, 0.f};
-  Key bar = 0;  // nothing below it is among the best
-  float bar_value = -INFINITY;
+  float bar = -INFINITY;  // nothing below it is among the best
   V next[TL_LOADS];
   sh.fetch(next, 0);
   if (TOP && tid == 0) added[0] = 0;
+  auto nth = [&](unsigned sorted) {  // of the warps' sorted values the n-th largest
+    merge_block(sorted, bars, warp, lane);
+    const unsigned r = bars[0][top - 1];
+    __syncthreads();
+    return r;
+  };
   for (int round = 0; round < sh.rounds; ++round) {
     V now[TL_LOADS];
     float tops[TL_LOADS], most = -INFINITY;
@@ -312,14 +344,21 @@ __global__ void __launch_bounds__(TL_THREADS, TL_CTAS) token_logprobs_kernel(con
     const float2 s2 = both(part.s), u2 = both(part.u);
     sum.s += s2.x + s2.y, sum.u += u2.x + u2.y;
     if constexpr (TOP) {
-      if (round == 0) {
-        merge_block(sort32(best_of(sh, now, 0, most), lane), lists, warp, lane);
-        bar = lists[0][top - 1], bar_value = value_of(bar);
-      }
-      if (most >= bar_value) {
+      if (round == 0) bar = value_of(nth(sort32(order_of(most), lane)));
+      if (most >= bar) {
 #pragma unroll
         for (int k = 0; k < TL_LOADS; ++k)
-          if (tops[k] >= bar_value) offer(sh, now[k], sh.index(round, k), bar, bar_value, list, 0, added);
+          if (tops[k] >= bar) offer(sh, now[k], sh.index(round, k), 0, bar, list, 0, added);
+      }
+      if (round > 0 && (round & (round + 1)) == 0 && round + 1 < sh.rounds) {  // as many rounds ahead as behind: the bar from the list
+        __syncthreads();
+        const int held = added[0];
+        if (held <= TL_LIST) {
+          unsigned mine = 0;
+          for (int at = warp * 32; at < held; at += TL_THREADS)
+            mine = merge32(mine, sort32(at + lane < held ? (unsigned)(list[at + lane] >> 32) : 0u, lane), lane);
+          bar = fmaxf(bar, value_of(nth(mine)));
+        }
       }
     }
   }
@@ -404,8 +443,13 @@ extern "C" int cachalot_token_logprobs(const void* logits, int dtype, int64_t ro
   if (!aligned(logits, es)) return fail(CACHALOT_EALIGN, "token_logprobs: logits are not aligned to their type");
   if (vocab > 0x7fffffff - 131072) return fail(CACHALOT_EUNSUPPORTED, "token_logprobs: vocabulary of %d", vocab);
   // CTAs of a row: enough to fill the GPU with few rows, a power of two up to the portable cluster size
+  const double slots = 148.0 * TL_CTAS, row_us = (double)vocab * es / 16e3, fixed_us = top ? 3.0 : 1.0;  // a CTA: 16 GB/s, and its joins
   int ctas = 1;
-  while (ctas < 8 && (long long)rows * ctas * 2 <= 1184 && (long long)vocab * es / ctas > 32768) ctas *= 2;
+  double least = 1e30;
+  for (int c = 1; c <= TL_WARPS; c *= 2) {
+    const double us = ceil((double)rows * c / slots) * (row_us / c + fixed_us);
+    if (us < least) least = us, ctas = c;
+  }
   if ((long long)rows * ctas > 0x7fffffffLL) return fail(CACHALOT_EUNSUPPORTED, "token_logprobs: %d rows", rows);
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeClusterDimension;
