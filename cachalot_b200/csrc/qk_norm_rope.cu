@@ -6,17 +6,25 @@
 //   one rounding at the end, to the activation type or to E4M3 of y / scale (saturated at 448)
 //
 // HBM-bound: 2 bytes in and 2 (or 1) out per element.  A head is a group of 8, 16 or 32 lanes with 8 elements (16 bytes)
-// each, so the norm is a shuffle tree and interleaved pairs sit in one lane; the half layout fetches the partner through
-// shared memory.  A CTA works on one token, so its angles are computed once for all of its heads: position * frequency in
-// 64 bits, reduced to a fraction of a turn there (a float product is off by 0.06 rad at position 10^6), then sincospif.
+// each, so the norm is a shuffle tree.  A CTA works on one token, so everything but the norm is the same for all of its
+// heads: an output element is r (x A + p B), r the head's 1 / rms, p the partner element, A = m w cos, B = -/+ m w_p sin
+// in registers.  Interleaved partners are in the same lane; those of the half layout are a second 16-byte load that hits
+// L1 (fp32 values handed through shared memory instead: 365 instead of about 100 instructions per two heads, 124 us for
+// 4096 tokens of 64 + 16 + 16 heads of 128).  Pairs that straddle 16-byte pieces are fetched element by element.
+// Angles are computed once per token: position * frequency in 64 bits, reduced to a fraction of a turn there (a float
+// product is off by 0.06 rad at position 10^6), then sincospif.
 #include <cuda_fp8.h>
 
+#include <type_traits>
+
 #include "paged.cuh"
+#include "pairs.cuh"
 
 namespace cachalot {
 namespace {
 
-constexpr int QR_THREADS = 256;
+constexpr int QR_THREADS = 128;
+constexpr int QR_BATCH = 2;  // query heads a group works on while it has as many in flight
 constexpr int QR_MAX_DIM = 256;
 
 struct Rows {  // activation rows, strides in elements
@@ -32,77 +40,188 @@ struct RopeArgs {
   const double* inv_freq;
   int half, interleaved;
   int heads, kv_heads, dim;
+  float inv_dim;
   void *q_out, *k_out;
   PagedView cache;  // cache.k null: none
   const int32_t* slots;
   int* status;
 };
 
+// 16 bytes of activations as four pairs, and back
 template <typename T>
-__device__ __forceinline__ void widen8(const uint4& u, float (&f)[8]) {
+__device__ __forceinline__ void widen8(const uint4& u, f32x2 (&f)[4]) {
   const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    if constexpr (sizeof(T) == 2 && std::is_same<T, __half>::value) {
+    if constexpr (std::is_same<T, __half>::value) {
       const float2 p = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-      f[2 * i] = p.x, f[2 * i + 1] = p.y;
+      f[i] = pair(p.x, p.y);
     } else {
-      f[2 * i] = __uint_as_float(w[i] << 16), f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+      f[i] = pair(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
     }
   }
 }
 template <typename T>
-__device__ __forceinline__ uint4 round8(const float (&f)[8]) {
+__device__ __forceinline__ uint4 round8(const f32x2 (&f)[4]) {
   uint32_t w[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
+    const float2 v = both(f[i]);
     if constexpr (std::is_same<T, __half>::value) {
-      const __half2 h = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
+      const __half2 h = __floats2half2_rn(v.x, v.y);
       w[i] = *reinterpret_cast<const uint32_t*>(&h);
     } else {
-      const __nv_bfloat162 h = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+      const __nv_bfloat162 h = __floats2bfloat162_rn(v.x, v.y);
       w[i] = *reinterpret_cast<const uint32_t*>(&h);
     }
   }
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
-__device__ __forceinline__ uint2 e4m3_8(const float (&f)[8]) {
+__device__ __forceinline__ uint2 e4m3_8(const f32x2 (&f)[4]) {
   uint32_t b[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-    b[i] = __nv_cvt_float2_to_fp8x2(make_float2(f[2 * i], f[2 * i + 1]), __NV_SATFINITE, __NV_E4M3);
+  for (int i = 0; i < 4; ++i) b[i] = __nv_cvt_float2_to_fp8x2(both(f[i]), __NV_SATFINITE, __NV_E4M3);
   return make_uint2(b[0] | b[1] << 16, b[2] | b[3] << 16);
 }
+// elements at .. at + 8 of a norm weight, 1 without one
 template <typename T>
-__device__ __forceinline__ void weights8(const void* w, int f32, int at, bool live, float (&f)[8]) {
+__device__ __forceinline__ float weight(const void* w, int f32, int at) {
+  if (!w) return 1.f;
+  if (f32) return static_cast<const float*>(w)[at];
+  if constexpr (std::is_same<T, __half>::value) return __half2float(static_cast<const T*>(w)[at]);
+  else return __bfloat162float(static_cast<const T*>(w)[at]);
+}
+template <typename T>
+__device__ __forceinline__ void weights8(const void* w, int f32, int at, f32x2 (&f)[4]) {
+  if (!w) {
 #pragma unroll
-  for (int e = 0; e < 8; ++e) f[e] = 1.f;
-  if (!w || !live) return;
-  if (f32) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) f[e] = static_cast<const float*>(w)[at + e];
+    for (int i = 0; i < 4; ++i) f[i] = pair(1.f, 1.f);
+  } else if (f32) {
+    const float4 a = static_cast<const float4*>(w)[at / 4], b = static_cast<const float4*>(w)[at / 4 + 1];
+    f[0] = pair(a.x, a.y), f[1] = pair(a.z, a.w), f[2] = pair(b.x, b.y), f[3] = pair(b.z, b.w);
   } else {
     widen8<T>(*reinterpret_cast<const uint4*>(static_cast<const T*>(w) + at), f);
   }
 }
+__device__ __forceinline__ f32x2 swapped(f32x2 p) {
+  const float2 v = both(p);
+  return pair(v.y, v.x);
+}
 
-template <typename T, int L>
-__global__ void __launch_bounds__(QR_THREADS) qk_norm_rope_kernel(RopeArgs a) {
+enum { PAIRS_ADJACENT, PAIRS_HALF, PAIRS_ANY };  // (2i, 2i+1) and (i, i+r/2) in whole 16-byte pieces; element by element
+
+template <typename T, int L, int PAIRS>
+struct Lane {  // what a lane does to its 8 elements of a query or key head
+  f32x2 a[4], b[4];
+  bool rotated;  // any of them
+  int partner;   // first element of the piece the partners are in
+  int half, at, adjacent;
+
+  __device__ __forceinline__ void set(const void* w, int f32, const float* cs, const float* sn) {
+    weights8<T>(w, f32, at, a);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) b[i] = pair(0.f, 0.f);
+    if constexpr (PAIRS == PAIRS_ANY) {
+      float x[8], z[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int i = at + e, k = adjacent ? i >> 1 : i < half ? i : i - half, j = mate(i);
+        const bool turns = i < 2 * half;
+        x[e] = weight<T>(w, f32, i) * (turns ? cs[k] : 1.f);
+        z[e] = turns ? weight<T>(w, f32, j) * (j > i ? -sn[k] : sn[k]) : 0.f;
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) a[i] = pair(x[2 * i], x[2 * i + 1]), b[i] = pair(z[2 * i], z[2 * i + 1]);
+    } else if (rotated) {
+      if constexpr (PAIRS == PAIRS_ADJACENT) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float c = cs[at / 2 + i], s = sn[at / 2 + i];
+          b[i] = mul2(swapped(a[i]), pair(-s, s)), a[i] = mul2(a[i], pair(c, c));
+        }
+      } else {
+        f32x2 other[4];
+        weights8<T>(w, f32, partner, other);
+        const int k = at < half ? at : partner;
+        const float sign = at < half ? -1.f : 1.f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float2 c = *reinterpret_cast<const float2*>(cs + k + 2 * i), s = *reinterpret_cast<const float2*>(sn + k + 2 * i);
+          a[i] = mul2(a[i], pair(c.x, c.y)), b[i] = mul2(other[i], pair(sign * s.x, sign * s.y));
+        }
+      }
+    }
+  }
+  __device__ __forceinline__ int mate(int i) const { return adjacent ? i ^ 1 : i < half ? i + half : i - half; }
+
+  // y <- (y A + p B) / rms (or without the norm), `times` a factor on top; `piece`: the partner's, `row`: the head in memory
+  __device__ __forceinline__ void apply(f32x2 (&y)[4], const uint4& piece, const T* row, bool normed, float eps, float inv_dim, float times) const {
+    float r = times;
+    if (normed) {
+      f32x2 s2 = mul2(y[0], y[0]);
+#pragma unroll
+      for (int i = 1; i < 4; ++i) s2 = fma2(y[i], y[i], s2);
+      float ss = both(s2).x + both(s2).y;
+#pragma unroll
+      for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+      r *= rsqrtf(fmaf(ss, inv_dim, eps));
+    }
+    const f32x2 r2 = pair(r, r);
+    if (PAIRS != PAIRS_ANY && !rotated) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) y[i] = mul2(y[i], mul2(a[i], r2));
+      return;
+    }
+    f32x2 p[4];
+    if constexpr (PAIRS == PAIRS_ADJACENT) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) p[i] = swapped(y[i]);
+    } else if constexpr (PAIRS == PAIRS_HALF) {
+      widen8<T>(piece, p);
+    } else {
+      float v[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = row && at + e < 2 * half ? weight<T>(row, 0, mate(at + e)) : 0.f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) p[i] = pair(v[2 * i], v[2 * i + 1]);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) y[i] = mul2(r2, fma2(p[i], b[i], mul2(y[i], a[i])));
+  }
+};
+
+template <typename T, int L, int PAIRS>
+__global__ void __launch_bounds__(QR_THREADS) qk_norm_rope_kernel(const RopeArgs a) {
   constexpr int GROUPS = QR_THREADS / L;
   __shared__ __align__(16) float cs[QR_MAX_DIM / 2], sn[QR_MAX_DIM / 2];
-  __shared__ __align__(16) float swap[GROUPS][2][L][4];  // a lane's elements 0-3 and 4-7 apart: no bank conflicts
-  const int token = blockIdx.x, group = threadIdx.x / L, lane = threadIdx.x % L;
-  const int at = lane * 8, half = a.half;
-  const bool in_head = at < a.dim;
+  const int token = blockIdx.x, group = threadIdx.x / L, half = a.half;
+  const int step = GROUPS * gridDim.y, first = blockIdx.y * GROUPS + group;
+  Lane<T, L, PAIRS> ln;
+  ln.at = threadIdx.x % L * 8, ln.half = half, ln.adjacent = a.interleaved;
+  const bool live = ln.at < a.dim;
+  const int at = live ? ln.at : 0;  // lanes past the head read its first piece and count as zeros
+  ln.at = at, ln.rotated = at < 2 * half;
+  ln.partner = PAIRS != PAIRS_HALF || !ln.rotated ? at : at < half ? at + half : at - half;
+  // the first query heads are on their way while the angles are computed
+  const T* q = static_cast<const T*>(a.q.x) + token * a.q.token;
+  T* q_out = static_cast<T*>(a.q_out) + (long long)token * a.heads * a.dim + at;
+  uint4 ahead[QR_BATCH], ahead_piece[QR_BATCH];
+  auto fetch = [&](int h0) {
+#pragma unroll
+    for (int i = 0; i < QR_BATCH; ++i) {
+      const int h = h0 + i * step;
+      const bool there = live && h < a.heads;
+      ahead[i] = there ? *reinterpret_cast<const uint4*>(q + h * a.q.head + at) : make_uint4(0, 0, 0, 0);
+      ahead_piece[i] = there && PAIRS == PAIRS_HALF ? *reinterpret_cast<const uint4*>(q + h * a.q.head + ln.partner) : make_uint4(0, 0, 0, 0);
+    }
+  };
+  fetch(first);
   for (int i = threadIdx.x; i < half; i += QR_THREADS) {
     const double turns = (double)a.positions[token] * a.inv_freq[i] * 0.15915494309189533577;  // 1 / (2 pi)
     float s, c;
     sincospif(2.0f * (float)(turns - rint(turns)), &s, &c);
     cs[i] = c * a.magnitude, sn[i] = s * a.magnitude;
   }
-  float wq[8], wk[8];
-  weights8<T>(a.q_weight, a.w_f32, at, in_head, wq);
-  weights8<T>(a.k_weight, a.w_f32, at, in_head, wk);
   long long page = 0;
   int off = 0;
   bool stored = false;
@@ -114,81 +233,58 @@ __global__ void __launch_bounds__(QR_THREADS) qk_norm_rope_kernel(RopeArgs a) {
     if (stored) page = slot / a.cache.page_size, off = slot - (int)page * a.cache.page_size;
   }
   const bool f8 = a.cache.dtype == CACHALOT_E4M3;
-  const int es = f8 ? 1 : 2;
-  const int k_from = a.heads, v_from = a.heads + (stored || a.k_out ? a.kv_heads : 0), items = v_from + (stored ? a.kv_heads : 0);
   __syncthreads();
-  for (int base = blockIdx.y * GROUPS; base < items; base += gridDim.y * GROUPS) {
-    const int it = base + group;
-    const bool live = it < items && in_head;
-    const int what = it < k_from ? 0 : it < v_from ? 1 : 2;
-    const int h = it - (what == 0 ? 0 : what == 1 ? k_from : v_from);
-    uint4 raw = make_uint4(0, 0, 0, 0);
-    if (live) {
-      const Rows& r = what == 0 ? a.q : what == 1 ? a.k : a.v;
-      raw = *reinterpret_cast<const uint4*>(static_cast<const T*>(r.x) + token * r.token + h * r.head + at);
+  ln.set(a.q_weight, a.w_f32, cs, sn);
+  const uint4 zero = make_uint4(0, 0, 0, 0);
+  for (int h0 = first;;) {
+    uint4 own[QR_BATCH], piece[QR_BATCH];
+#pragma unroll
+    for (int i = 0; i < QR_BATCH; ++i) own[i] = ahead[i], piece[i] = ahead_piece[i];
+    const int next = h0 + QR_BATCH * step;
+    const bool more = next - group < a.heads;
+    if (more) fetch(next);
+#pragma unroll
+    for (int i = 0; i < QR_BATCH; ++i) {
+      const int h = h0 + i * step;
+      if (h - group >= a.heads) break;
+      const bool there = live && h < a.heads;
+      f32x2 y[4];
+      widen8<T>(own[i], y);
+      ln.apply(y, piece[i], there ? q + h * a.q.head : nullptr, a.q_weight != nullptr, a.eps, a.inv_dim, 1.f);
+      if (there) *reinterpret_cast<uint4*>(q_out + h * a.dim) = round8<T>(y);
     }
-    float y[8];
-    widen8<T>(raw, y);
-    float ss = 0.f;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) ss = fmaf(y[e], y[e], ss);
-#pragma unroll
-    for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-    const bool normed = what == 0 ? a.q_weight != nullptr : what == 1 && a.k_weight != nullptr;
-    if (normed) {
-      const float inv = rsqrtf(ss / (float)a.dim + a.eps);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) y[e] = y[e] * inv * (what ? wk[e] : wq[e]);
-    }
-    if (a.interleaved) {
-      if (what < 2) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int i = lane * 4 + e;
-          if (i < half) {
-            const float u = y[2 * e], v = y[2 * e + 1];
-            y[2 * e] = u * cs[i] - v * sn[i], y[2 * e + 1] = v * cs[i] + u * sn[i];
-          }
-        }
-      }
-    } else {
-      float4* mine = reinterpret_cast<float4*>(&swap[group][0][lane][0]);
-      mine[0] = make_float4(y[0], y[1], y[2], y[3]);
-      mine[L] = make_float4(y[4], y[5], y[6], y[7]);
-      __syncwarp();
-      if (what < 2) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const int i = at + e;
-          if (i < 2 * half) {
-            const int j = i < half ? i + half : i - half, k = i < half ? i : j;
-            const float p = swap[group][(j >> 2) & 1][j >> 3][j & 3];
-            y[e] = i < half ? y[e] * cs[k] - p * sn[k] : y[e] * cs[k] + p * sn[k];
-          }
-        }
-      }
-      __syncwarp();
-    }
-    if (!live) continue;
-    if (what == 0) {
-      *reinterpret_cast<uint4*>(static_cast<T*>(a.q_out) + ((long long)token * a.heads + h) * a.dim + at) = round8<T>(y);
-      continue;
-    }
-    if (what == 1 && a.k_out) *reinterpret_cast<uint4*>(static_cast<T*>(a.k_out) + ((long long)token * a.kv_heads + h) * a.dim + at) = round8<T>(y);
+    if (!more) break;
+    h0 = next;
+  }
+  if (!stored && !a.k_out) return;
+  ln.set(a.k_weight, a.w_f32, cs, sn);
+  const T* k = static_cast<const T*>(a.k.x) + token * a.k.token;
+  const T* v = static_cast<const T*>(a.v.x) + token * a.v.token;
+  for (int h = first; h - group < a.kv_heads; h += step) {
+    const bool there = live && h < a.kv_heads;
+    const uint4 own = there ? *reinterpret_cast<const uint4*>(k + h * a.k.head + at) : zero;
+    const uint4 piece = there && PAIRS == PAIRS_HALF ? *reinterpret_cast<const uint4*>(k + h * a.k.head + ln.partner) : zero;
+    const uint4 value = there && stored ? *reinterpret_cast<const uint4*>(v + h * a.v.head + at) : zero;
+    f32x2 y[4];
+    widen8<T>(own, y);
+    // E4M3: times 1 / scale, one more rounding to fp32 than the division, instead of eight divisions
+    const float k_times = f8 && a.cache.k_scale && there ? 1.f / a.cache.k_scale[h] : 1.f;
+    ln.apply(y, piece, there ? k + h * a.k.head : nullptr, a.k_weight != nullptr, a.eps, a.inv_dim, k_times);
+    if (!there) continue;
+    if (a.k_out) *reinterpret_cast<uint4*>(static_cast<T*>(a.k_out) + ((long long)token * a.kv_heads + h) * a.dim + at) = round8<T>(y);
     if (!stored) continue;
-    uint8_t* row = what == 1 ? a.cache.k + page * a.cache.k_page + h * a.cache.k_head + off * a.cache.k_token
-                             : a.cache.v + page * a.cache.v_page + h * a.cache.v_head + off * a.cache.v_token;
-    row += at * es;
+    uint8_t* k_row = a.cache.k + page * a.cache.k_page + h * a.cache.k_head + off * a.cache.k_token;
+    uint8_t* v_row = a.cache.v + page * a.cache.v_page + h * a.cache.v_head + off * a.cache.v_token;
     if (f8) {
-      const float* scales = what == 1 ? a.cache.k_scale : a.cache.v_scale;
-      if (scales) {
-        const float s = scales[h];
+      *reinterpret_cast<uint2*>(k_row + at) = e4m3_8(y);
+      widen8<T>(value, y);
+      const float v_times = a.cache.v_scale ? 1.f / a.cache.v_scale[h] : 1.f;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) y[e] = y[e] / s;
-      }
-      *reinterpret_cast<uint2*>(row) = e4m3_8(y);
+      for (int i = 0; i < 4; ++i) y[i] = mul2(y[i], pair(v_times, v_times));
+      *reinterpret_cast<uint2*>(v_row + at) = e4m3_8(y);
     } else {
-      *reinterpret_cast<uint4*>(row) = what == 1 ? round8<T>(y) : raw;
+      *reinterpret_cast<uint4*>(k_row + at * 2) = round8<T>(y);
+      *reinterpret_cast<uint4*>(v_row + at * 2) = value;
     }
   }
 }
@@ -236,17 +332,23 @@ extern "C" int cachalot_qk_norm_rope(const void* q, int64_t q_token_stride, int6
   a.q = {q, q_token_stride, q_head_stride}, a.k = {k, k_token_stride, k_head_stride}, a.v = {v, v_token_stride, v_head_stride};
   a.q_weight = q_weight, a.k_weight = k_weight, a.w_f32 = w_dtype == CACHALOT_F32, a.eps = eps, a.magnitude = magnitude;
   a.positions = positions, a.inv_freq = inv_freq, a.half = rotary_dim / 2, a.interleaved = interleaved != 0;
-  a.heads = heads, a.kv_heads = kv_heads, a.dim = head_dim, a.q_out = q_out, a.k_out = k_out, a.slots = slots, a.status = status;
+  a.heads = heads, a.kv_heads = kv_heads, a.dim = head_dim, a.inv_dim = 1.f / (float)head_dim, a.q_out = q_out, a.k_out = k_out, a.slots = slots, a.status = status;
   const int lanes = head_dim <= 64 ? 8 : head_dim <= 128 ? 16 : 32, groups = QR_THREADS / lanes;
-  const long long parts = ((long long)heads + 2 * kv_heads + groups - 1) / groups;  // passes of a CTA that takes a whole token
-  const long long want = (600 + (long long)tokens - 1) / tokens;                    // few tokens: their heads over more CTAs
+  const long long parts = ((long long)heads + groups - 1) / groups;         // CTAs of a token at most
+  const long long want = (600 + (long long)tokens - 1) / tokens;           // few tokens: their heads over more CTAs
   const dim3 grid((unsigned)tokens, (unsigned)(parts < want ? parts : want));
   cudaStream_t s = (cudaStream_t)stream;
-  auto go = [&](auto type) {
+  auto run = [&](auto type, auto l) {
     using T = decltype(type);
-    if (lanes == 8) qk_norm_rope_kernel<T, 8><<<grid, QR_THREADS, 0, s>>>(a);
-    else if (lanes == 16) qk_norm_rope_kernel<T, 16><<<grid, QR_THREADS, 0, s>>>(a);
-    else qk_norm_rope_kernel<T, 32><<<grid, QR_THREADS, 0, s>>>(a);
+    constexpr int L = decltype(l)::value;
+    if (rotary_dim % 8 == 0 && interleaved) qk_norm_rope_kernel<T, L, PAIRS_ADJACENT><<<grid, QR_THREADS, 0, s>>>(a);
+    else if (rotary_dim % 16 == 0 && !interleaved) qk_norm_rope_kernel<T, L, PAIRS_HALF><<<grid, QR_THREADS, 0, s>>>(a);
+    else qk_norm_rope_kernel<T, L, PAIRS_ANY><<<grid, QR_THREADS, 0, s>>>(a);
+  };
+  auto go = [&](auto type) {
+    if (lanes == 8) run(type, std::integral_constant<int, 8>{});
+    else if (lanes == 16) run(type, std::integral_constant<int, 16>{});
+    else run(type, std::integral_constant<int, 32>{});
   };
   if (dtype == CACHALOT_F16) go(__half{});
   else go(__nv_bfloat16{});

@@ -20,6 +20,7 @@
 #include <cooperative_groups.h>
 
 #include "common.cuh"
+#include "pairs.cuh"
 
 namespace cachalot {
 namespace {
@@ -55,32 +56,17 @@ struct Sums {  // a maximum that covers the terms (never below -FLT_MAX), sum, s
     s += o.s, u += o.u;
   }
 };
-// two fp32 values in one register pair: Blackwell's packed add, multiply and multiply-add halve the issue slots of a sum
-__device__ __forceinline__ uint64_t pair(float a, float b) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ float2 both(uint64_t p) {
-  float2 r;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(p));
-  return r;
-}
-struct PairSums {  // terms relative to one maximum
-  uint64_t s = 0, u = 0;
-  __device__ __forceinline__ void add(float x, float y, uint64_t minus_m) {
-    uint64_t d, t, p;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(pair(x, y)), "l"(minus_m));
-    const float2 f = both(d);
-    d = pair(fmax_nan(f.x, TL_FAR), fmax_nan(f.y, TL_FAR));
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(t) : "l"(d), "l"(pair(TL_LOG2E, TL_LOG2E)));
-    const float2 e = both(t);
+struct PairSums {  // terms relative to one maximum, two at a time
+  f32x2 s = 0, u = 0;
+  __device__ __forceinline__ void add(float x, float y, f32x2 minus_m) {
+    const float2 f = both(add2(pair(x, y), minus_m));
+    const f32x2 d = pair(fmax_nan(f.x, TL_FAR), fmax_nan(f.y, TL_FAR));
+    const float2 e = both(mul2(d, pair(TL_LOG2E, TL_LOG2E)));
     float2 v;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(v.x) : "f"(e.x));
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(v.y) : "f"(e.y));
-    p = pair(v.x, v.y);
-    asm("add.rn.f32x2 %0, %0, %1;" : "+l"(s) : "l"(p));
-    asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(u) : "l"(p), "l"(d));
+    const f32x2 p = pair(v.x, v.y);
+    s = add2(s, p), u = fma2(p, d, u);
   }
 };
 
@@ -336,7 +322,7 @@ __global__ void __launch_bounds__(TL_THREADS, TL_CTAS) token_logprobs_kernel(con
     if (round + 1 < sh.rounds) sh.fetch(next, round + 1);
     if (most > sum.m) sum.move(most);
     PairSums part;
-    const uint64_t minus_m = pair(-sum.m, -sum.m);
+    const f32x2 minus_m = pair(-sum.m, -sum.m);
 #pragma unroll
     for (int k = 0; k < TL_LOADS; ++k)
 #pragma unroll
