@@ -24,7 +24,7 @@ namespace cachalot {
 namespace {
 
 constexpr int QR_THREADS = 128;
-constexpr int QR_BATCH = 2;  // query heads a group works on while it has as many in flight
+constexpr int QR_BATCH = 4;  // query heads a group has in flight
 constexpr int QR_MAX_DIM = 256;
 
 struct Rows {  // activation rows, strides in elements
@@ -193,100 +193,107 @@ struct Lane {  // what a lane does to its 8 elements of a query or key head
 template <typename T, int L, int PAIRS>
 __global__ void __launch_bounds__(QR_THREADS) qk_norm_rope_kernel(const RopeArgs a) {
   constexpr int GROUPS = QR_THREADS / L;
+  using std::integral_constant;
   __shared__ __align__(16) float cs[QR_MAX_DIM / 2], sn[QR_MAX_DIM / 2];
   const int token = blockIdx.x, group = threadIdx.x / L, half = a.half;
-  const int step = GROUPS * gridDim.y, first = blockIdx.y * GROUPS + group;
+  const int step = GROUPS * gridDim.y, first = blockIdx.y * GROUPS;  // heads first + group, + step, ..
   Lane<T, L, PAIRS> ln;
   ln.at = threadIdx.x % L * 8, ln.half = half, ln.adjacent = a.interleaved;
   const bool live = ln.at < a.dim;
-  const int at = live ? ln.at : 0;  // lanes past the head read its first piece and count as zeros
+  const int at = live ? ln.at : 0;  // lanes past the head count as zeros
   ln.at = at, ln.rotated = at < 2 * half;
   ln.partner = PAIRS != PAIRS_HALF || !ln.rotated ? at : at < half ? at + half : at - half;
-  // the first query heads are on their way while the angles are computed
-  const T* q = static_cast<const T*>(a.q.x) + token * a.q.token;
-  T* q_out = static_cast<T*>(a.q_out) + (long long)token * a.heads * a.dim + at;
-  uint4 ahead[QR_BATCH], ahead_piece[QR_BATCH];
-  auto fetch = [&](int h0) {
-#pragma unroll
-    for (int i = 0; i < QR_BATCH; ++i) {
-      const int h = h0 + i * step;
-      const bool there = live && h < a.heads;
-      ahead[i] = there ? *reinterpret_cast<const uint4*>(q + h * a.q.head + at) : make_uint4(0, 0, 0, 0);
-      ahead_piece[i] = there && PAIRS == PAIRS_HALF ? *reinterpret_cast<const uint4*>(q + h * a.q.head + ln.partner) : make_uint4(0, 0, 0, 0);
-    }
-  };
-  fetch(first);
   for (int i = threadIdx.x; i < half; i += QR_THREADS) {
     const double turns = (double)a.positions[token] * a.inv_freq[i] * 0.15915494309189533577;  // 1 / (2 pi)
     float s, c;
     sincospif(2.0f * (float)(turns - rint(turns)), &s, &c);
     cs[i] = c * a.magnitude, sn[i] = s * a.magnitude;
   }
-  long long page = 0;
-  int off = 0;
+  __syncthreads();
+  const uint4 zero = make_uint4(0, 0, 0, 0);
+  // heads h0 + group, + step, .. (N of them); CHECK: the last ones may not be there
+  auto loads = [&](auto n, auto check, const T* x, long long head, int heads, int h0, int from, uint4* v) {
+    const T* p = x + (long long)(h0 + group) * head + from;
+#pragma unroll
+    for (int i = 0; i < decltype(n)::value; ++i, p += step * head)
+      v[i] = live && (!decltype(check)::value || h0 + group + i * step < heads) ? *reinterpret_cast<const uint4*>(p) : zero;
+  };
+  // as many whole batches as there are, then one by one
+  auto over = [&](int heads, auto batch, auto&& work) {
+    constexpr int N = decltype(batch)::value;
+    int h = first;
+    for (; h + (N - 1) * step + GROUPS <= heads; h += N * step) work(batch, integral_constant<bool, false>{}, h);
+    for (; h < heads; h += step) work(integral_constant<int, 1>{}, integral_constant<bool, true>{}, h);
+  };
+
+  const T* q = static_cast<const T*>(a.q.x) + token * a.q.token;
+  T* q_out = static_cast<T*>(a.q_out) + (long long)token * a.heads * a.dim + at;
+  ln.set(a.q_weight, a.w_f32, cs, sn);
+  over(a.heads, integral_constant<int, QR_BATCH>{}, [&](auto n, auto check, int h0) {
+    constexpr int N = decltype(n)::value;
+    uint4 own[N], piece[N];
+    loads(n, check, q, a.q.head, a.heads, h0, at, own);
+    if (PAIRS == PAIRS_HALF) loads(n, check, q, a.q.head, a.heads, h0, ln.partner, piece);
+    T* out = q_out + (h0 + group) * a.dim;
+#pragma unroll
+    for (int i = 0; i < N; ++i, out += step * a.dim) {
+      const int h = h0 + group + i * step;
+      const bool there = live && (!decltype(check)::value || h < a.heads);
+      f32x2 y[4];
+      widen8<T>(own[i], y);
+      ln.apply(y, piece[i], there ? q + h * a.q.head : nullptr, a.q_weight != nullptr, a.eps, a.inv_dim, 1.f);
+      if (there) *reinterpret_cast<uint4*>(out) = round8<T>(y);
+    }
+  });
+
   bool stored = false;
+  uint8_t *k_row = nullptr, *v_row = nullptr;
   if (a.cache.k) {
     const int slot = a.slots[token];
     const int n = a.cache.n_pages * a.cache.page_size;
     stored = slot >= 0 && slot < n;
     if (slot >= n && a.status && threadIdx.x == 0 && blockIdx.y == 0) atomicOr(a.status, CACHALOT_STATUS_SLOT_RANGE);
-    if (stored) page = slot / a.cache.page_size, off = slot - (int)page * a.cache.page_size;
-  }
-  const bool f8 = a.cache.dtype == CACHALOT_E4M3;
-  __syncthreads();
-  ln.set(a.q_weight, a.w_f32, cs, sn);
-  const uint4 zero = make_uint4(0, 0, 0, 0);
-  for (int h0 = first;;) {
-    uint4 own[QR_BATCH], piece[QR_BATCH];
-#pragma unroll
-    for (int i = 0; i < QR_BATCH; ++i) own[i] = ahead[i], piece[i] = ahead_piece[i];
-    const int next = h0 + QR_BATCH * step;
-    const bool more = next - group < a.heads;
-    if (more) fetch(next);
-#pragma unroll
-    for (int i = 0; i < QR_BATCH; ++i) {
-      const int h = h0 + i * step;
-      if (h - group >= a.heads) break;
-      const bool there = live && h < a.heads;
-      f32x2 y[4];
-      widen8<T>(own[i], y);
-      ln.apply(y, piece[i], there ? q + h * a.q.head : nullptr, a.q_weight != nullptr, a.eps, a.inv_dim, 1.f);
-      if (there) *reinterpret_cast<uint4*>(q_out + h * a.dim) = round8<T>(y);
-    }
-    if (!more) break;
-    h0 = next;
+    const int page = stored ? slot / a.cache.page_size : 0, off = stored ? slot - page * a.cache.page_size : 0;
+    k_row = a.cache.k + page * a.cache.k_page + off * a.cache.k_token;
+    v_row = a.cache.v + page * a.cache.v_page + off * a.cache.v_token;
   }
   if (!stored && !a.k_out) return;
-  ln.set(a.k_weight, a.w_f32, cs, sn);
+  const bool f8 = a.cache.dtype == CACHALOT_E4M3;
   const T* k = static_cast<const T*>(a.k.x) + token * a.k.token;
   const T* v = static_cast<const T*>(a.v.x) + token * a.v.token;
-  for (int h = first; h - group < a.kv_heads; h += step) {
-    const bool there = live && h < a.kv_heads;
-    const uint4 own = there ? *reinterpret_cast<const uint4*>(k + h * a.k.head + at) : zero;
-    const uint4 piece = there && PAIRS == PAIRS_HALF ? *reinterpret_cast<const uint4*>(k + h * a.k.head + ln.partner) : zero;
-    const uint4 value = there && stored ? *reinterpret_cast<const uint4*>(v + h * a.v.head + at) : zero;
-    f32x2 y[4];
-    widen8<T>(own, y);
-    // E4M3: times 1 / scale, one more rounding to fp32 than the division, instead of eight divisions
-    const float k_times = f8 && a.cache.k_scale && there ? 1.f / a.cache.k_scale[h] : 1.f;
-    ln.apply(y, piece, there ? k + h * a.k.head : nullptr, a.k_weight != nullptr, a.eps, a.inv_dim, k_times);
-    if (!there) continue;
-    if (a.k_out) *reinterpret_cast<uint4*>(static_cast<T*>(a.k_out) + ((long long)token * a.kv_heads + h) * a.dim + at) = round8<T>(y);
-    if (!stored) continue;
-    uint8_t* k_row = a.cache.k + page * a.cache.k_page + h * a.cache.k_head + off * a.cache.k_token;
-    uint8_t* v_row = a.cache.v + page * a.cache.v_page + h * a.cache.v_head + off * a.cache.v_token;
-    if (f8) {
-      *reinterpret_cast<uint2*>(k_row + at) = e4m3_8(y);
-      widen8<T>(value, y);
-      const float v_times = a.cache.v_scale ? 1.f / a.cache.v_scale[h] : 1.f;
+  ln.set(a.k_weight, a.w_f32, cs, sn);
+  over(a.kv_heads, integral_constant<int, 2>{}, [&](auto n, auto check, int h0) {
+    constexpr int N = decltype(n)::value;
+    uint4 own[N], piece[N], value[N];
+    loads(n, check, k, a.k.head, a.kv_heads, h0, at, own);
+    if (PAIRS == PAIRS_HALF) loads(n, check, k, a.k.head, a.kv_heads, h0, ln.partner, piece);
+    if (stored) loads(n, check, v, a.v.head, a.kv_heads, h0, at, value);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) y[i] = mul2(y[i], pair(v_times, v_times));
-      *reinterpret_cast<uint2*>(v_row + at) = e4m3_8(y);
-    } else {
-      *reinterpret_cast<uint4*>(k_row + at * 2) = round8<T>(y);
-      *reinterpret_cast<uint4*>(v_row + at * 2) = value;
+    for (int i = 0; i < N; ++i) {
+      const int h = h0 + group + i * step;
+      const bool there = live && (!decltype(check)::value || h < a.kv_heads);
+      f32x2 y[4];
+      widen8<T>(own[i], y);
+      // E4M3: times 1 / scale, one more rounding to fp32 than the division, instead of eight divisions
+      const float k_times = f8 && a.cache.k_scale && there ? 1.f / a.cache.k_scale[h] : 1.f;
+      ln.apply(y, piece[i], there ? k + h * a.k.head : nullptr, a.k_weight != nullptr, a.eps, a.inv_dim, k_times);
+      if (!there) continue;
+      if (a.k_out) *reinterpret_cast<uint4*>(static_cast<T*>(a.k_out) + ((long long)token * a.kv_heads + h) * a.dim + at) = round8<T>(y);
+      if (!stored) continue;
+      uint8_t *ks = k_row + h * a.cache.k_head, *vs = v_row + h * a.cache.v_head;
+      if (f8) {
+        *reinterpret_cast<uint2*>(ks + at) = e4m3_8(y);
+        widen8<T>(value[i], y);
+        const float v_times = a.cache.v_scale ? 1.f / a.cache.v_scale[h] : 1.f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) y[j] = mul2(y[j], pair(v_times, v_times));
+        *reinterpret_cast<uint2*>(vs + at) = e4m3_8(y);
+      } else {
+        *reinterpret_cast<uint4*>(ks + at * 2) = round8<T>(y);
+        *reinterpret_cast<uint4*>(vs + at * 2) = value[i];
+      }
     }
-  }
+  });
 }
 
 int check_rows(const char* name, const void* x, int64_t token, int64_t head) {
