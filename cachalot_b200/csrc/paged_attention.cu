@@ -137,14 +137,14 @@ extern "C" int cachalot_paged_attention(const void* q, int64_t q_row_stride, int
   a.page_shift = -1;
   for (int s = 0; s < 28; ++s)
     if (a.c.page_size == 8 << s) a.page_shift = s;
-  a.min_steps = 1;
+  a.unit_cost = (48 * 1024 + PA_STEP * 2 * a.c.head_dim * paged_elem_bytes(a.c.dtype) - 1) / (PA_STEP * 2 * a.c.head_dim * paged_elem_bytes(a.c.dtype));
   a.scale = scale, a.softcap = softcap, a.window = window, a.out = out, a.out_dtype = out_dtype, a.lse = lse, a.status = status;
   uint8_t* w = static_cast<uint8_t*>(workspace);
   a.parts = reinterpret_cast<int4*>(w), w += up((size_t)most * 2 * sizeof(int4));
   a.part_ml = reinterpret_cast<float2*>(w), w += up((size_t)most * 2 * l.unit_heads * sizeof(float2));
   a.part_o = reinterpret_cast<float*>(w);
   // no more CTAs than there can be steps
-  const long long steps = ((long long)width * a.c.page_size + PA_STEP - 1) / PA_STEP + 1;
+  const long long steps = ((long long)width * a.c.page_size + PA_STEP - 1) / PA_STEP + 1 + a.unit_cost;
   const long long bound = steps * requests * a.c.kv_heads * l.head_blocks;
   const int ctas = (int)(bound < most ? bound : most);
   cudaStream_t s = (cudaStream_t)stream;

@@ -17,9 +17,12 @@
 //   * the running maximum moves only when a score exceeds it by more than 2^8 (one vote per tile instead of six shuffles
 //     and a rescaling); P stays below 2^8 in bf16, and is shifted by 2^7 in f16 to use that type's range.
 // Work is cut on the device, where the lengths are: the steps (64 tokens of one request and key-value head) of the whole
-// batch are numbered through and every CTA takes an equal run of them, so a batch of very different lengths is balanced
-// and one long request fills the GPU.  A CTA merges its four warps in shared memory; a unit (request, head) that lies in
-// one CTA is finished there, a unit that crosses CTAs leaves (m, l, O) of each part for the join kernel.
+// batch are laid on a line and every CTA takes an equal run of it, so a batch of very different lengths is balanced
+// and one long request fills the GPU.  A unit (request, head) also occupies what it costs to begin one (query, first
+// page, empty pipeline, merge: as long as about 48 KB of keys and values; without that, CTAs with many short requests
+// took twice the average and 32 requests of 1 to 8192 tokens 79 us), and a cut that falls near a unit's end is moved there.
+// A CTA merges its four warps in shared memory; a unit that lies in one CTA is finished there, a unit that crosses
+// CTAs leaves (m, l, O) of each part for the join kernel.
 #pragma once
 #include "paged.cuh"
 
@@ -39,7 +42,7 @@ struct AttendArgs {
   int requests, heads, group;      // group: query heads per key-value head
   int tiles, head_blocks;          // head tiles (of 8 NT heads) a CTA's warps are split over; units per key-value head
   int page_shift;                  // log2(page_size / 8) or -1; tokens one by one where the page size is no multiple of 8
-  int min_steps;
+  int unit_cost;                   // what beginning a unit costs, in steps
   float scale, softcap;
   int window;
   float* part_o;                   // [ctas][2][heads of a unit][dim]
@@ -126,7 +129,7 @@ struct AttendShape {
   static constexpr int SMEM(int tiles) { return Q_BYTES(tiles) + PA_WARPS * TILE_HEADS * (O_PITCH * 4 + 8) + 4 * TILE_HEADS * 4; }
   static constexpr int MAX_TILES = 4;
   // CTAs per SM that the registers are cut for
-  static constexpr int CTAS = D * NT <= 64 ? 4 : D * NT <= 128 ? 3 : 2;
+  static constexpr int CTAS = D * NT <= (F8 ? 128 : 64) ? 4 : D * NT <= 128 ? 3 : 2;
 };
 
 struct Span {  // what is visible of a request
@@ -167,10 +170,11 @@ __global__ void __launch_bounds__(PA_THREADS, AttendShape<F8, D, NT>::CTAS) atte
   const int per_request = a.c.kv_heads * a.head_blocks;
   int flags = 0;
 
-  // ---- which steps are this CTA's ----
+  // ---- which part of the line is this CTA's ----
+  auto cost_of = [&](int steps) { return steps ? (long long)(steps + a.unit_cost) * per_request : 0LL; };
   long long mine = 0;
   for (int r = tid; r < a.requests; r += PA_THREADS) {
-    mine += span_of(a, r).steps;
+    mine += cost_of(span_of(a, r).steps);
     const int n = a.lens[r];
     if (n < 0 || n > (long long)a.width * a.c.page_size) flags |= CACHALOT_STATUS_LENGTH;
   }
@@ -182,15 +186,14 @@ __global__ void __launch_bounds__(PA_THREADS, AttendShape<F8, D, NT>::CTAS) atte
   long long total = 0;
 #pragma unroll
   for (int w = 0; w < PA_WARPS; ++w) total += sums[w];
-  total *= per_request;
-  long long per = (total + gridDim.x - 1) / gridDim.x;
-  if (per < a.min_steps) per = a.min_steps;
-  const long long begin = per * blockIdx.x, end = min(begin + per, total);
+  const long long per = max((total + gridDim.x - 1) / gridDim.x, 1LL);
+  const int near_end = (int)max(min((long long)a.unit_cost, per / 4), 1LL);  // a cut is at least that many steps inside a unit
+  const long long begin = per * blockIdx.x;
   long long before = 0;
-  if (begin < end) {
+  if (begin < total) {  // the request that lies there
     for (int r0 = 0; r0 < a.requests; r0 += PA_THREADS) {
       const int r = r0 + tid;
-      const long long own = r < a.requests ? (long long)span_of(a, r).steps * per_request : 0;
+      const long long own = r < a.requests ? cost_of(span_of(a, r).steps) : 0;
       long long v = own;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -220,19 +223,34 @@ __global__ void __launch_bounds__(PA_THREADS, AttendShape<F8, D, NT>::CTAS) atte
   }
   if (tid < 2) a.parts[blockIdx.x * 2 + tid] = make_int4(0, 0, 0, 0);
   __syncthreads();
-  if (begin >= end || found < 0) {
+  if (found < 0) {
     if (a.status && flags) atomicOr(a.status, flags);
     return;
   }
 
   int r = found;
   Span sp = span_of(a, r);
-  int unit = (int)((begin - found_at) / sp.steps), step0 = (int)((begin - found_at) % sp.steps);
+  int unit = (int)((begin - found_at) / (sp.steps + a.unit_cost));
+  long long at = found_at + (long long)unit * (sp.steps + a.unit_cost);  // where the unit begins on the line
   const int mt = warp % a.tiles, slice = warp / a.tiles, slices = PA_WARPS / a.tiles;
   const int unit_heads = a.tiles * S::TILE_HEADS;
 
-  for (long long at = begin; at < end;) {
-    const int steps = (int)min((long long)(sp.steps - step0), end - at);
+  for (;; at += sp.steps + a.unit_cost, ++unit) {
+    if (unit == per_request) {
+      unit = 0;
+      do {
+        if (++r >= a.requests) goto done;
+        sp = span_of(a, r);
+      } while (sp.steps == 0);
+    }
+    // the unit is cut where multiples of `per` fall among its steps, not within `inside` of either end: CTAs c0 .. c1
+    const int inside = min(near_end, sp.steps);
+    const long long cta = blockIdx.x, steps_at = at + a.unit_cost;
+    const long long c0 = (steps_at + inside - 1) / per, c1 = max(c0, (steps_at + sp.steps - inside) / per);
+    if (c0 > cta) break;
+    if (c1 < cta) continue;  // this CTA's run begins so near the unit's end that another one does all of it
+    const int step0 = cta == c0 ? 0 : (int)(cta * per - steps_at);
+    const int steps = (cta == c1 ? sp.steps : (int)((cta + 1) * per - steps_at)) - step0;
     const int h = unit / a.head_blocks, block = unit % a.head_blocks;
     const int head0 = block * unit_heads, heads = min(unit_heads, a.group - head0);  // within the group
     const long long row0 = (long long)r * a.heads + (long long)h * a.group + head0;  // first output row of the unit
@@ -502,8 +520,8 @@ __global__ void __launch_bounds__(PA_THREADS, AttendShape<F8, D, NT>::CTAS) atte
         }
       }
     __syncthreads();
-    const bool whole = step0 == 0 && steps == sp.steps;
-    const int which = step0 > 0 ? 0 : 1;
+    const bool whole = c0 == c1;
+    const int which = cta == c0 ? 1 : 0;
     const long long slot = (long long)blockIdx.x * 2 + which;
     const float v_scale = F8 && a.c.v_scale ? a.c.v_scale[h] : 1.f;
     for (int i = tid; i < heads * (D / 4); i += PA_THREADS) {
@@ -529,21 +547,10 @@ __global__ void __launch_bounds__(PA_THREADS, AttendShape<F8, D, NT>::CTAS) atte
         if (d == 0) a.part_ml[slot * unit_heads + head] = make_float2(top, sum);
       }
     }
-    if (!whole && tid == 0) {
-      const long long first = at - step0;  // the unit's first step
-      const int c0 = (int)(first / per), c1 = (int)((first + sp.steps - 1) / per);
-      a.parts[slot] = make_int4(r, unit, c0, c1 - c0 + 1);
-    }
+    if (!whole && tid == 0) a.parts[slot] = make_int4(r, unit, (int)c0, (int)(c1 - c0) + 1);
     __syncthreads();
-    at += steps, step0 = 0;
-    if (at < end && ++unit == per_request) {
-      unit = 0;
-      do {
-        if (++r >= a.requests) return;  // not with lengths that stay as they are during the call
-        sp = span_of(a, r);
-      } while (sp.steps == 0);
-    }
   }
+done:
   if (a.status && flags) atomicOr(a.status, flags);
 }
 
