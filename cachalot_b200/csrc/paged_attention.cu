@@ -119,6 +119,8 @@ extern "C" int cachalot_paged_attention(const void* q, int64_t q_row_stride, int
   if (heads % a.c.kv_heads) return fail(CACHALOT_EINVAL, "paged_attention: %d query heads over %d key-value heads", heads, a.c.kv_heads);
   if (a.c.dtype != CACHALOT_E4M3 && a.c.dtype != q_dtype) return fail(CACHALOT_EINVAL, "paged_attention: cache and queries differ in type");
   if (window < 0 || !(softcap >= 0.f)) return fail(CACHALOT_EINVAL, "paged_attention: window and softcap must not be negative");
+  for (long long stride : {a.c.k_page, a.c.k_token, a.c.v_page, a.c.v_token})
+    if (stride > 0xffffffffLL) return fail(CACHALOT_EUNSUPPORTED, "paged_attention: pages or tokens %lld bytes apart", stride);
   const bool f8 = a.c.dtype == CACHALOT_E4M3;
   AttendLaunch l;
   if (!shape_of(f8, a.c.head_dim, heads / a.c.kv_heads, &l))
@@ -132,19 +134,22 @@ extern "C" int cachalot_paged_attention(const void* q, int64_t q_row_stride, int
   if (workspace_bytes < workspace_of(l, a.c.head_dim, most))
     return fail(CACHALOT_ESCRATCH, "paged_attention: workspace of %zu bytes, %zu needed", workspace_bytes, workspace_of(l, a.c.head_dim, most));
   a.q = q, a.q_row = q_row_stride, a.q_head = q_head_stride, a.q_bf16 = q_dtype == CACHALOT_BF16;
-  a.table = block_table, a.table_stride = table_stride, a.width = width, a.lens = lens;
+  a.table = block_table, a.table_stride = table_stride, a.lens = lens;
+  const long long room = (long long)width * a.c.page_size;
+  a.room = room < 0x7fffff00LL ? (int)room : 0x7fffff00;
   a.requests = requests, a.heads = heads, a.group = heads / a.c.kv_heads, a.tiles = l.tiles, a.head_blocks = l.head_blocks;
   a.page_shift = -1;
   for (int s = 0; s < 28; ++s)
     if (a.c.page_size == 8 << s) a.page_shift = s;
-  a.unit_cost = (48 * 1024 + PA_STEP * 2 * a.c.head_dim * paged_elem_bytes(a.c.dtype) - 1) / (PA_STEP * 2 * a.c.head_dim * paged_elem_bytes(a.c.dtype));
+  const int step_bytes = l.step * 2 * a.c.head_dim * paged_elem_bytes(a.c.dtype);
+  a.unit_cost = (48 * 1024 + step_bytes - 1) / step_bytes;
   a.scale = scale, a.softcap = softcap, a.window = window, a.out = out, a.out_dtype = out_dtype, a.lse = lse, a.status = status;
   uint8_t* w = static_cast<uint8_t*>(workspace);
   a.parts = reinterpret_cast<int4*>(w), w += up((size_t)most * 2 * sizeof(int4));
   a.part_ml = reinterpret_cast<float2*>(w), w += up((size_t)most * 2 * l.unit_heads * sizeof(float2));
   a.part_o = reinterpret_cast<float*>(w);
   // no more CTAs than there can be steps
-  const long long steps = ((long long)width * a.c.page_size + PA_STEP - 1) / PA_STEP + 1 + a.unit_cost;
+  const long long steps = (a.room + l.step - 1) / l.step + 1 + a.unit_cost;
   const long long bound = steps * requests * a.c.kv_heads * l.head_blocks;
   const int ctas = (int)(bound < most ? bound : most);
   cudaStream_t s = (cudaStream_t)stream;

@@ -7,7 +7,7 @@
 // HBM-bound: every visible key and value is read once for the G query heads that share it, 2 G FLOP per byte of a 16-bit
 // cache.  On CUDA cores G = 8 would already need the whole fp32 rate; the legacy warp MMA (m16n8k16) has ten times the
 // arithmetic this needs and, unlike tcgen05, takes its operands from registers, so nothing is staged:
-//   * a warp works on tiles of 16 tokens.  S^T = K Q^T has the tokens as MMA rows and 8 query heads as columns, O^T = V^T P^T
+//   * a warp works on tiles of 16 tokens, 32 where a row is 128 bytes or less.  S^T = K Q^T has the tokens as MMA rows and 8 query heads as columns, O^T = V^T P^T
 //     the head's elements as rows and the 8 heads as columns: no row of an MMA is spent on padding for G = 8.
 //   * the order of the reduction index is free, so a lane's 16-byte loads of a key row ARE its operand fragments; for the
 //     values, whose fragments pair two tokens, one byte permute per register pairs the words of two rows.
@@ -16,7 +16,7 @@
 //   * S^T fragments become P^T fragments by one movmatrix each.
 //   * the running maximum moves only when a score exceeds it by more than 2^8 (one vote per tile instead of six shuffles
 //     and a rescaling); P stays below 2^8 in bf16, and is shifted by 2^7 in f16 to use that type's range.
-// Work is cut on the device, where the lengths are: the steps (64 tokens of one request and key-value head) of the whole
+// Work is cut on the device, where the lengths are: the steps (a tile for each warp, of one request and key-value head) of the whole
 // batch are laid on a line and every CTA takes an equal run of it, so a batch of very different lengths is balanced
 // and one long request fills the GPU.  A unit (request, head) also occupies what it costs to begin one (query, first
 // page, empty pipeline, merge: as long as about 48 KB of keys and values; without that, CTAs with many short requests
@@ -28,7 +28,7 @@
 
 namespace cachalot {
 
-constexpr int PA_THREADS = 128, PA_WARPS = 4, PA_STEP = 64, PA_TILE = 16;
+constexpr int PA_THREADS = 128, PA_WARPS = 4;
 
 struct AttendArgs {
   const void* q;
@@ -37,7 +37,7 @@ struct AttendArgs {
   PagedView c;
   const int32_t* table;
   long long table_stride;
-  int width;
+  int room;                        // tokens that a request's row of the table holds
   const int32_t* lens;
   int requests, heads, group;      // group: query heads per key-value head
   int tiles, head_blocks;          // head tiles (of 8 NT heads) a CTA's warps are split over; units per key-value head
@@ -119,6 +119,8 @@ struct AttendShape {
   static constexpr int KB = KBYTES % 16 == 0 ? 16 : 8;
   static constexpr int VB = VBYTES % 16 == 0 ? 16 : VBYTES % 8 == 0 ? 8 : 4;
   static constexpr int KW = KBYTES / 4, VW = VBYTES / 4;
+  static constexpr int U = D * ES <= 128 ? 2 : 1;       // MMA tiles of 16 tokens that a warp works on at a time
+  static constexpr int TILE = 16 * U, STEP = PA_WARPS * TILE;
   static constexpr int KSTEPS = D / 16;                 // MMAs over the head's elements = MMA row tiles of O^T
   static constexpr int TILE_HEADS = 8 * NT;
   static constexpr int O_PITCH = D + 4;
@@ -129,22 +131,32 @@ struct AttendShape {
   static constexpr int SMEM(int tiles) { return Q_BYTES(tiles) + PA_WARPS * TILE_HEADS * (O_PITCH * 4 + 8) + 4 * TILE_HEADS * 4; }
   static constexpr int MAX_TILES = 4;
   // CTAs per SM that the registers are cut for
-  static constexpr int CTAS = D * NT <= (F8 ? 128 : 64) ? 4 : D * NT <= 128 ? 3 : 2;
+  static constexpr int CTAS = D * NT <= 64 ? 4 : D * NT <= 128 ? 3 : 2;
 };
 
 struct Span {  // what is visible of a request
   int lo, len, first_tile, steps;
 };
+template <typename S>
 __device__ __forceinline__ Span span_of(const AttendArgs& a, int r) {
-  const long long room = (long long)a.width * a.c.page_size;
-  const int n = a.lens[r];
   Span s;
-  s.len = (int)min((long long)max(n, 0), room);
+  s.len = min(max(__ldg(a.lens + r), 0), a.room);
   s.lo = a.window > 0 ? max(0, s.len - a.window) : 0;
-  s.first_tile = s.lo / PA_TILE;
-  s.steps = s.len > 0 ? (s.len - s.first_tile * PA_TILE + PA_STEP - 1) / PA_STEP : 0;
+  s.first_tile = s.lo / S::TILE;
+  s.steps = s.len > 0 ? (s.len - s.first_tile * S::TILE + S::STEP - 1) / S::STEP : 0;
   return s;
 }
+
+// Division by a number that stays the same, of dividends below 2^53 (a 64-bit division takes a thousand cycles).
+struct Divisor {
+  long long d;
+  double inverse;
+  __device__ __forceinline__ explicit Divisor(long long by) : d(by), inverse(1.0 / (double)by) {}
+  __device__ __forceinline__ long long of(long long x) const {
+    const long long q = (long long)((double)x * inverse), rest = x - q * d;
+    return rest < 0 ? q - 1 : rest >= d ? q + 1 : q;
+  }
+};
 
 __device__ __forceinline__ void store_out(void* out, int dtype, long long at, float v) {
   if (dtype == CACHALOT_F32) static_cast<float*>(out)[at] = v;
@@ -163,97 +175,204 @@ __global__ void __launch_bounds__(PA_THREADS, AttendShape<F8, D, NT>::CTAS) atte
   float2* sml = reinterpret_cast<float2*>(so + PA_WARPS * S::TILE_HEADS * S::O_PITCH);  // [warps][TILE_HEADS]
   float* sexp = reinterpret_cast<float*>(sml + PA_WARPS * S::TILE_HEADS);            // [tiles * TILE_HEADS] scale of the query
   __shared__ long long sums[PA_WARPS];
-  __shared__ long long found_at;
-  __shared__ int found;
+  __shared__ long long shared_found_at;
+  __shared__ int shared_found;
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
   const int per_request = a.c.kv_heads * a.head_blocks;
   int flags = 0;
 
   // ---- which part of the line is this CTA's ----
-  auto cost_of = [&](int steps) { return steps ? (long long)(steps + a.unit_cost) * per_request : 0LL; };
-  long long mine = 0;
-  for (int r = tid; r < a.requests; r += PA_THREADS) {
-    mine += cost_of(span_of(a, r).steps);
-    const int n = a.lens[r];
-    if (n < 0 || n > (long long)a.width * a.c.page_size) flags |= CACHALOT_STATUS_LENGTH;
-  }
+  auto cost_of = [&](int r) {
+    if (r >= a.requests) return 0LL;
+    const int n = __ldg(a.lens + r);
+    if (n < 0 || n > a.room) flags |= CACHALOT_STATUS_LENGTH;
+    const int steps = span_of<S>(a, r).steps;
+    return steps ? (long long)(steps + a.unit_cost) * per_request : 0LL;
+  };
+  auto scan = [&](long long v) {  // inclusive, over the warp
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
-  if (lane == 0) sums[warp] = mine;
-  if (tid == 0) found = -1;
-  __syncthreads();
-  long long total = 0;
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long u = __shfl_up_sync(0xffffffffu, v, o);
+      if (lane >= o) v += u;
+    }
+    return v;
+  };
+  int found = -1;  // the request that lies where the run begins, and where that request begins
+  long long found_at = 0, total = 0, per, begin;
+  auto cut = [&] {
+    per = max(Divisor(gridDim.x).of(total + gridDim.x - 1), 1LL);
+    begin = per * blockIdx.x;
+  };
+  if (a.requests <= 32) {  // every warp for itself
+    const long long own = cost_of(lane), end = scan(own);
+    total = __shfl_sync(0xffffffffu, end, 31);
+    cut();
+    const unsigned here = __ballot_sync(0xffffffffu, begin >= end - own && begin < end);
+    if (here) found = __ffs(here) - 1, found_at = __shfl_sync(0xffffffffu, end - own, found);
+  } else {
+    for (int r = tid; r < a.requests; r += PA_THREADS) total += cost_of(r);
+    total = __shfl_sync(0xffffffffu, scan(total), 31);
+    if (lane == 0) sums[warp] = total;
+    if (tid == 0) shared_found = -1;
+    __syncthreads();
+    total = 0;
 #pragma unroll
-  for (int w = 0; w < PA_WARPS; ++w) total += sums[w];
-  const long long per = max((total + gridDim.x - 1) / gridDim.x, 1LL);
-  const int near_end = (int)max(min((long long)a.unit_cost, per / 4), 1LL);  // a cut is at least that many steps inside a unit
-  const long long begin = per * blockIdx.x;
-  long long before = 0;
-  if (begin < total) {  // the request that lies there
-    for (int r0 = 0; r0 < a.requests; r0 += PA_THREADS) {
-      const int r = r0 + tid;
-      const long long own = r < a.requests ? cost_of(span_of(a, r).steps) : 0;
-      long long v = own;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const long long u = __shfl_up_sync(0xffffffffu, v, o);
-        if (lane >= o) v += u;
-      }
+    for (int w = 0; w < PA_WARPS; ++w) total += sums[w];
+    cut();
+    long long before = 0;
+    for (int r0 = 0; r0 < a.requests && begin < total; r0 += PA_THREADS) {
+      const long long own = cost_of(r0 + tid);
+      long long end = scan(own);
       __syncthreads();
-      if (lane == 31) sums[warp] = v;
+      if (lane == 31) sums[warp] = end;
       __syncthreads();
 #pragma unroll
-      for (int w = 0; w < PA_WARPS; ++w) v += w < warp ? sums[w] : 0;
-      v += before;
-      if (begin >= v - own && begin < v) found = r, found_at = v - own;
+      for (int w = 0; w < PA_WARPS; ++w) end += w < warp ? sums[w] : 0;
+      end += before;
+      if (begin >= end - own && begin < end) shared_found = r0 + tid, shared_found_at = end - own;
 #pragma unroll
       for (int w = 0; w < PA_WARPS; ++w) before += sums[w];
-      __syncthreads();
-      if (found >= 0) break;
+      if (before > begin) break;
     }
-  }
-
-  // ---- rows without a visible key ----
-  for (int r = blockIdx.x; r < a.requests; r += gridDim.x) {
-    if (span_of(a, r).steps) continue;
-    for (int i = tid; i < a.heads * D; i += PA_THREADS) store_out(a.out, a.out_dtype, (long long)r * a.heads * D + i, 0.f);
-    if (a.lse)
-      for (int i = tid; i < a.heads; i += PA_THREADS) a.lse[(long long)r * a.heads + i] = -INFINITY;
+    __syncthreads();
+    found = shared_found, found_at = shared_found_at;
   }
   if (tid < 2) a.parts[blockIdx.x * 2 + tid] = make_int4(0, 0, 0, 0);
   __syncthreads();
-  if (found < 0) {
-    if (a.status && flags) atomicOr(a.status, flags);
-    return;
-  }
+  const Divisor by_per(per);
+  const int near_end = (int)max(min((long long)a.unit_cost, per / 4), 1LL);  // a cut is at least that many steps inside a unit
 
-  int r = found;
-  Span sp = span_of(a, r);
-  int unit = (int)((begin - found_at) / (sp.steps + a.unit_cost));
-  long long at = found_at + (long long)unit * (sp.steps + a.unit_cost);  // where the unit begins on the line
   const int mt = warp % a.tiles, slice = warp / a.tiles, slices = PA_WARPS / a.tiles;
   const int unit_heads = a.tiles * S::TILE_HEADS;
+  int r = max(found, 0);
+  Span sp = span_of<S>(a, r);
+  int unit = 0;
+  if (found >= 0) unit = (int)Divisor(sp.steps + a.unit_cost).of(begin - found_at);
+  long long at = found_at + (long long)unit * (sp.steps + a.unit_cost);  // where the unit begins on the line
 
-  for (;; at += sp.steps + a.unit_cost, ++unit) {
+  for (; found >= 0; at += sp.steps + a.unit_cost, ++unit) {
     if (unit == per_request) {
       unit = 0;
-      do {
-        if (++r >= a.requests) goto done;
-        sp = span_of(a, r);
-      } while (sp.steps == 0);
+      do sp = ++r < a.requests ? span_of<S>(a, r) : Span{0, 0, 0, -1};
+      while (sp.steps == 0);
+      if (sp.steps < 0) break;
     }
     // the unit is cut where multiples of `per` fall among its steps, not within `inside` of either end: CTAs c0 .. c1
     const int inside = min(near_end, sp.steps);
     const long long cta = blockIdx.x, steps_at = at + a.unit_cost;
-    const long long c0 = (steps_at + inside - 1) / per, c1 = max(c0, (steps_at + sp.steps - inside) / per);
+    const long long c0 = by_per.of(steps_at + inside - 1), c1 = max(c0, by_per.of(steps_at + sp.steps - inside));
     if (c0 > cta) break;
     if (c1 < cta) continue;  // this CTA's run begins so near the unit's end that another one does all of it
     const int step0 = cta == c0 ? 0 : (int)(cta * per - steps_at);
     const int steps = (cta == c1 ? sp.steps : (int)((cta + 1) * per - steps_at)) - step0;
-    const int h = unit / a.head_blocks, block = unit % a.head_blocks;
+    const int h = a.head_blocks == 1 ? unit : unit / a.head_blocks, block = a.head_blocks == 1 ? 0 : unit % a.head_blocks;
     const int head0 = block * unit_heads, heads = min(unit_heads, a.group - head0);  // within the group
     const long long row0 = (long long)r * a.heads + (long long)h * a.group + head0;  // first output row of the unit
+
+    // ---- this warp's tiles ----
+    const uint8_t* kbase = a.c.k + h * a.c.k_head + t4 * S::KB;
+    const uint8_t* vbase = a.c.v + h * a.c.v_head + g * S::VB;
+    const uint32_t k_page = (uint32_t)a.c.k_page, k_token = (uint32_t)a.c.k_token, v_page = (uint32_t)a.c.v_page, v_token = (uint32_t)a.c.v_token;
+    const uint8_t *klane = kbase + (uint64_t)(uint32_t)g * k_token, *vlane = vbase + (uint64_t)(uint32_t)(2 * t4) * v_token;
+    const int32_t* pages = a.table + r * a.table_stride;
+    const int tile_end = min(sp.first_tile + (step0 + steps) * PA_WARPS, (sp.len + S::TILE - 1) / S::TILE);
+    uint32_t kr[S::U][2][S::KW], vr[S::U][4][S::VW];
+
+    // page of a token, -1 where the table names none of the cache's
+    auto page_of = [&](int token, int index) {
+      if (token >= sp.len) return -1;
+      const int p = __ldg(pages + index);
+      if ((unsigned)p < (unsigned)a.c.n_pages) return p;
+      flags |= CACHALOT_STATUS_SLOT_RANGE;
+      return -1;
+    };
+    struct Place {  // where a tile lies: page and place in it of its pieces of 8 tokens (pages of 8 k tokens)
+      int tile, page[2 * S::U], off[2 * S::U];
+      bool full;
+    };
+    auto locate = [&](int tile) {
+      Place p;
+      p.tile = tile;
+      p.full = tile * S::TILE >= sp.lo && (tile + 1) * S::TILE <= sp.len;
+      if constexpr (PAGE8) {
+#pragma unroll
+        for (int i = 0; i < 2 * S::U; ++i) {
+          const int token = tile * S::TILE + 8 * i;
+          const int index = a.page_shift >= 0 ? (token >> 3) >> a.page_shift : token / a.c.page_size;
+          p.off[i] = token - index * a.c.page_size;
+          p.page[i] = token + 8 <= sp.lo ? -1 : page_of(token, index);
+          p.full = p.full && p.page[i] >= 0;
+        }
+      } else {
+        p.full = false;
+      }
+      return p;
+    };
+    // place of token i of piece `piece` of a tile: true and its page and offset if it is visible
+    auto token_at = [&](const Place& p, int piece, int i, int& page, int& off) {
+      const int token = p.tile * S::TILE + piece * 8 + i;
+      const bool ok = token >= sp.lo && token < sp.len;
+      if constexpr (PAGE8) {
+        page = p.page[piece], off = p.off[piece] + i;
+        return ok && page >= 0;
+      } else {
+        if (!ok) return false;
+        const int index = token / a.c.page_size;
+        page = page_of(token, index), off = token - index * a.c.page_size;
+        return page >= 0;
+      }
+    };
+    int seen = 0;  // bit i: key row g of piece i of the tile in `kr` is visible
+    auto load_k = [&](const Place& p) {
+      seen = (1 << 2 * S::U) - 1;
+      if (p.full) {
+#pragma unroll
+        for (int i = 0; i < 2 * S::U; ++i)
+          load_words<S::KB, S::KW, 4 * S::KB, KEEP>(kr[i / 2][i % 2], klane + (uint64_t)(uint32_t)p.page[i] * k_page + (uint64_t)(uint32_t)p.off[i] * k_token);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 2 * S::U; ++i) {
+          int page, off;
+          if (token_at(p, i, g, page, off)) {
+            load_words<S::KB, S::KW, 4 * S::KB, KEEP>(kr[i / 2][i % 2], kbase + (uint64_t)(uint32_t)page * k_page + (uint64_t)(uint32_t)off * k_token);
+          } else {
+            seen &= ~(1 << i);
+#pragma unroll
+            for (int w = 0; w < S::KW; ++w) kr[i / 2][i % 2][w] = 0;
+          }
+        }
+      }
+    };
+    auto load_v = [&](const Place& p) {  // rows 2 t4, 2 t4 + 1 of every piece; what is hidden must be zero, 0 * NaN is not
+      if (p.full) {
+#pragma unroll
+        for (int i = 0; i < 2 * S::U; ++i) {
+          const uint8_t* row = vlane + (uint64_t)(uint32_t)p.page[i] * v_page + (uint64_t)(uint32_t)p.off[i] * v_token;
+          load_words<S::VB, S::VW, 8 * S::VB, KEEP>(vr[i / 2][i % 2 * 2], row);
+          load_words<S::VB, S::VW, 8 * S::VB, KEEP>(vr[i / 2][i % 2 * 2 + 1], row + v_token);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4 * S::U; ++i) {
+          int page, off;
+          if (token_at(p, i / 2, 2 * t4 + i % 2, page, off)) {
+            load_words<S::VB, S::VW, 8 * S::VB, KEEP>(vr[i / 4][i % 4], vbase + (uint64_t)(uint32_t)page * v_page + (uint64_t)(uint32_t)off * v_token);
+          } else {
+#pragma unroll
+            for (int w = 0; w < S::VW; ++w) vr[i / 4][i % 4][w] = 0;
+          }
+        }
+      }
+    };
+
+    int tile = sp.first_tile + step0 * PA_WARPS + slice;
+    Place next;
+    if (tile < tile_end) {  // on their way while the queries are laid out
+      const Place p = locate(tile);
+      load_k(p), load_v(p);
+      if (tile + slices < tile_end) next = locate(tile + slices);
+    }
 
     // ---- the query heads as MMA fragments ----
     if constexpr (F8) {  // f16 from here on: a bf16 head is brought into range by a power of two
@@ -298,11 +417,6 @@ __global__ void __launch_bounds__(PA_THREADS, AttendShape<F8, D, NT>::CTAS) atte
       }
     const float cap = a.softcap * PA_LOG2E;
 
-    // ---- this warp's tiles ----
-    const uint8_t* kbase = a.c.k + h * a.c.k_head + t4 * S::KB;
-    const uint8_t* vbase = a.c.v + h * a.c.v_head + g * S::VB;
-    const int32_t* pages = a.table + r * a.table_stride;
-    const int tile_end = min(sp.first_tile + (step0 + steps) * (PA_STEP / PA_TILE), (sp.len + PA_TILE - 1) / PA_TILE);
     float o[S::KSTEPS][NT][4];
     float m[NT][2], base[NT][2], l[NT][2];
 #pragma unroll
@@ -314,120 +428,32 @@ __global__ void __launch_bounds__(PA_THREADS, AttendShape<F8, D, NT>::CTAS) atte
 #pragma unroll
         for (int c = 0; c < 4; ++c) o[k][n][c] = 0.f;
     }
-    uint32_t kr[2][S::KW], vr[4][S::VW];
-
-    // page of a token, -1 where the table names none of the cache's
-    auto page_of = [&](int token, int index) {
-      if (token >= sp.len) return -1;
-      const int p = pages[index];
-      if ((unsigned)p < (unsigned)a.c.n_pages) return p;
-      flags |= CACHALOT_STATUS_SLOT_RANGE;
-      return -1;
-    };
-    struct Place {  // where a tile lies: page and place in it of its two halves of 8 tokens (pages of 8 k tokens)
-      int tile, page[2], off[2];
-      bool full;
-    };
-    auto locate = [&](int tile) {
-      Place p;
-      p.tile = tile;
-      p.full = tile * PA_TILE >= sp.lo && (tile + 1) * PA_TILE <= sp.len;
-      if constexpr (PAGE8) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int token = tile * PA_TILE + 8 * i;
-          const int index = a.page_shift >= 0 ? (token >> 3) >> a.page_shift : token / a.c.page_size;
-          p.off[i] = token - index * a.c.page_size;
-          p.page[i] = token + 8 <= sp.lo ? -1 : page_of(token, index);
-          p.full = p.full && p.page[i] >= 0;
-        }
-      } else {
-        p.full = false;
-      }
-      return p;
-    };
-    // place of token `half * 8 + i` of a tile: true and its page and offset if it is visible
-    auto token_at = [&](const Place& p, int half, int i, int& page, int& off) {
-      const int token = p.tile * PA_TILE + half * 8 + i;
-      bool ok = token >= sp.lo && token < sp.len;
-      if constexpr (PAGE8) {
-        page = p.page[half], off = p.off[half] + i;
-        return ok && page >= 0;
-      } else {
-        if (!ok) return false;
-        const int index = token / a.c.page_size;
-        page = page_of(token, index), off = token - index * a.c.page_size;
-        return page >= 0;
-      }
-    };
-    int seen = 0;  // bit i: key row g + 8 i of the tile in `kr` is visible
-    auto load_k = [&](const Place& p) {
-      seen = 3;
-      if (p.full) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-          load_words<S::KB, S::KW, 4 * S::KB, KEEP>(kr[i], kbase + p.page[i] * a.c.k_page + (p.off[i] + g) * a.c.k_token);
-      } else {
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          int page, off;
-          if (token_at(p, i, g, page, off)) {
-            load_words<S::KB, S::KW, 4 * S::KB, KEEP>(kr[i], kbase + page * a.c.k_page + off * a.c.k_token);
-          } else {
-            seen &= ~(1 << i);
-#pragma unroll
-            for (int w = 0; w < S::KW; ++w) kr[i][w] = 0;
-          }
-        }
-      }
-    };
-    auto load_v = [&](const Place& p) {  // rows 2 t4, 2 t4 + 1 of either half; what is hidden must be zero, 0 * NaN is not
-      if (p.full) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          load_words<S::VB, S::VW, 8 * S::VB, KEEP>(vr[i], vbase + p.page[i >> 1] * a.c.v_page + (p.off[i >> 1] + 2 * t4 + (i & 1)) * a.c.v_token);
-      } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          int page, off;
-          if (token_at(p, i >> 1, 2 * t4 + (i & 1), page, off)) {
-            load_words<S::VB, S::VW, 8 * S::VB, KEEP>(vr[i], vbase + page * a.c.v_page + off * a.c.v_token);
-          } else {
-#pragma unroll
-            for (int w = 0; w < S::VW; ++w) vr[i][w] = 0;
-          }
-        }
-      }
-    };
-
-    int tile = sp.first_tile + step0 * (PA_STEP / PA_TILE) + slice;
-    Place next;
-    if (tile < tile_end) {
-      const Place p = locate(tile);
-      load_k(p), load_v(p);
-      if (tile + slices < tile_end) next = locate(tile + slices);
-    }
     const uint2* q = sq + mt * NT * S::KSTEPS * 32 + lane;
     for (; tile < tile_end; tile += slices) {
       const bool more = tile + slices < tile_end;
-      float s[NT][4];
+      float s[S::U][NT][4];
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
+      for (int u = 0; u < S::U; ++u)
 #pragma unroll
-        for (int c = 0; c < 4; ++c) s[n][c] = 0.f;
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) s[u][n][c] = 0.f;
 #pragma unroll
       for (int k = 0; k < S::KSTEPS; ++k) {
-        uint32_t a0, a1, a2, a3;
-        if constexpr (F8) {
-          a0 = e4m3x2_f16x2(kr[0][k]), a1 = e4m3x2_f16x2(kr[1][k]);
-          a2 = e4m3x2_f16x2(kr[0][k] >> 16), a3 = e4m3x2_f16x2(kr[1][k] >> 16);
-        } else {
-          a0 = kr[0][2 * k], a1 = kr[1][2 * k], a2 = kr[0][2 * k + 1], a3 = kr[1][2 * k + 1];
-        }
+        uint2 b[NT];
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          const uint2 b = q[(n * S::KSTEPS + k) * 32];
-          mma16816<M>(s[n], a0, a1, a2, a3, b.x, b.y);
+        for (int n = 0; n < NT; ++n) b[n] = q[(n * S::KSTEPS + k) * 32];
+#pragma unroll
+        for (int u = 0; u < S::U; ++u) {
+          uint32_t a0, a1, a2, a3;
+          if constexpr (F8) {
+            a0 = e4m3x2_f16x2(kr[u][0][k]), a1 = e4m3x2_f16x2(kr[u][1][k]);
+            a2 = e4m3x2_f16x2(kr[u][0][k] >> 16), a3 = e4m3x2_f16x2(kr[u][1][k] >> 16);
+          } else {
+            a0 = kr[u][0][2 * k], a1 = kr[u][1][2 * k], a2 = kr[u][0][2 * k + 1], a3 = kr[u][1][2 * k + 1];
+          }
+#pragma unroll
+          for (int n = 0; n < NT; ++n) mma16816<M>(s[u][n], a0, a1, a2, a3, b[n].x, b[n].y);
         }
       }
       const int visible = seen;
@@ -435,20 +461,26 @@ __global__ void __launch_bounds__(PA_THREADS, AttendShape<F8, D, NT>::CTAS) atte
       bool higher = false;
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
+        float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          float x = s[n][c] * hs[n][c & 1];
-          if (a.softcap > 0.f) x = cap - __fdividef(2.f * cap, 1.f + ex2(x));
-          s[n][c] = visible >> (c >> 1) & 1 ? x : -INFINITY;
-        }
-        higher = higher || fmaxf(s[n][0], s[n][2]) > m[n][0] + SLACK || fmaxf(s[n][1], s[n][3]) > m[n][1] + SLACK;
+        for (int u = 0; u < S::U; ++u)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            float x = s[u][n][c] * hs[n][c & 1];
+            if (a.softcap > 0.f) x = cap - __fdividef(2.f * cap, 1.f + ex2(x));
+            s[u][n][c] = x = visible >> (2 * u + (c >> 1)) & 1 ? x : -INFINITY;
+            top[c & 1] = fmaxf(top[c & 1], x);
+          }
+        higher = higher || top[0] > m[n][0] + SLACK || top[1] > m[n][1] + SLACK;
       }
       if (__any_sync(0xffffffffu, higher)) {
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
-            float top = fmaxf(s[n][c], s[n][c + 2]);
+            float top = -INFINITY;
+#pragma unroll
+            for (int u = 0; u < S::U; ++u) top = fmaxf(top, fmaxf(s[u][n][c], s[u][n][c + 2]));
 #pragma unroll
             for (int x = 4; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
             const float now = fmaxf(m[n][c], top);
@@ -459,32 +491,36 @@ __global__ void __launch_bounds__(PA_THREADS, AttendShape<F8, D, NT>::CTAS) atte
             for (int k = 0; k < S::KSTEPS; ++k) o[k][n][c] *= keep, o[k][n][c + 2] *= keep;
           }
       }
-      uint32_t pb[NT][2];
+      uint32_t pb[S::U][NT][2];
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        float p[4];
+      for (int u = 0; u < S::U; ++u)
 #pragma unroll
-        for (int c = 0; c < 4; ++c) p[c] = ex2(s[n][c] - base[n][c & 1]);
-        l[n][0] += p[0] + p[2], l[n][1] += p[1] + p[3];
-        pb[n][0] = movmatrix(pack2<M>(p[0], p[1])), pb[n][1] = movmatrix(pack2<M>(p[2], p[3]));
-      }
+        for (int n = 0; n < NT; ++n) {
+          float p[4];
 #pragma unroll
-      for (int w = 0; w < S::VW; ++w) {
-        if constexpr (F8) {
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const uint32_t x = __byte_perm(vr[0][w], vr[1][w], i ? 0x7362 : 0x5140), y = __byte_perm(vr[2][w], vr[3][w], i ? 0x7362 : 0x5140);
-            const uint32_t a0 = e4m3x2_f16x2(x), a1 = e4m3x2_f16x2(x >> 16), a2 = e4m3x2_f16x2(y), a3 = e4m3x2_f16x2(y >> 16);
-#pragma unroll
-            for (int n = 0; n < NT; ++n) mma16816<M>(o[2 * w + i][n], a0, a1, a2, a3, pb[n][0], pb[n][1]);
-          }
-        } else {
-          const uint32_t a0 = __byte_perm(vr[0][w], vr[1][w], 0x5410), a1 = __byte_perm(vr[0][w], vr[1][w], 0x7632);
-          const uint32_t a2 = __byte_perm(vr[2][w], vr[3][w], 0x5410), a3 = __byte_perm(vr[2][w], vr[3][w], 0x7632);
-#pragma unroll
-          for (int n = 0; n < NT; ++n) mma16816<M>(o[w][n], a0, a1, a2, a3, pb[n][0], pb[n][1]);
+          for (int c = 0; c < 4; ++c) p[c] = ex2(s[u][n][c] - base[n][c & 1]);
+          l[n][0] += p[0] + p[2], l[n][1] += p[1] + p[3];
+          pb[u][n][0] = movmatrix(pack2<M>(p[0], p[1])), pb[u][n][1] = movmatrix(pack2<M>(p[2], p[3]));
         }
-      }
+#pragma unroll
+      for (int u = 0; u < S::U; ++u)
+#pragma unroll
+        for (int w = 0; w < S::VW; ++w) {
+          if constexpr (F8) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const uint32_t x = __byte_perm(vr[u][0][w], vr[u][1][w], i ? 0x7362 : 0x5140), y = __byte_perm(vr[u][2][w], vr[u][3][w], i ? 0x7362 : 0x5140);
+              const uint32_t a0 = e4m3x2_f16x2(x), a1 = e4m3x2_f16x2(x >> 16), a2 = e4m3x2_f16x2(y), a3 = e4m3x2_f16x2(y >> 16);
+#pragma unroll
+              for (int n = 0; n < NT; ++n) mma16816<M>(o[2 * w + i][n], a0, a1, a2, a3, pb[u][n][0], pb[u][n][1]);
+            }
+          } else {
+            const uint32_t a0 = __byte_perm(vr[u][0][w], vr[u][1][w], 0x5410), a1 = __byte_perm(vr[u][0][w], vr[u][1][w], 0x7632);
+            const uint32_t a2 = __byte_perm(vr[u][2][w], vr[u][3][w], 0x5410), a3 = __byte_perm(vr[u][2][w], vr[u][3][w], 0x7632);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) mma16816<M>(o[w][n], a0, a1, a2, a3, pb[u][n][0], pb[u][n][1]);
+          }
+        }
       if (more) {
         load_v(next);
         if (tile + 2 * slices < tile_end) next = locate(tile + 2 * slices);
@@ -550,12 +586,19 @@ __global__ void __launch_bounds__(PA_THREADS, AttendShape<F8, D, NT>::CTAS) atte
     if (!whole && tid == 0) a.parts[slot] = make_int4(r, unit, (int)c0, (int)(c1 - c0) + 1);
     __syncthreads();
   }
-done:
+
+  // ---- rows without a visible key ----
+  for (int r = blockIdx.x; r < a.requests; r += gridDim.x) {
+    if (span_of<S>(a, r).steps) continue;
+    for (int i = tid; i < a.heads * D; i += PA_THREADS) store_out(a.out, a.out_dtype, (long long)r * a.heads * D + i, 0.f);
+    if (a.lse)
+      for (int i = tid; i < a.heads; i += PA_THREADS) a.lse[(long long)r * a.heads + i] = -INFINITY;
+  }
   if (a.status && flags) atomicOr(a.status, flags);
 }
 
 struct AttendLaunch {
-  int unit_heads, tiles, head_blocks, ctas_per_sm;
+  int unit_heads, tiles, head_blocks, ctas_per_sm, step;
 };
 // head tiles and units of a group of query heads
 template <bool F8, int D, int NT>
@@ -565,7 +608,7 @@ AttendLaunch attend_shape(int group) {
   l.tiles = need >= 3 ? 4 : need;
   l.unit_heads = l.tiles * 8 * NT;
   l.head_blocks = (group + l.unit_heads - 1) / l.unit_heads;
-  l.ctas_per_sm = AttendShape<F8, D, NT>::CTAS;
+  l.ctas_per_sm = AttendShape<F8, D, NT>::CTAS, l.step = AttendShape<F8, D, NT>::STEP;
   return l;
 }
 // Up to 8 query heads per key-value head take one MMA column tile per warp, more take two where the registers hold them.
