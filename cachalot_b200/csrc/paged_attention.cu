@@ -19,57 +19,98 @@ struct JoinArgs {
   float* lse;
 };
 
-// One CTA per CTA of the attention kernel.  The n CTAs that hold a part of a unit share its heads: head i belongs to the
-// (i mod n)-th of them.  Few parts (n below the number of heads): a warp takes a head of its own; many parts: the four
-// warps split a head's parts and meet in shared memory.  Part 0 of a unit is the second record of its CTA (the unit
+// Some elements of an output head in the making, from the parts that a lane has seen: running maximum and sum with them.
+template <int E>
+struct Joined {
+  float m = -INFINITY, l = 0.f, v[E] = {};
+  __device__ __forceinline__ void add(float om, float ol, const float (&o)[E]) {
+    const float top = fmaxf(m, om), f = m == -INFINITY ? 0.f : ex2(m - top), g = om == -INFINITY ? 0.f : ex2(om - top);
+    m = top, l = l * f + ol * g;
+#pragma unroll
+    for (int e = 0; e < E; ++e) v[e] = v[e] * f + o[e] * g;
+  }
+  __device__ __forceinline__ void across(int lanes) {  // with the lane `lanes` away
+    float o[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) o[e] = __shfl_xor_sync(0xffffffffu, v[e], lanes);
+    add(__shfl_xor_sync(0xffffffffu, m, lanes), __shfl_xor_sync(0xffffffffu, l, lanes), o);
+  }
+};
+
+// One CTA per CTA of the attention kernel.  The n CTAs that hold a part of a unit share its work:
+//   n <= 8   a task is a head, a warp's; its lanes hold the whole head and go through the parts
+//   n <= 32  a task is 32 elements of a head, a warp's; eight lanes hold them, four parts at a time
+//   n > 32   the same for a whole CTA, 16 parts at a time
+// so that there are one or two rounds of loads in each case.  Part 0 of a unit is the second record of its CTA (the unit
 // began there), the others are the first record of theirs.
 template <int D>
 __global__ void __launch_bounds__(PA_THREADS) attend_join_kernel(const JoinArgs a) {
-  constexpr int E = D / 32;
-  __shared__ float sums[PA_WARPS][D];
+  __shared__ Joined<4> shared[PA_WARPS][8];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   for (int which = 0; which < 2; ++which) {
     const int4 u = a.parts[blockIdx.x * 2 + which];  // request, unit, first CTA, CTAs
     if (u.w == 0) continue;
-    const int n = u.w, h = u.y / a.head_blocks, head0 = u.y % a.head_blocks * a.unit_heads;
+    const int n = u.w, h = u.y / a.head_blocks, head0 = u.y % a.head_blocks * a.unit_heads, me = (int)blockIdx.x - u.z;
     const int heads = min(a.unit_heads, a.group - head0);
-    const bool together = n >= heads;
     const long long row0 = (long long)u.x * a.heads + (long long)h * a.group + head0;
     const float v_scale = a.v_scale ? a.v_scale[h] : 1.f;
-    for (int i = (int)blockIdx.x - u.z + (together ? 0 : warp * n); i < heads; i += together ? n : PA_WARPS * n) {
-      auto slot = [&](int p) { return ((long long)(u.z + p) * 2 + (p == 0)) * a.unit_heads + i; };
-      float top = -INFINITY, sum = 0.f;
-      for (int p = lane; p < n; p += 32) top = fmaxf(top, a.part_ml[slot(p)].x);
-      top = warp_max(top);
-      for (int p = lane; p < n; p += 32) {
-        const float2 ml = a.part_ml[slot(p)];
-        sum += ml.x == -INFINITY ? 0.f : ml.y * ex2(ml.x - top);
-      }
-      sum = warp_sum(sum);
-      float v[E];
+    // parts p0, p0 + every, .. of elements d, d + stride, .. of a head
+    auto gather = [&](auto& j, int p0, int every, int head, int d, auto vec) {
+      constexpr int E = sizeof(j.v) / sizeof(float);
+      for (int p = p0; p < n; p += 4 * every) {
+        float2 ml[4];
+        float o[4][E];
 #pragma unroll
-      for (int e = 0; e < E; ++e) v[e] = 0.f;
-#pragma unroll 4
-      for (int p = together ? warp : 0; p < n; p += together ? PA_WARPS : 1) {
-        const float m = a.part_ml[slot(p)].x, f = m == -INFINITY ? 0.f : ex2(m - top);
-        const float* from = a.part_o + slot(p) * D + lane;
+        for (int i = 0; i < 4; ++i) {
+          const int q = p + i * every;
+          const long long slot = ((long long)(u.z + q) * 2 + (q == 0)) * a.unit_heads + head;
+          ml[i] = q < n ? a.part_ml[slot] : make_float2(-INFINITY, 0.f);
+          const float* from = a.part_o + slot * D + d;
+          if constexpr (decltype(vec)::value) {
+            const float4 x = q < n ? *reinterpret_cast<const float4*>(from) : make_float4(0.f, 0.f, 0.f, 0.f);
+            o[i][0] = x.x, o[i][1] = x.y, o[i][2] = x.z, o[i][3] = x.w;
+          } else {
 #pragma unroll
-        for (int e = 0; e < E; ++e) v[e] = fmaf(from[32 * e], f, v[e]);
+            for (int e = 0; e < E; ++e) o[i][e] = q < n ? from[32 * e] : 0.f;
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) j.add(ml[i].x, ml[i].y, o[i]);
       }
-      const float inv = sum == 0.f ? 0.f : v_scale / sum;
+    };
+    auto finish = [&](const auto& j, int head, int d, int stride) {
+      constexpr int E = sizeof(j.v) / sizeof(float);
+      const float inv = j.l == 0.f ? 0.f : v_scale / j.l;
+#pragma unroll
+      for (int e = 0; e < E; ++e) store_out(a.out, a.out_dtype, (row0 + head) * D + d + e * stride, j.v[e] * inv);
+      if (a.lse && d == 0) a.lse[row0 + head] = j.l == 0.f ? -INFINITY : (j.m - a.shift + log2f(j.l)) * PA_LN2;
+    };
+    if (n <= 8) {
+      for (int head = me * PA_WARPS + warp; head < heads; head += n * PA_WARPS) {
+        Joined<D / 32> j;
+        gather(j, 0, 1, head, lane, std::false_type{});
+        finish(j, head, lane, 32);
+      }
+      continue;
+    }
+    const bool together = n > 32;
+    const int sub = lane >> 3, at = (lane & 7) * 4;
+    for (int task = together ? me : me * PA_WARPS + warp; task < heads * (D / 32); task += together ? n : n * PA_WARPS) {
+      const int head = task / (D / 32), d = task % (D / 32) * 32 + at;
+      Joined<4> j;
+      gather(j, together ? warp * 4 + sub : sub, together ? 4 * PA_WARPS : 4, head, d, std::true_type{});
+      __syncwarp();
+      j.across(8), j.across(16);
       if (together) {
+        if (sub == 0) shared[warp][lane] = j;
         __syncthreads();
-#pragma unroll
-        for (int e = 0; e < E; ++e) sums[warp][lane + 32 * e] = v[e];
+        j = shared[sub][lane & 7];
+        j.across(8), j.across(16);
         __syncthreads();
-        for (int d = threadIdx.x; d < D; d += PA_THREADS)
-          store_out(a.out, a.out_dtype, (row0 + i) * D + d, (sums[0][d] + sums[1][d] + sums[2][d] + sums[3][d]) * inv);
-      } else {
-#pragma unroll
-        for (int e = 0; e < E; ++e) store_out(a.out, a.out_dtype, (row0 + i) * D + lane + 32 * e, v[e] * inv);
+        if (warp) continue;
       }
-      if (a.lse && lane == 0 && (!together || warp == 0)) a.lse[row0 + i] = sum == 0.f ? -INFINITY : (top - a.shift + log2f(sum)) * PA_LN2;
+      if (sub == 0) finish(j, head, d, 1);
     }
   }
 }
