@@ -182,6 +182,8 @@ extern "C" int cachalot_paged_attention(const void* q, int64_t q_row_stride, int
   a.page_shift = -1;
   for (int s = 0; s < 28; ++s)
     if (a.c.page_size == 8 << s) a.page_shift = s;
+  const uint64_t pieces = (uint64_t)a.c.page_size / 8;
+  a.page_magic = pieces > 0 && pieces < 128 ? ((1ull << 35) + pieces - 1) / pieces : 0;
   const int step_bytes = l.step * 2 * a.c.head_dim * paged_elem_bytes(a.c.dtype);
   a.unit_cost = (48 * 1024 + step_bytes - 1) / step_bytes;
   a.scale = scale, a.softcap = softcap, a.window = window, a.out = out, a.out_dtype = out_dtype, a.lse = lse, a.status = status;

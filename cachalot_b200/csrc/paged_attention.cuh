@@ -42,6 +42,7 @@ struct AttendArgs {
   int requests, heads, group;      // group: query heads per key-value head
   int tiles, head_blocks;          // head tiles (of 8 NT heads) a CTA's warps are split over; units per key-value head
   int page_shift;                  // log2(page_size / 8) or -1; tokens one by one where the page size is no multiple of 8
+  uint64_t page_magic;             // ceil(2^35 / (page_size / 8)) for page sizes below 1024, else 0
   int unit_cost;                   // what beginning a unit costs, in steps
   float scale, softcap;
   int window;
@@ -299,7 +300,10 @@ __global__ void __launch_bounds__(PA_THREADS, AttendShape<F8, D, NT>::CTAS) atte
 #pragma unroll
         for (int i = 0; i < 2 * S::U; ++i) {
           const int token = tile * S::TILE + 8 * i;
-          const int index = a.page_shift >= 0 ? (token >> 3) >> a.page_shift : token / a.c.page_size;
+          // token / 8 < 2^28 and page_size / 8 < 2^7, so the magic product is exact and fits 64 bits
+          const int index = a.page_shift >= 0 ? (token >> 3) >> a.page_shift
+                            : a.page_magic    ? (int)((uint64_t)(uint32_t)(token >> 3) * a.page_magic >> 35)
+                                              : token / a.c.page_size;
           p.off[i] = token - index * a.c.page_size;
           p.page[i] = token + 8 <= sp.lo ? -1 : page_of(token, index);
           p.full = p.full && p.page[i] >= 0;

@@ -11,7 +11,7 @@
 // The alternatives are kept as 64-bit keys (value mapped to an ordered integer, complement of the index: all distinct,
 // ties to the lower index).  The first round of a CTA finds the n-th largest of its 256 threads' own maxima, a lower
 // bound of the n-th best that only about n of the round's elements reach; from then on a thread looks closer only when its
-// maximum reaches that bar and appends what does to a list in shared memory.  After 2, 4, 8 .. rounds the bar is taken from
+// maximum reaches that bar and appends what does to a list in shared memory.  After 4, 8, 16 .. rounds the bar is taken from
 // the list again, so about n elements are appended per doubling on logits in no particular order.  Where the list
 // overflows (rising logits, many equal ones) the share is read once more with the bar raised as needed.
 // Selections are bitonic: warps sort 32 keys across their lanes and merge sorted lists.
@@ -120,18 +120,19 @@ __device__ __forceinline__ unsigned merge32(unsigned a, unsigned b, int lane) {
   return x;
 }
 
-// ... of the warps' sorted lists, in warp 0 and in lists[0]
+// ... of the first `n` warps' sorted lists, in warp 0 and in lists[0]; the others' lists are empty
 template <typename K>
-__device__ __forceinline__ K merge_block(K x, K (*lists)[32], int warp, int lane) {
+__device__ __forceinline__ K merge_block(K x, K (*lists)[32], int warp, int lane, int n = TL_WARPS) {
   lists[warp][lane] = x;
-#pragma unroll
-  for (int step = 1; step < TL_WARPS; step <<= 1) {
+  for (int step = 1; step < n; step <<= 1) {
     __syncthreads();
     if (warp % (2 * step) == 0) lists[warp][lane] = x = merge32(x, lists[warp + step][lane], lane);
   }
   __syncthreads();
   return x;
 }
+// warps that sort a list of this length, 32 at a time each
+__device__ __forceinline__ int warps_of(int length) { return min((length + 31) / 32, TL_WARPS); }
 
 // 16 bytes of logits
 template <typename T>
@@ -308,8 +309,8 @@ __global__ void __launch_bounds__(TL_THREADS, TL_CTAS) token_logprobs_kernel(con
   V next[TL_LOADS];
   sh.fetch(next, 0);
   if (TOP && tid == 0) added[0] = 0;
-  auto nth = [&](unsigned sorted) {  // of the warps' sorted values the n-th largest
-    merge_block(sorted, bars, warp, lane);
+  auto nth = [&](unsigned sorted, int warps) {  // of the warps' sorted values the n-th largest
+    merge_block(sorted, bars, warp, lane, warps);
     const unsigned r = bars[0][top - 1];
     __syncthreads();
     return r;
@@ -330,20 +331,20 @@ __global__ void __launch_bounds__(TL_THREADS, TL_CTAS) token_logprobs_kernel(con
     const float2 s2 = both(part.s), u2 = both(part.u);
     sum.s += s2.x + s2.y, sum.u += u2.x + u2.y;
     if constexpr (TOP) {
-      if (round == 0) bar = value_of(nth(sort32(order_of(most), lane)));
+      if (round == 0) bar = value_of(nth(sort32(order_of(most), lane), TL_WARPS));
       if (most >= bar) {
 #pragma unroll
         for (int k = 0; k < TL_LOADS; ++k)
           if (tops[k] >= bar) offer(sh, now[k], sh.index(round, k), 0, bar, list, 0, added);
       }
-      if (round > 0 && (round & (round + 1)) == 0 && round + 1 < sh.rounds) {  // as many rounds ahead as behind: the bar from the list
+      if (round > 2 && (round & (round + 1)) == 0 && round + 1 < sh.rounds) {  // about as many ahead as behind: the bar from the list
         __syncthreads();
         const int held = added[0];
         if (held <= TL_LIST) {
           unsigned mine = 0;
           for (int at = warp * 32; at < held; at += TL_THREADS)
             mine = merge32(mine, sort32(at + lane < held ? (unsigned)(list[at + lane] >> 32) : 0u, lane), lane);
-          bar = fmaxf(bar, value_of(nth(mine)));
+          bar = fmaxf(bar, value_of(nth(mine, warps_of(held))));
         }
       }
     }
@@ -364,7 +365,7 @@ __global__ void __launch_bounds__(TL_THREADS, TL_CTAS) token_logprobs_kernel(con
     int held = added[0];
     if (held > TL_LIST) held = select_carefully(sh, top, list, lists, added);
     for (int at = warp * 32; at < held; at += TL_THREADS) best = merge32(best, sort32(at + lane < held ? list[at + lane] : 0, lane), lane);
-    best = merge_block(best, lists, warp, lane);
+    best = merge_block(best, lists, warp, lane, warps_of(held));
   }
   if (warp == 0) {
     sum = parts[lane % TL_WARPS];
@@ -382,7 +383,7 @@ __global__ void __launch_bounds__(TL_THREADS, TL_CTAS) token_logprobs_kernel(con
       }
     }
     cluster.sync();  // nobody leaves, and no list is written, before all have been read
-    if (TOP && rank == 0) best = merge_block(warp < ctas ? best : 0, lists, warp, lane);
+    if (TOP && rank == 0) best = merge_block(warp < ctas ? best : 0, lists, warp, lane, ctas);
   }
   if (rank == 0 && warp == 0) {
     const float log_s = logf(sum.s);
