@@ -8,13 +8,14 @@
 // worked on.  A row is split over a cluster of CTAs where there are few rows, joined through distributed shared memory:
 // one launch, no workspace.
 //
-// The alternatives are kept as 64-bit keys (value mapped to an ordered integer, complement of the index: all distinct,
-// ties to the lower index).  The first round of a CTA finds the n-th largest of its 256 threads' own maxima, a lower
-// bound of the n-th best that only about n of the round's elements reach; from then on a thread looks closer only when its
-// maximum reaches that bar and appends what does to a list in shared memory.  After 4, 8, 16 .. rounds the bar is taken from
-// the list again, so about n elements are appended per doubling on logits in no particular order.  Where the list
-// overflows (rising logits, many equal ones) the share is read once more with the bar raised as needed.
-// Selections are bitonic: warps sort 32 keys across their lanes and merge sorted lists.
+// The alternatives.  The first round of a CTA finds the n-th largest of its 256 threads' own maxima, a lower bound ("bar")
+// of the n-th best that about n threads reach; from then on a thread whose maximum reaches the bar appends that maximum and
+// its place to a list in shared memory, and after 4, 8, 16 .. rounds the bar is raised to the list's n-th largest: about n
+// entries per doubling on logits in no particular order.  At the end the entries that reach the last bar, about n, are read again, an
+// element per lane, and their elements that reach it sorted as 64-bit keys (value mapped to an ordered integer, complement
+// of the index: all distinct, ties to the lower index).  Where a list overflows (rising logits, many equal ones) the share is
+// read once more, bar raised as needed.  Selections are bitonic: warps sort 32 keys across their lanes and merge sorted lists.
+// (Keeping the elements themselves while passing by cost 500 instructions for every thread that had one.)
 #include <cfloat>
 #include <cmath>
 #include <cooperative_groups.h>
@@ -29,6 +30,7 @@ namespace cg = cooperative_groups;
 
 constexpr int TL_THREADS = 256, TL_WARPS = TL_THREADS / 32, TL_MAX_TOP = 32, TL_LOADS = 4;
 constexpr int TL_CTAS = 4;     // per SM: up to 64 KB of loads in flight
+constexpr int TL_SEEN = 1024;
 constexpr int TL_LIST = 1088;  // 32 kept + 32 threads of 32 elements
 constexpr float TL_LOG2E = 1.4426950408889634f;
 constexpr float TL_FAR = -200.f;  // e^-200 is zero in fp32; stands for -inf, which would make 0 * -inf
@@ -195,9 +197,10 @@ struct Share {
     shift = (int)(reinterpret_cast<uintptr_t>(r) % 16 / sizeof(T));
     rounds = ((n + shift + Vec<T>::PER - 1) / Vec<T>::PER + c * TL_LOADS * TL_THREADS - 1) / (c * TL_LOADS * TL_THREADS);
   }
-  __device__ __forceinline__ int index(int round, int k) const {  // of the first element of a thread's k-th vector
-    return (((round * ctas + rank) * TL_LOADS + k) * TL_THREADS + (int)threadIdx.x) * Vec<T>::PER - shift;
+  __device__ __forceinline__ int index(int round, int k, int thread) const {  // of the first element of a thread's k-th vector
+    return (((round * ctas + rank) * TL_LOADS + k) * TL_THREADS + thread) * Vec<T>::PER - shift;
   }
+  __device__ __forceinline__ int index(int round, int k) const { return index(round, k, (int)threadIdx.x); }
   __device__ __forceinline__ void fetch(Vec<T> (&v)[TL_LOADS], int round) const {
 #pragma unroll
     for (int k = 0; k < TL_LOADS; ++k) v[k].load(row, index(round, k), vocab);
@@ -217,39 +220,28 @@ __device__ __forceinline__ Key best_of(const Share<T>& sh, const Vec<T> (&v)[TL_
     }
   return best;
 }
+// A thread's elements of a round that reach the bar, appended to the list.
 template <typename T>
-__device__ __forceinline__ void offer_one(float x, int i, int vocab, Key bar, float bar_value, Key* list, int base, int* count) {
-  if (x >= bar_value && i >= 0 && i < vocab) {
-    const Key key = key_of(x, i);
-    if (key >= bar) {
-      const int at = base + atomicAdd(count, 1);
-      if (at < TL_LIST) list[at] = key;
+__device__ __forceinline__ void offer(const Share<T>& sh, const Vec<T> (&v)[TL_LOADS], int round, Key bar, float bar_value, Key* list, int base, int* count) {
+#pragma unroll
+  for (int k = 0; k < TL_LOADS; ++k) {
+    if (!(v[k].top() >= bar_value)) continue;
+#pragma unroll
+    for (int j = 0; j < Vec<T>::PER; ++j) {
+      const float x = v[k].at(j);
+      const int i = sh.index(round, k) + j;
+      if (x >= bar_value && i >= 0 && i < sh.vocab) {
+        const Key key = key_of(x, i);
+        if (key >= bar) {
+          const int at = base + atomicAdd(count, 1);
+          if (at < TL_LIST) list[at] = key;
+        }
+      }
     }
   }
 }
-// 16-bit logits: a function of its own and a loop over the words.  A vector that reaches the bar is rare, and code that is
-// seldom run is fetched slowly: unrolled into the main loop, 32 elements of it, 2048 rows with 8 alternatives took 162 us
-// instead of 130.  (The 16 elements of a round of float32 are better off in the loop: 187 us against 210 with the call.)
-template <typename T>
-__device__ __noinline__ void offer_rare(Vec<T> v, int first, int vocab, Key bar, float bar_value, Key* list, int base, int* count) {
-#pragma unroll 1
-  for (int w = 0; w < 4; ++w) {
-#pragma unroll
-    for (int j = 0; j < Vec<T>::PER / 4; ++j) offer_one<T>(v.at(j), first + w * (Vec<T>::PER / 4) + j, vocab, bar, bar_value, list, base, count);
-    v.raw = make_uint4(v.raw.y, v.raw.z, v.raw.w, v.raw.x);
-  }
-}
-template <typename T>
-__device__ __forceinline__ void offer(const Vec<T>& v, int first, int vocab, Key bar, float bar_value, Key* list, int base, int* count) {
-  if constexpr (sizeof(T) == 2) {
-    offer_rare(v, first, vocab, bar, bar_value, list, base, count);
-  } else {
-#pragma unroll
-    for (int j = 0; j < Vec<T>::PER; ++j) offer_one<T>(v.at(j), first + j, vocab, bar, bar_value, list, base, count);
-  }
-}
 
-// The careful selection, for rows whose list overflowed: over the share once more, the bar raised in every round that would
+// The careful selection, for rows where a list overflowed: over the share once more, the bar raised in every round that would
 // overflow the list, from the list and the threads' own best together (at most n threads reach it, so at most 32 n elements).
 // Returns the length of the list.  `added`: three counters for the rounds in turn (one counted, one still read, one cleared).
 template <typename T>
@@ -271,8 +263,7 @@ __device__ __noinline__ int select_carefully(const Share<T> sh, int top, Key* li
     int* count = &added[round % 3];
     if (tid == 0) added[(round + 1) % 3] = 0;
     auto offer_all = [&](int base) {
-      if (most >= bar_value)
-        for (int k = 0; k < TL_LOADS; ++k) offer(v[k], sh.index(round, k), sh.vocab, bar, bar_value, list, base, count);
+      if (most >= bar_value) offer(sh, v, round, bar, bar_value, list, base, count);
     };
     if (round > 0) {
       offer_all(held);
@@ -312,7 +303,8 @@ __global__ void __launch_bounds__(TL_THREADS, TL_CTAS) token_logprobs_kernel(con
   __shared__ Sums parts[TL_WARPS];
   __shared__ Key lists[TOP ? TL_WARPS : 1][32];
   __shared__ Key list[TOP ? TL_LIST : 1];
-  __shared__ int added[3];
+  __shared__ uint2 seen[TOP ? TL_SEEN : 1];  // maxima that reached the bar: ordered value, round * threads + thread
+  __shared__ int added[3], noted;
   unsigned(*bars)[32] = reinterpret_cast<unsigned(*)[32]>(lists);
   cg::cluster_group cluster = cg::this_cluster();
   const int ctas = cluster.num_blocks(), rank = cluster.block_rank();
@@ -324,18 +316,26 @@ __global__ void __launch_bounds__(TL_THREADS, TL_CTAS) token_logprobs_kernel(con
   float bar = -INFINITY;  // nothing below it is among the best
   V next[TL_LOADS];
   sh.fetch(next, 0);
-  if (TOP && tid == 0) added[0] = 0;
+  if (TOP && tid == 0) added[0] = noted = 0;
   auto nth = [&](unsigned sorted, int warps) {  // of the warps' sorted values the n-th largest
     merge_block(sorted, bars, warp, lane, warps);
     const unsigned r = bars[0][top - 1];
     __syncthreads();
     return r;
   };
+  auto raise = [&] {  // to the n-th largest of the maxima so far
+    __syncthreads();
+    const int n = noted;
+    if (n > TL_SEEN) return;
+    unsigned mine = 0;
+    for (int at = warp * 32; at < n; at += TL_THREADS) mine = merge32(mine, sort32(at + lane < n ? seen[at + lane].x : 0u, lane), lane);
+    bar = fmaxf(bar, value_of(nth(mine, warps_of(n))));
+  };
   for (int round = 0; round < sh.rounds; ++round) {
     V now[TL_LOADS];
-    float tops[TL_LOADS], most = -INFINITY;
+    float most = -INFINITY;
 #pragma unroll
-    for (int k = 0; k < TL_LOADS; ++k) now[k] = next[k], tops[k] = now[k].top(), most = fmaxf(most, tops[k]);
+    for (int k = 0; k < TL_LOADS; ++k) now[k] = next[k], most = fmaxf(most, now[k].top());
     if (round + 1 < sh.rounds) sh.fetch(next, round + 1);
     if (most > sum.m) sum.move(most);
     PairSums part;
@@ -349,20 +349,10 @@ __global__ void __launch_bounds__(TL_THREADS, TL_CTAS) token_logprobs_kernel(con
     if constexpr (TOP) {
       if (round == 0) bar = value_of(nth(sort32(order_of(most), lane), TL_WARPS));
       if (most >= bar) {
-#pragma unroll
-        for (int k = 0; k < TL_LOADS; ++k)
-          if (tops[k] >= bar) offer(now[k], sh.index(round, k), vocab, 0, bar, list, 0, added);
+        const int at = atomicAdd(&noted, 1);
+        if (at < TL_SEEN) seen[at] = make_uint2(order_of(most), round * TL_THREADS + tid);
       }
-      if (round > 2 && (round & (round + 1)) == 0 && round + 1 < sh.rounds) {  // about as many ahead as behind: the bar from the list
-        __syncthreads();
-        const int held = added[0];
-        if (held <= TL_LIST) {
-          unsigned mine = 0;
-          for (int at = warp * 32; at < held; at += TL_THREADS)
-            mine = merge32(mine, sort32(at + lane < held ? (unsigned)(list[at + lane] >> 32) : 0u, lane), lane);
-          bar = fmaxf(bar, value_of(nth(mine, warps_of(held))));
-        }
-      }
+      if (round > 2 && (round & (round + 1)) == 0 && round + 1 < sh.rounds) raise();
     }
   }
 
@@ -378,7 +368,25 @@ __global__ void __launch_bounds__(TL_THREADS, TL_CTAS) token_logprobs_kernel(con
   Key best = 0;
   __syncthreads();
   if constexpr (TOP) {
-    int held = added[0];
+    raise();
+    const int n = noted;
+    int held = TL_LIST + 1;
+    if (n <= TL_SEEN) {  // the elements of the entries that reach the bar, a lane each
+      for (int at = warp; at < n; at += TL_WARPS) {
+        const uint2 entry = seen[at];
+        if (!(value_of(entry.x) >= bar)) continue;
+        const int i = sh.index(entry.y / TL_THREADS, lane / PER % TL_LOADS, entry.y % TL_THREADS) + lane % PER;
+        const bool there = lane < PER * TL_LOADS && i >= 0 && i < vocab;
+        const float v = there ? V::widen(x[i]) : 0.f;
+        const unsigned hit = __ballot_sync(0xffffffffu, there && v >= bar);
+        int to = 0;
+        if (lane == 0) to = atomicAdd(added, __popc(hit));
+        to = __shfl_sync(0xffffffffu, to, 0) + __popc(hit & ((1u << lane) - 1));
+        if ((hit >> lane & 1) && to < TL_LIST) list[to] = key_of(v, i);
+      }
+      __syncthreads();
+      held = added[0];
+    }
     if (held > TL_LIST) held = select_carefully(sh, top, list, lists, added);
     for (int at = warp * 32; at < held; at += TL_THREADS) best = merge32(best, sort32(at + lane < held ? list[at + lane] : 0, lane), lane);
     best = merge_block(best, lists, warp, lane, warps_of(held));
