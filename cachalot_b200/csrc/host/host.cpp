@@ -407,6 +407,28 @@ PyObject* moe_block(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
 
 // ---- the decode step around the experts ----
 
+// Several outputs in one allocation, 256-byte aligned each: an allocation costs 0.6 us, a tensor over a piece of one 0.1.
+// The pieces share their storage: it lives as long as any of them.
+struct Pieces {
+  c10::Device device;
+  int64_t bytes = 0;
+  at::Tensor all;
+  explicit Pieces(int dev) : device(c10::kCUDA, (c10::DeviceIndex)dev) {}
+  int64_t room(int64_t elements, ScalarType dt) {  // all of them first; the offset of the piece
+    const int64_t at = bytes;
+    bytes += (int64_t)up256((size_t)(elements * (int64_t)c10::elementSize(dt)));
+    return at;
+  }
+  void allocate() { all = empty({bytes > 0 ? bytes : 1}, ScalarType::Byte, device.index()); }
+  at::Tensor piece(int64_t at, std::initializer_list<int64_t> shape, ScalarType dt) const {
+    at::Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(all.storage()), c10::DispatchKeySet(c10::DispatchKey::CUDA),
+                                                            c10::scalarTypeToTypeMeta(dt));
+    t.unsafeGetTensorImpl()->set_storage_offset(at / (int64_t)c10::elementSize(dt));
+    t.unsafeGetTensorImpl()->set_sizes_contiguous(c10::IntArrayRef(shape.begin(), shape.size()));
+    return t;
+  }
+};
+
 // int32 [n], contiguous
 bool plain_ints(const at::Tensor* t, int64_t n, int device) { return plain(t, ScalarType::Int, device) && t->dim() == 1 && t->size(0) == n; }
 // int32 [rows, width] with contiguous rows that do not overlap
@@ -433,7 +455,11 @@ PyObject* plan_pages(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   PLAIN_OR_NONE(a[7] == Py_None || tensor_of(a[7])->numel() > 0);
   at::Tensor out[6];
   const int64_t sizes[6] = {r + 1, tokens, tokens, tokens, r, 1};
-  for (int i = 0; i < 6; ++i) out[i] = empty({sizes[i]}, ScalarType::Int, dev);
+  int64_t offset[6];
+  Pieces memory(dev);
+  for (int i = 0; i < 6; ++i) offset[i] = memory.room(sizes[i], ScalarType::Int);
+  memory.allocate();
+  for (int i = 0; i < 6; ++i) out[i] = memory.piece(offset[i], {sizes[i]}, ScalarType::Int);
   const int rc = UNLOCKED(lib.cachalot_plan_pages(ints(*ctx), ints(*fresh), (int)r, ints(*table), table->stride(0), (int)table->size(1), ints(*pages),
                                                   (int)pages->size(0), ints(*count), page, tokens, ints(out[0]), ints(out[1]), ints(out[2]),
                                                   ints(out[3]), ints(out[4]), ints(out[5]), static_cast<int*>(ptr_or_null(a[7])), current_stream(dev)));
@@ -567,8 +593,12 @@ PyObject* token_logprobs(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   const int64_t rows = x->size(0), vocab = x->size(1);
   PLAIN_OR_NONE(rows > 0 && rows < (1LL << 31) && vocab > 0 && vocab < (1LL << 31) && top >= 0 && top <= vocab && plain_ints(ids, rows, dev));
   PLAIN_OR_NONE(none_or_plain(a[3], ScalarType::Int, dev) && (a[3] == Py_None || tensor_of(a[3])->numel() > 0));
-  at::Tensor lp = empty({rows}, ScalarType::Float, dev), h = empty({rows}, ScalarType::Float, dev);
-  at::Tensor ti = empty({rows, top}, ScalarType::Int, dev), tv = empty({rows, top}, ScalarType::Float, dev);
+  Pieces memory(dev);
+  const int64_t at[4] = {memory.room(rows, ScalarType::Float), memory.room(rows, ScalarType::Float), memory.room(rows * top, ScalarType::Int),
+                         memory.room(rows * top, ScalarType::Float)};
+  memory.allocate();
+  at::Tensor lp = memory.piece(at[0], {rows}, ScalarType::Float), h = memory.piece(at[1], {rows}, ScalarType::Float);
+  at::Tensor ti = memory.piece(at[2], {rows, top}, ScalarType::Int), tv = memory.piece(at[3], {rows, top}, ScalarType::Float);
   const int rc = UNLOCKED(lib.cachalot_token_logprobs(x->data_ptr(), dt, x->stride(0), (int)rows, (int)vocab, ints(*ids), top, static_cast<float*>(lp.data_ptr()),
                                                       static_cast<float*>(h.data_ptr()), ints(ti), static_cast<float*>(tv.data_ptr()),
                                                       static_cast<int*>(ptr_or_null(a[3])), current_stream(dev)));

@@ -105,7 +105,7 @@ def plan_pages(context_lens: torch.Tensor, new_lens: torch.Tensor, block_table: 
     `free_count`, and pages given back are appended at that place."""
     p = _host.plan_pages(context_lens, new_lens, block_table, free_pages, free_count, page_size, tokens, status)
     if p is not None:
-        return PagePlan(*p)
+        return PagePlan._make(p)
     dev = _same_device(context_lens, new_lens, block_table, free_pages, free_count, status)
     r = context_lens.numel()
     ctx, new = _ints(context_lens, "context_lens", (r,)), _ints(new_lens, "new_lens", (r,))
@@ -289,7 +289,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, top: int = 0, 
     of -inf have no weight, and a row of nothing else gives -inf and entropy 0."""
     r = _host.token_logprobs(logits, tokens, top, status)
     if r is not None:
-        return TokenLogprobs(*r)
+        return TokenLogprobs._make(r)
     dev = _same_device(logits, tokens, status)
     if logits.dim() != 2 or logits.dtype not in (torch.float32, torch.bfloat16, torch.float16):
         raise ValueError(f"logits must be float32, bfloat16 or float16 [rows, vocab], got {logits.dtype} {tuple(logits.shape)}")
