@@ -82,6 +82,11 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
     return *reinterpret_cast<const uint32_t*>(&h);
   }
 }
+template <typename M>
+__device__ __forceinline__ float2 unpack2(uint32_t x) {
+  if constexpr (std::is_same<M, __half>::value) return __half22float2(*reinterpret_cast<const __half2*>(&x));
+  else return make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u));
+}
 __device__ __forceinline__ uint32_t movmatrix(uint32_t x) {
   uint32_t y;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
@@ -170,6 +175,7 @@ __global__ void __launch_bounds__(PA_THREADS, AttendShape<F8, D, NT>::CTAS) atte
   using S = AttendShape<F8, D, NT>;
   constexpr bool HALF = std::is_same<M, __half>::value;
   constexpr float SHIFT = HALF ? 7.f : 0.f, SLACK = 8.f;
+  constexpr int TERMS = F8 ? 1 : 2;  // of P
   extern __shared__ __align__(16) uint8_t smem[];
   uint2* sq = reinterpret_cast<uint2*>(smem);                                        // [tiles * NT][KSTEPS][32]
   float* so = reinterpret_cast<float*>(smem + S::Q_BYTES(a.tiles));                  // [warps][TILE_HEADS][O_PITCH]
@@ -495,7 +501,7 @@ __global__ void __launch_bounds__(PA_THREADS, AttendShape<F8, D, NT>::CTAS) atte
             for (int k = 0; k < S::KSTEPS; ++k) o[k][n][c] *= keep, o[k][n][c + 2] *= keep;
           }
       }
-      uint32_t pb[S::U][NT][2];
+      uint32_t pb[S::U][NT][TERMS][2];
 #pragma unroll
       for (int u = 0; u < S::U; ++u)
 #pragma unroll
@@ -504,7 +510,13 @@ __global__ void __launch_bounds__(PA_THREADS, AttendShape<F8, D, NT>::CTAS) atte
 #pragma unroll
           for (int c = 0; c < 4; ++c) p[c] = ex2(s[u][n][c] - base[n][c & 1]);
           l[n][0] += p[0] + p[2], l[n][1] += p[1] + p[3];
-          pb[u][n][0] = movmatrix(pack2<M>(p[0], p[1])), pb[u][n][1] = movmatrix(pack2<M>(p[2], p[3]));
+#pragma unroll
+          for (int i = 0; i < TERMS; ++i) {
+            const uint32_t lo = pack2<M>(p[0], p[1]), hi = pack2<M>(p[2], p[3]);
+            pb[u][n][i][0] = movmatrix(lo), pb[u][n][i][1] = movmatrix(hi);
+            const float2 x = unpack2<M>(lo), y = unpack2<M>(hi);
+            p[0] -= x.x, p[1] -= x.y, p[2] -= y.x, p[3] -= y.y;
+          }
         }
 #pragma unroll
       for (int u = 0; u < S::U; ++u)
@@ -516,13 +528,15 @@ __global__ void __launch_bounds__(PA_THREADS, AttendShape<F8, D, NT>::CTAS) atte
               const uint32_t x = __byte_perm(vr[u][0][w], vr[u][1][w], i ? 0x7362 : 0x5140), y = __byte_perm(vr[u][2][w], vr[u][3][w], i ? 0x7362 : 0x5140);
               const uint32_t a0 = e4m3x2_f16x2(x), a1 = e4m3x2_f16x2(x >> 16), a2 = e4m3x2_f16x2(y), a3 = e4m3x2_f16x2(y >> 16);
 #pragma unroll
-              for (int n = 0; n < NT; ++n) mma16816<M>(o[2 * w + i][n], a0, a1, a2, a3, pb[u][n][0], pb[u][n][1]);
+              for (int n = 0; n < NT; ++n) mma16816<M>(o[2 * w + i][n], a0, a1, a2, a3, pb[u][n][0][0], pb[u][n][0][1]);
             }
           } else {
             const uint32_t a0 = __byte_perm(vr[u][0][w], vr[u][1][w], 0x5410), a1 = __byte_perm(vr[u][0][w], vr[u][1][w], 0x7632);
             const uint32_t a2 = __byte_perm(vr[u][2][w], vr[u][3][w], 0x5410), a3 = __byte_perm(vr[u][2][w], vr[u][3][w], 0x7632);
 #pragma unroll
-            for (int n = 0; n < NT; ++n) mma16816<M>(o[w][n], a0, a1, a2, a3, pb[u][n][0], pb[u][n][1]);
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+              for (int i = 0; i < TERMS; ++i) mma16816<M>(o[w][n], a0, a1, a2, a3, pb[u][n][i][0], pb[u][n][i][1]);
           }
         }
       if (more) {

@@ -5,8 +5,9 @@ Tolerance per output element, with spread = sum p |v| / sum p of the element's h
     order, and the scaling; `reach` bounds it) and, under a soft cap, cap * 2^-18 of the approximate exp and reciprocal;
     a bf16 query over an E4M3 cache is held in f16 relative to its largest element (2^-24 of it per element, under dim
     times reach * 2^-24): e^d - 1 <= 2 d of every weight, in the sum above and below: 4 d * spread;
-  * a weight is rounded to the matrix type: half a step, 2^-8 bf16 / 2^-11 f16, of spread; in f16 also 2^-25 absolute on
-    weights that are shifted by 2^7 over the running maximum: 2^-32 of floor = sum |v| / sum p;
+  * a weight is rounded to the matrix type: over a 16-bit cache twice, the second time what the first left (half a step of half
+    a step: 2^-16 bf16, 2^-22 f16, of spread), over an E4M3 cache once to f16 (2^-11); in f16 also 2^-25 absolute on weights
+    that are shifted by 2^7 over the running maximum: 2^-32 of floor = sum |v| / sum p;
   * exp2 and the fp32 sums: 2^-16 of spread;
   * the result is rounded: half a step of the output type (none for float32).
 lse: the scores' d, 2^-16 for the sum of weights, 2^-22 of the value."""
@@ -93,7 +94,8 @@ class Case:
         wout, wlse, spread, reach, floor = want
         f16 = self.caches[0].dtype != BF16
         d = (self.dim * 2.0 ** -22 * reach + softcap * 2.0 ** -18 + (self.dim * 2.0 ** -24 * reach if self.caches[0].dtype == E4M3 else 0))
-        tol = (4 * d[..., None] + 2.0 ** -16 + HALF[F16 if f16 else BF16]) * spread + (2.0 ** -32 * floor if f16 else 0)
+        weight = {BF16: 2.0 ** -16, F16: 2.0 ** -22, E4M3: 2.0 ** -11}[self.caches[0].dtype]
+        tol = (4 * d[..., None] + 2.0 ** -16 + weight) * spread + (2.0 ** -32 * floor if f16 else 0)
         tol = tol + HALF[out.dtype] * (np.abs(wout) + tol) + (2.0 ** -25 if out.dtype == F16 else 0)
         got = out.double().cpu().numpy()
         bad = ~(np.abs(got - wout) <= tol)
