@@ -173,4 +173,20 @@ inline cudaError_t smem_optin_once(K kern, int bytes) {
   return e;
 }
 
+// Launches of kernels whose first statement is wait_for_predecessor(): the set-up of such a launch runs under the end of the
+// kernel before it in the stream (programmatic dependent launch) instead of after it.
+__device__ __forceinline__ void wait_for_predecessor() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+template <typename... Params, typename... Args>
+inline cudaError_t launch_early(void (*kern)(Params...), dim3 grid, int threads, size_t smem, cudaStream_t stream, int cluster, Args&&... args) {
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim = {(unsigned)cluster, 1, 1};
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid, cfg.blockDim = dim3((unsigned)threads), cfg.dynamicSmemBytes = smem, cfg.stream = stream;
+  cfg.attrs = at, cfg.numAttrs = cluster > 1 ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, kern, static_cast<Params>(args)...);
+}
+
 }  // namespace cachalot

@@ -1,5 +1,7 @@
 // Paged attention: argument checks, workspace, and the join of units that lie in several CTAs (the kernel itself:
 // paged_attention.cuh).
+#include <atomic>
+
 #include "paged_attention.cuh"
 
 namespace cachalot {
@@ -47,7 +49,7 @@ template <int D>
 __global__ void __launch_bounds__(PA_THREADS) attend_join_kernel(const JoinArgs a) {
   __shared__ Joined<4> shared[PA_WARPS][8];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  wait_for_predecessor();
   for (int which = 0; which < 2; ++which) {
     const int4 u = a.parts[blockIdx.x * 2 + which];  // request, unit, first CTA, CTAs
     if (u.w == 0) continue;
@@ -120,13 +122,17 @@ bool shape_of(bool f8, int dim, int group, AttendLaunch* l) {
   return f8 ? attend_dispatch<true>(dim, group, take) : attend_dispatch<false>(dim, group, take);
 }
 
-int sm_count() {
+int sm_count() {  // of the current device; an attribute of the device, asked for once
+  static std::atomic<int> known[16];
   int dev = 0, sms = 0;
+  if (cudaGetDevice(&dev) == cudaSuccess && dev >= 0 && dev < 16 && (sms = known[dev].load(std::memory_order_relaxed)) > 0) return sms;
   if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || sms <= 0) {
     (void)cudaGetLastError();
-    sms = PA_MAX_SMS;  // no device: sizes only
+    return PA_MAX_SMS;  // no device: sizes only
   }
-  return sms < PA_MAX_SMS ? sms : PA_MAX_SMS;
+  sms = sms < PA_MAX_SMS ? sms : PA_MAX_SMS;
+  if (dev < 16) known[dev].store(sms, std::memory_order_relaxed);
+  return sms;
 }
 
 size_t up(size_t v) { return (v + 255) / 256 * 256; }
@@ -201,18 +207,14 @@ extern "C" int cachalot_paged_attention(const void* q, int64_t q_row_stride, int
   if (rc) return rc;
   JoinArgs j{a.part_o, a.part_ml, a.parts, l.unit_heads, l.head_blocks, heads, a.group, a.c.head_dim,
              f8 || q_dtype == CACHALOT_F16 ? 7.f : 0.f, f8 ? a.c.v_scale : nullptr, out, out_dtype, lse};
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(ctas), cfg.blockDim = dim3(PA_THREADS), cfg.stream = s, cfg.attrs = &attr, cfg.numAttrs = 1;
   cudaError_t e = cudaSuccess;
+  auto join = [&](auto kern) { e = launch_early(kern, dim3(ctas), PA_THREADS, 0, s, 1, j); };
   switch (a.c.head_dim) {
-    case 64: e = cudaLaunchKernelEx(&cfg, attend_join_kernel<64>, j); break;
-    case 96: e = cudaLaunchKernelEx(&cfg, attend_join_kernel<96>, j); break;
-    case 128: e = cudaLaunchKernelEx(&cfg, attend_join_kernel<128>, j); break;
-    case 192: e = cudaLaunchKernelEx(&cfg, attend_join_kernel<192>, j); break;
-    default: e = cudaLaunchKernelEx(&cfg, attend_join_kernel<256>, j); break;
+    case 64: join(attend_join_kernel<64>); break;
+    case 96: join(attend_join_kernel<96>); break;
+    case 128: join(attend_join_kernel<128>); break;
+    case 192: join(attend_join_kernel<192>); break;
+    default: join(attend_join_kernel<256>); break;
   }
   if (e != cudaSuccess) return fail(CACHALOT_ECUDA, "paged_attention: %s", cudaGetErrorString(e));
   return check_launch("paged_attention");

@@ -92,10 +92,15 @@ __device__ __forceinline__ uint32_t movmatrix(uint32_t x) {
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
-// two E4M3 codes (low half of `x`) -> two f16
-__device__ __forceinline__ uint32_t e4m3x2_f16x2(uint32_t x) {
+// two E4M3 codes, the low or the high half of `x` -> two f16
+__device__ __forceinline__ uint32_t e4m3_lo(uint32_t x) {
   uint32_t y;
   asm("{\n.reg .b16 l, h;\nmov.b32 {l, h}, %1;\ncvt.rn.f16x2.e4m3x2 %0, l;\n}" : "=r"(y) : "r"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t e4m3_hi(uint32_t x) {
+  uint32_t y;
+  asm("{\n.reg .b16 l, h;\nmov.b32 {l, h}, %1;\ncvt.rn.f16x2.e4m3x2 %0, h;\n}" : "=r"(y) : "r"(x));
   return y;
 }
 
@@ -185,6 +190,7 @@ __global__ void __launch_bounds__(PA_THREADS, AttendShape<F8, D, NT>::CTAS) atte
   __shared__ long long shared_found_at;
   __shared__ int shared_found;
 
+  wait_for_predecessor();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
   const int per_request = a.c.kv_heads * a.head_blocks;
   int flags = 0;
@@ -457,8 +463,7 @@ __global__ void __launch_bounds__(PA_THREADS, AttendShape<F8, D, NT>::CTAS) atte
         for (int u = 0; u < S::U; ++u) {
           uint32_t a0, a1, a2, a3;
           if constexpr (F8) {
-            a0 = e4m3x2_f16x2(kr[u][0][k]), a1 = e4m3x2_f16x2(kr[u][1][k]);
-            a2 = e4m3x2_f16x2(kr[u][0][k] >> 16), a3 = e4m3x2_f16x2(kr[u][1][k] >> 16);
+            a0 = e4m3_lo(kr[u][0][k]), a1 = e4m3_lo(kr[u][1][k]), a2 = e4m3_hi(kr[u][0][k]), a3 = e4m3_hi(kr[u][1][k]);
           } else {
             a0 = kr[u][0][2 * k], a1 = kr[u][1][2 * k], a2 = kr[u][0][2 * k + 1], a3 = kr[u][1][2 * k + 1];
           }
@@ -468,6 +473,28 @@ __global__ void __launch_bounds__(PA_THREADS, AttendShape<F8, D, NT>::CTAS) atte
       }
       const int visible = seen;
       if (more) load_k(next);
+#pragma unroll
+      for (int u = 0; u < S::U; ++u)
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) s[u][n][c] *= hs[n][c & 1];
+      if (a.softcap > 0.f) {
+#pragma unroll
+        for (int u = 0; u < S::U; ++u)
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) s[u][n][c] = cap - __fdividef(2.f * cap, 1.f + ex2(s[u][n][c]));
+      }
+      if (visible != (1 << 2 * S::U) - 1) {
+#pragma unroll
+        for (int u = 0; u < S::U; ++u)
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) s[u][n][c] = visible >> (2 * u + (c >> 1)) & 1 ? s[u][n][c] : -INFINITY;
+      }
       bool higher = false;
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
@@ -475,12 +502,7 @@ __global__ void __launch_bounds__(PA_THREADS, AttendShape<F8, D, NT>::CTAS) atte
 #pragma unroll
         for (int u = 0; u < S::U; ++u)
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            float x = s[u][n][c] * hs[n][c & 1];
-            if (a.softcap > 0.f) x = cap - __fdividef(2.f * cap, 1.f + ex2(x));
-            s[u][n][c] = x = visible >> (2 * u + (c >> 1)) & 1 ? x : -INFINITY;
-            top[c & 1] = fmaxf(top[c & 1], x);
-          }
+          for (int c = 0; c < 4; ++c) top[c & 1] = fmaxf(top[c & 1], s[u][n][c]);
         higher = higher || top[0] > m[n][0] + SLACK || top[1] > m[n][1] + SLACK;
       }
       if (__any_sync(0xffffffffu, higher)) {
@@ -526,7 +548,7 @@ __global__ void __launch_bounds__(PA_THREADS, AttendShape<F8, D, NT>::CTAS) atte
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
               const uint32_t x = __byte_perm(vr[u][0][w], vr[u][1][w], i ? 0x7362 : 0x5140), y = __byte_perm(vr[u][2][w], vr[u][3][w], i ? 0x7362 : 0x5140);
-              const uint32_t a0 = e4m3x2_f16x2(x), a1 = e4m3x2_f16x2(x >> 16), a2 = e4m3x2_f16x2(y), a3 = e4m3x2_f16x2(y >> 16);
+              const uint32_t a0 = e4m3_lo(x), a1 = e4m3_hi(x), a2 = e4m3_lo(y), a3 = e4m3_hi(y);
 #pragma unroll
               for (int n = 0; n < NT; ++n) mma16816<M>(o[2 * w + i][n], a0, a1, a2, a3, pb[u][n][0][0], pb[u][n][0][1]);
             }
@@ -658,7 +680,7 @@ int launch_attend(AttendArgs& a, int dim, int ctas, cudaStream_t stream) {
     using S = AttendShape<F8, D, NT>;
     auto run = [&](auto kern) {
       e = smem_optin_once(kern, S::SMEM(S::MAX_TILES));
-      if (e == cudaSuccess) kern<<<ctas, PA_THREADS, S::SMEM(l.tiles), stream>>>(a);
+      if (e == cudaSuccess) e = launch_early(kern, dim3(ctas), PA_THREADS, S::SMEM(l.tiles), stream, 1, a);
     };
     const bool page8 = a.c.page_size % 8 == 0;
     if (page8 && l.tiles == 1) run(attend_kernel<M, F8, D, NT, true, false>);

@@ -47,6 +47,7 @@ struct PlanArgs {
 
 __global__ void __launch_bounds__(PP_THREADS) plan_pages_kernel(PlanArgs a) {
   extern __shared__ int sm[];
+  wait_for_predecessor();
   __shared__ long long warp_sums[PP_THREADS / 32];
   int* start = sm;                     // [requests + 1] first token
   int* page0 = sm + a.requests + 1;    // [requests] pages taken by the requests before
@@ -149,6 +150,7 @@ extern "C" int cachalot_plan_pages(const int32_t* context_lens, const int32_t* n
     if (e != cudaSuccess) return fail(CACHALOT_ECUDA, "plan_pages: %s", cudaGetErrorString(e));
   }
   const unsigned grid = tokens ? (unsigned)(((long long)tokens + PP_THREADS - 1) / PP_THREADS) : 1u;
-  plan_pages_kernel<<<grid, PP_THREADS, smem, (cudaStream_t)stream>>>(a);
+  const cudaError_t e = launch_early(plan_pages_kernel, dim3(grid), PP_THREADS, smem, (cudaStream_t)stream, 1, a);
+  if (e != cudaSuccess) return fail(CACHALOT_ECUDA, "plan_pages: %s", cudaGetErrorString(e));
   return check_launch("plan_pages");
 }

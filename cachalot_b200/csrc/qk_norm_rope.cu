@@ -194,6 +194,7 @@ template <typename T, int L, int PAIRS>
 __global__ void __launch_bounds__(QR_THREADS) qk_norm_rope_kernel(const RopeArgs a) {
   constexpr int GROUPS = QR_THREADS / L;
   using std::integral_constant;
+  wait_for_predecessor();
   __shared__ __align__(16) float cs[QR_MAX_DIM / 2], sn[QR_MAX_DIM / 2];
   const int token = blockIdx.x, group = threadIdx.x / L, half = a.half;
   const int step = GROUPS * gridDim.y, first = blockIdx.y * GROUPS;  // heads first + group, + step, ..
@@ -345,12 +346,14 @@ extern "C" int cachalot_qk_norm_rope(const void* q, int64_t q_token_stride, int6
   const long long want = (600 + (long long)tokens - 1) / tokens;           // few tokens: their heads over more CTAs
   const dim3 grid((unsigned)tokens, (unsigned)(parts < want ? parts : want));
   cudaStream_t s = (cudaStream_t)stream;
+  cudaError_t e = cudaSuccess;
   auto run = [&](auto type, auto l) {
     using T = decltype(type);
     constexpr int L = decltype(l)::value;
-    if (rotary_dim % 8 == 0 && interleaved) qk_norm_rope_kernel<T, L, PAIRS_ADJACENT><<<grid, QR_THREADS, 0, s>>>(a);
-    else if (rotary_dim % 16 == 0 && !interleaved) qk_norm_rope_kernel<T, L, PAIRS_HALF><<<grid, QR_THREADS, 0, s>>>(a);
-    else qk_norm_rope_kernel<T, L, PAIRS_ANY><<<grid, QR_THREADS, 0, s>>>(a);
+    const auto kern = rotary_dim % 8 == 0 && interleaved     ? qk_norm_rope_kernel<T, L, PAIRS_ADJACENT>
+                      : rotary_dim % 16 == 0 && !interleaved ? qk_norm_rope_kernel<T, L, PAIRS_HALF>
+                                                             : qk_norm_rope_kernel<T, L, PAIRS_ANY>;
+    e = launch_early(kern, grid, QR_THREADS, 0, s, 1, a);
   };
   auto go = [&](auto type) {
     if (lanes == 8) run(type, std::integral_constant<int, 8>{});
@@ -359,5 +362,6 @@ extern "C" int cachalot_qk_norm_rope(const void* q, int64_t q_token_stride, int6
   };
   if (dtype == CACHALOT_F16) go(__half{});
   else go(__nv_bfloat16{});
+  if (e != cudaSuccess) return fail(CACHALOT_ECUDA, "qk_norm_rope: %s", cudaGetErrorString(e));
   return check_launch("qk_norm_rope");
 }

@@ -306,6 +306,7 @@ __global__ void __launch_bounds__(TL_THREADS, TL_CTAS) token_logprobs_kernel(con
   __shared__ uint2 seen[TOP ? TL_SEEN : 1];  // maxima that reached the bar: ordered value, round * threads + thread
   __shared__ int added[3], noted;
   unsigned(*bars)[32] = reinterpret_cast<unsigned(*)[32]>(lists);
+  wait_for_predecessor();
   cg::cluster_group cluster = cg::this_cluster();
   const int ctas = cluster.num_blocks(), rank = cluster.block_rank();
   const int row = blockIdx.x / ctas, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -428,11 +429,11 @@ __global__ void __launch_bounds__(TL_THREADS, TL_CTAS) token_logprobs_kernel(con
 }
 
 template <typename T>
-cudaError_t launch(bool with_top, const cudaLaunchConfig_t& cfg, const void* logits, long long stride, int vocab, const int32_t* tokens, int top,
+cudaError_t launch(bool with_top, int rows, int ctas, cudaStream_t stream, const void* logits, long long stride, int vocab, const int32_t* tokens, int top,
                    float* logprobs, float* entropy, int32_t* top_ids, float* top_logprobs, int* status) {
-  const T* x = static_cast<const T*>(logits);
-  return with_top ? cudaLaunchKernelEx(&cfg, token_logprobs_kernel<T, true>, x, stride, vocab, tokens, top, logprobs, entropy, top_ids, top_logprobs, status)
-                  : cudaLaunchKernelEx(&cfg, token_logprobs_kernel<T, false>, x, stride, vocab, tokens, top, logprobs, entropy, top_ids, top_logprobs, status);
+  const auto kern = with_top ? token_logprobs_kernel<T, true> : token_logprobs_kernel<T, false>;
+  return launch_early(kern, dim3((unsigned)rows * ctas), TL_THREADS, 0, stream, ctas, static_cast<const T*>(logits), stride, vocab, tokens, top, logprobs,
+                      entropy, top_ids, top_logprobs, status);
 }
 
 }  // namespace
@@ -462,13 +463,8 @@ extern "C" int cachalot_token_logprobs(const void* logits, int dtype, int64_t ro
     if (us < least) least = us, ctas = c;
   }
   if ((long long)rows * ctas > 0x7fffffffLL) return fail(CACHALOT_EUNSUPPORTED, "token_logprobs: %d rows", rows);
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim = {(unsigned)ctas, 1, 1};
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)rows * ctas), cfg.blockDim = dim3(TL_THREADS), cfg.stream = (cudaStream_t)stream, cfg.attrs = &attr, cfg.numAttrs = 1;
   const auto go = dtype == CACHALOT_F32 ? launch<float> : dtype == CACHALOT_BF16 ? launch<__nv_bfloat16> : launch<__half>;
-  const cudaError_t e = go(top > 0, cfg, logits, row_stride, vocab, tokens, top, logprobs, entropy, top_ids, top_logprobs, status);
+  const cudaError_t e = go(top > 0, rows, ctas, (cudaStream_t)stream, logits, row_stride, vocab, tokens, top, logprobs, entropy, top_ids, top_logprobs, status);
   if (e != cudaSuccess) return fail(CACHALOT_ECUDA, "token_logprobs: %s", cudaGetErrorString(e));
   return check_launch("token_logprobs");
 }
