@@ -173,8 +173,27 @@ inline cudaError_t smem_optin_once(K kern, int bytes) {
   return e;
 }
 
+// Streaming loads of memory that the kernel before may have written (no .nc).
+__device__ __forceinline__ uint4 ld_once_u4(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint2 ld_once_u2(const void* p) {
+  uint2 v;
+  asm volatile("ld.global.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint32_t ld_once_u32(const void* p) {
+  uint32_t v;
+  asm volatile("ld.global.L1::no_allocate.u32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
+  return v;
+}
+
 // Launches of kernels whose first statement is wait_for_predecessor(): the set-up of such a launch runs under the end of the
-// kernel before it in the stream (programmatic dependent launch) instead of after it.
+// kernel before it in the stream (programmatic dependent launch) instead of after it.  What such a kernel reads may be
+// written while it already exists, so it is not read-only in the sense of ld.global.nc, __ldg or const __restrict__: those
+// may be moved in front of the wait.
 __device__ __forceinline__ void wait_for_predecessor() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 template <typename... Params, typename... Args>
 inline cudaError_t launch_early(void (*kern)(Params...), dim3 grid, int threads, size_t smem, cudaStream_t stream, int cluster, Args&&... args) {

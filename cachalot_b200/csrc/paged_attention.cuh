@@ -19,7 +19,7 @@
 // Work is cut on the device, where the lengths are: the steps (a tile for each warp, of one request and key-value head) of the whole
 // batch are laid on a line and every CTA takes an equal run of it, so a batch of very different lengths is balanced
 // and one long request fills the GPU.  A unit (request, head) also occupies what it costs to begin one (query, first
-// page, empty pipeline, merge: as long as about 48 KB of keys and values; without that, CTAs with many short requests
+// page, empty pipeline, merge: as long as 48 KB of keys and values, 72 KB of E4M3; without that, CTAs with many short requests
 // took twice the average and 32 requests of 1 to 8192 tokens 79 us), and a cut that falls near a unit's end is moved there.
 // A CTA merges its four warps in shared memory; a unit that lies in one CTA is finished there, a unit that crosses
 // CTAs leaves (m, l, O) of each part for the join kernel.
@@ -111,13 +111,13 @@ __device__ __forceinline__ void load_words(uint32_t (&r)[W], const uint8_t* p) {
   for (int c = 0; c < W * 4 / B; ++c) {
     const uint8_t* at = p + c * STRIDE;
     if constexpr (B == 16) {
-      const uint4 v = KEEP ? __ldg(reinterpret_cast<const uint4*>(at)) : ld_stream_u4(at);
+      const uint4 v = KEEP ? *reinterpret_cast<const uint4*>(at) : ld_once_u4(at);
       r[c * 4] = v.x, r[c * 4 + 1] = v.y, r[c * 4 + 2] = v.z, r[c * 4 + 3] = v.w;
     } else if constexpr (B == 8) {
-      const uint2 v = KEEP ? __ldg(reinterpret_cast<const uint2*>(at)) : ld_stream_u2(at);
+      const uint2 v = KEEP ? *reinterpret_cast<const uint2*>(at) : ld_once_u2(at);
       r[c * 2] = v.x, r[c * 2 + 1] = v.y;
     } else {
-      r[c] = KEEP ? __ldg(reinterpret_cast<const uint32_t*>(at)) : ld_stream_u32(at);
+      r[c] = KEEP ? *reinterpret_cast<const uint32_t*>(at) : ld_once_u32(at);
     }
   }
 }
@@ -151,7 +151,7 @@ struct Span {  // what is visible of a request
 template <typename S>
 __device__ __forceinline__ Span span_of(const AttendArgs& a, int r) {
   Span s;
-  s.len = min(max(__ldg(a.lens + r), 0), a.room);
+  s.len = min(max(a.lens[r], 0), a.room);
   s.lo = a.window > 0 ? max(0, s.len - a.window) : 0;
   s.first_tile = s.lo / S::TILE;
   s.steps = s.len > 0 ? (s.len - s.first_tile * S::TILE + S::STEP - 1) / S::STEP : 0;
@@ -198,7 +198,7 @@ __global__ void __launch_bounds__(PA_THREADS, AttendShape<F8, D, NT>::CTAS) atte
   // ---- which part of the line is this CTA's ----
   auto cost_of = [&](int r) {
     if (r >= a.requests) return 0LL;
-    const int n = __ldg(a.lens + r);
+    const int n = a.lens[r];
     if (n < 0 || n > a.room) flags |= CACHALOT_STATUS_LENGTH;
     const int steps = span_of<S>(a, r).steps;
     return steps ? (long long)(steps + a.unit_cost) * per_request : 0LL;
@@ -295,7 +295,7 @@ __global__ void __launch_bounds__(PA_THREADS, AttendShape<F8, D, NT>::CTAS) atte
     // page of a token, -1 where the table names none of the cache's
     auto page_of = [&](int token, int index) {
       if (token >= sp.len) return -1;
-      const int p = __ldg(pages + index);
+      const int p = pages[index];
       if ((unsigned)p < (unsigned)a.c.n_pages) return p;
       flags |= CACHALOT_STATUS_SLOT_RANGE;
       return -1;

@@ -172,7 +172,7 @@ struct Vec {
   // elements [from, from + PER) of a row, -inf outside [0, vocab)
   __device__ __forceinline__ void load(const T* row, int from, int vocab) {
     if (from >= 0 && from + PER <= vocab) {
-      raw = ld_stream_u4(row + from);
+      raw = ld_once_u4(row + from);
       return;
     }
     uint32_t w[4] = {0, 0, 0, 0};
@@ -294,10 +294,10 @@ __device__ __noinline__ int select_carefully(const Share<T> sh, int top, Key* li
 }
 
 template <typename T, bool TOP>
-__global__ void __launch_bounds__(TL_THREADS, TL_CTAS) token_logprobs_kernel(const T* __restrict__ logits, long long stride, int vocab,
-                                                                             const int32_t* __restrict__ tokens, int top, float* __restrict__ logprobs,
-                                                                             float* __restrict__ entropy, int32_t* __restrict__ top_ids,
-                                                                             float* __restrict__ top_logprobs, int* status) {
+__global__ void __launch_bounds__(TL_THREADS, TL_CTAS) token_logprobs_kernel(const T* logits, long long stride, int vocab,
+                                                                             const int32_t* tokens, int top, float* logprobs,
+                                                                             float* entropy, int32_t* top_ids,
+                                                                             float* top_logprobs, int* status) {
   using V = Vec<T>;
   constexpr int PER = V::PER;
   __shared__ Sums parts[TL_WARPS];
