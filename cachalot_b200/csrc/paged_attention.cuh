@@ -19,7 +19,7 @@
 // Work is cut on the device, where the lengths are: the steps (a tile for each warp, of one request and key-value head) of the whole
 // batch are laid on a line and every CTA takes an equal run of it, so a batch of very different lengths is balanced
 // and one long request fills the GPU.  A unit (request, head) also occupies what it costs to begin one (query, first
-// page, empty pipeline, merge: as long as 48 KB of keys and values, 72 KB of E4M3; without that, CTAs with many short requests
+// page, empty pipeline, merge: as long as 48 KB of keys and values, or 384 tokens of E4M3; without that, CTAs with many short requests
 // took twice the average and 32 requests of 1 to 8192 tokens 79 us), and a cut that falls near a unit's end is moved there.
 // A CTA merges its four warps in shared memory; a unit that lies in one CTA is finished there, a unit that crosses
 // CTAs leaves (m, l, O) of each part for the join kernel.
@@ -130,7 +130,9 @@ struct AttendShape {
   static constexpr int KB = KBYTES % 16 == 0 ? 16 : 8;
   static constexpr int VB = VBYTES % 16 == 0 ? 16 : VBYTES % 8 == 0 ? 8 : 4;
   static constexpr int KW = KBYTES / 4, VW = VBYTES / 4;
-  static constexpr int U = D * ES <= 128 ? 2 : 1;       // MMA tiles of 16 tokens that a warp works on at a time
+  // MMA tiles of 16 tokens that a warp works on at a time.  (E4M3, 128 elements, two column tiles: 148 us with one and three
+  // CTAs per SM, 168 us with two and two, batch of 64 with 16 heads to a key-value head.)
+  static constexpr int U = D * ES <= 128 && !(F8 && D * NT > 192) ? 2 : 1;
   static constexpr int TILE = 16 * U, STEP = PA_WARPS * TILE;
   static constexpr int KSTEPS = D / 16;                 // MMAs over the head's elements = MMA row tiles of O^T
   static constexpr int TILE_HEADS = 8 * NT;
@@ -142,7 +144,7 @@ struct AttendShape {
   static constexpr int SMEM(int tiles) { return Q_BYTES(tiles) + PA_WARPS * TILE_HEADS * (O_PITCH * 4 + 8) + 4 * TILE_HEADS * 4; }
   static constexpr int MAX_TILES = 4;
   // CTAs per SM that the registers are cut for
-  static constexpr int CTAS = D * NT <= 64 ? 4 : D * NT <= 128 ? 3 : 2;
+  static constexpr int CTAS = D * NT <= 64 ? 4 : D * NT <= 128 || (F8 && D == 128) ? 3 : 2;
 };
 
 struct Span {  // what is visible of a request
