@@ -19,7 +19,7 @@
 // Work is cut on the device, where the lengths are: the steps (a tile for each warp, of one request and key-value head) of the whole
 // batch are laid on a line and every CTA takes an equal run of it, so a batch of very different lengths is balanced
 // and one long request fills the GPU.  A unit (request, head) also occupies what it costs to begin one (query, first
-// page, empty pipeline, merge: as long as 48 KB of keys and values, or 384 tokens of E4M3; without that, CTAs with many short requests
+// page, empty pipeline, merge: as long as 48 or 96 KB of keys and values, or 384 tokens of E4M3; without that, CTAs with many short requests
 // took twice the average and 32 requests of 1 to 8192 tokens 79 us), and a cut that falls near a unit's end is moved there.
 // A CTA merges its four warps in shared memory; a unit that lies in one CTA is finished there, a unit that crosses
 // CTAs leaves (m, l, O) of each part for the join kernel.
