@@ -144,7 +144,7 @@ struct AttendShape {
   static constexpr int SMEM(int tiles) { return Q_BYTES(tiles) + PA_WARPS * TILE_HEADS * (O_PITCH * 4 + 8) + 4 * TILE_HEADS * 4; }
   static constexpr int MAX_TILES = 4;
   // CTAs per SM that the registers are cut for
-  static constexpr int CTAS = D * NT <= 64 ? 4 : D * NT <= 128 || (F8 && D == 128) ? 3 : 2;
+  static constexpr int CTAS = D * NT <= 64 ? 4 : D * NT <= 128 || (F8 && D * NT == 256) ? 3 : 2;
 };
 
 struct Span {  // what is visible of a request
@@ -653,13 +653,16 @@ AttendLaunch attend_shape(int group) {
   l.ctas_per_sm = AttendShape<F8, D, NT>::CTAS, l.step = AttendShape<F8, D, NT>::STEP;
   return l;
 }
-// Up to 8 query heads per key-value head take one MMA column tile per warp, more take two where the registers hold them.
+// Column tiles of 8 query heads per warp: as few warps as possible read the same keys, up to three tiles where the registers hold
+// their sums (heads of up to 128).  24 heads to a key-value head: 121 us with three tiles, 178 with two tiles in two warps.
 template <bool F8, typename Fn>
 bool attend_dispatch(int dim, int group, Fn&& fn) {
   auto go = [&](auto d, auto nt) { fn(d, nt, attend_shape<F8, decltype(d)::value, decltype(nt)::value>(group)); };
   using std::integral_constant;
   auto nt = [&](auto d) {
     if constexpr (decltype(d)::value <= 128) {
+      const int two = (group + 15) / 16, three = (group + 23) / 24;  // warps
+      if (group > 16 && (three == 1 || (two > 2 && three == 2))) return go(d, integral_constant<int, 3>{});
       if (group > 8) return go(d, integral_constant<int, 2>{});
     }
     go(d, integral_constant<int, 1>{});
