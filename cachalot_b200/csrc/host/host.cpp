@@ -16,6 +16,7 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <cmath>
 #include <initializer_list>
 
 #include "../../../include/cachalot_b200.h"
@@ -544,7 +545,7 @@ PyObject* qk_norm_rope(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   END_HANDLE_TH_ERRORS
 }
 
-// (q, k_cache, v_cache, block_table, lens, scale, window, softcap, k_scale | None, v_scale | None, out dtype, want_lse, status | None)
+// (q, k_cache, v_cache, block_table, lens, scale | None, window, softcap, k_scale | None, v_scale | None, out dtype | None, want_lse, status | None)
 //  -> out, or (out, lse)
 PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   HANDLE_TH_ERRORS
@@ -553,13 +554,15 @@ PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   const at::Tensor *q = tensor_of(a[0]), *table = tensor_of(a[3]), *lens = tensor_of(a[4]);
   PLAIN_OR_NONE(q && q->is_cuda());
   const int dev = current_device();
-  const double scale = p.f(5), softcap = p.f(7);
-  const int window = (int)p.i(6), odt = (int)p.i(10), want = PyObject_IsTrue(a[11]);
   const ScalarType dt = q->scalar_type();
+  const double softcap = p.f(7);
+  const int window = (int)p.i(6), odt = a[10] == Py_None ? element_code(dt) : (int)p.i(10), want = PyObject_IsTrue(a[11]);
   PLAIN_OR_NONE(!p.bad && want >= 0 && (dt == ScalarType::Half || dt == ScalarType::BFloat16) && q->get_device() == dev && q->dim() == 3 && q->stride(2) == 1);
   PLAIN_OR_NONE(q->stride(0) % 2 == 0 && q->stride(1) % 2 == 0 && reinterpret_cast<uintptr_t>(q->data_ptr()) % 4 == 0);
   const int64_t requests = q->size(0), heads = q->size(1), dim = q->size(2);
   PLAIN_OR_NONE(requests > 0 && requests < (1LL << 30) && heads > 0 && heads < (1 << 20) && odt >= CACHALOT_F16 && odt <= CACHALOT_F32 && window >= 0);
+  const double scale = a[5] == Py_None ? 1.0 / std::sqrt((double)dim) : p.f(5);
+  PLAIN_OR_NONE(!p.bad);
   cachalot_paged_kv cache;
   PLAIN_OR_NONE(cache_from(tensor_of(a[1]), tensor_of(a[2]), a[8], a[9], dev, &cache) && cache.head_dim == dim && heads % cache.kv_heads == 0);
   PLAIN_OR_NONE(table_of(table, requests, dev) && plain_ints(lens, requests, dev));

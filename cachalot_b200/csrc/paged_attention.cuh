@@ -130,9 +130,9 @@ struct AttendShape {
   static constexpr int KB = KBYTES % 16 == 0 ? 16 : 8;
   static constexpr int VB = VBYTES % 16 == 0 ? 16 : VBYTES % 8 == 0 ? 8 : 4;
   static constexpr int KW = KBYTES / 4, VW = VBYTES / 4;
-  // MMA tiles of 16 tokens that a warp works on at a time.  (E4M3, 128 elements, two column tiles: 148 us with one and three
-  // CTAs per SM, 168 us with two and two, batch of 64 with 16 heads to a key-value head.)
-  static constexpr int U = D * ES <= 128 && !(F8 && D * NT > 192) ? 2 : 1;
+  // MMA tiles of 16 tokens that a warp works on at a time.  (E4M3 with several column tiles: one tile and three CTAs per SM 141 us,
+  // two and two 168 us, batch of 64 with 16 heads of 128 to a key-value head.)
+  static constexpr int U = D * ES <= 128 && !(F8 && NT > 1 && D > 64) ? 2 : 1;
   static constexpr int TILE = 16 * U, STEP = PA_WARPS * TILE;
   static constexpr int KSTEPS = D / 16;                 // MMAs over the head's elements = MMA row tiles of O^T
   static constexpr int TILE_HEADS = 8 * NT;
@@ -144,7 +144,7 @@ struct AttendShape {
   static constexpr int SMEM(int tiles) { return Q_BYTES(tiles) + PA_WARPS * TILE_HEADS * (O_PITCH * 4 + 8) + 4 * TILE_HEADS * 4; }
   static constexpr int MAX_TILES = 4;
   // CTAs per SM that the registers are cut for
-  static constexpr int CTAS = D * NT <= 64 ? 4 : D * NT <= 128 || (F8 && D * NT == 256) ? 3 : 2;
+  static constexpr int CTAS = D * NT <= 64 ? 4 : D * NT <= 128 || (F8 && NT > 1 && D * NT <= 256) ? 3 : 2;
 };
 
 struct Span {  // what is visible of a request

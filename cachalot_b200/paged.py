@@ -235,10 +235,8 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     float32 [requests, heads] log sum exp of the scores.  A request of length 0 gives zeros and -inf; tokens whose table
     entry is no page of the cache are hidden, lengths past the table cut (bits in `status`).  The lengths are read on the
     device: nothing waits for them, and a captured call replays with new ones."""
-    if scale is None:
-        scale = q.shape[-1] ** -0.5
     r = _host.paged_attention(q, k_cache, v_cache, block_table, lens, scale, window, softcap, k_scale, v_scale,
-                              _DT.get(q.dtype if out_dtype is None else out_dtype, -1), want_lse, status)
+                              None if out_dtype is None else _DT.get(out_dtype, -1), want_lse, status)
     if r is not None:
         return r
     dev = _same_device(q, k_cache, v_cache, block_table, lens, k_scale, v_scale, status)
@@ -250,6 +248,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     if out_dtype not in (torch.float16, torch.bfloat16, torch.float32):
         raise ValueError(f"out_dtype must be float16, bfloat16 or float32, got {out_dtype}")
     requests, heads, dim = q.shape
+    scale = dim ** -0.5 if scale is None else scale
     desc = _cache(k_cache, v_cache, k_scale, v_scale)
     if desc.head_dim != dim:
         raise ValueError(f"q has heads of {dim}, the cache of {desc.head_dim}")
