@@ -96,12 +96,13 @@ def test_paged_attention_refusals():
     lib, p = _lib.lib, C.c_void_p(base)
 
     def call(qs=256, dtype=_lib.BF16, requests=1, heads=4, kv=2, dim=64, cdt=_lib.BF16, table=p, stride=4, width=4, lens=p, window=0, cap=0.0, ws=p, room=1 << 40,
-             odt=_lib.BF16, q=p):
+             odt=_lib.BF16, q=p, far=0):
         d = _lib.PagedKV()
         d.k = d.v = base
         d.k_page_stride = d.v_page_stride = 16 * kv * dim
         d.k_head_stride = d.v_head_stride = 16 * dim
         d.k_token_stride = d.v_token_stride = dim
+        d.v_page_stride += far
         d.n_pages, d.page_size, d.kv_heads, d.head_dim, d.dtype = 2, 16, kv, dim, cdt
         return lib.cachalot_paged_attention(q, qs, dim, dtype, requests, heads, C.byref(d), table, stride, width, lens, 0.125, window, cap, ws, room, p, odt, None,
                                             None, None)
@@ -109,7 +110,7 @@ def test_paged_attention_refusals():
     for kw, rc, word in ((dict(requests=-1), _lib.EINVAL, "shape"), (dict(dtype=_lib.F32), _lib.EINVAL, "queries"), (dict(odt=_lib.E4M3), _lib.EINVAL, "output"),
                          (dict(heads=5), _lib.EINVAL, "heads"), (dict(cdt=_lib.F16), _lib.EINVAL, "differ"), (dict(window=-1), _lib.EINVAL, "window"),
                          (dict(cap=-1.0), _lib.EINVAL, "softcap"), (dict(cap=float("nan")), _lib.EINVAL, "softcap"), (dict(dim=80), _lib.EUNSUPPORTED, "80"),
-                         (dict(table=None), _lib.EINVAL, "null"), (dict(lens=None), _lib.EINVAL, "null"), (dict(ws=None), _lib.EINVAL, "null"),
+                         (dict(far=2 ** 31), _lib.EUNSUPPORTED, "apart"), (dict(table=None), _lib.EINVAL, "null"), (dict(lens=None), _lib.EINVAL, "null"), (dict(ws=None), _lib.EINVAL, "null"),
                          (dict(q=C.c_void_p(base + 2)), _lib.EALIGN, "4-byte"), (dict(qs=255), _lib.EALIGN, "4-byte"),
                          (dict(requests=2, stride=3), _lib.EINVAL, "overlap"), (dict(ws=C.c_void_p(base + 16)), _lib.EALIGN, "256"),
                          (dict(room=1000), _lib.ESCRATCH, "workspace")):
