@@ -377,7 +377,7 @@ typedef struct {
   int32_t dtype;
 } cachalot_paged_kv;
 
-/* No counterpart in the reference (one request, contiguous caches).  Places a step's new tokens: request r holds
+/* No counterpart in the reference.  Places a step's new tokens: request r holds
  * context_lens[r] tokens and gets new_lens[r] more (both i32 [requests]).  The new tokens are numbered request by request,
  * those past `tokens` are left out (CACHALOT_STATUS_LENGTH) as if they had not been asked for; pages that a request needs
  * beyond the ceil(context / page_size) it has come from the end of free_pages[0 .. *free_count), request by request and
@@ -392,15 +392,15 @@ CACHALOT_API int cachalot_plan_pages(const int32_t* context_lens, const int32_t*
                         int page_size, int tokens, int32_t* starts, int32_t* request_of, int32_t* positions, int32_t* slots,
                         int32_t* lens, int32_t* free_count_out, int* status, cachalot_stream_t stream);
 
-/* Replaces model/norm_rope_mlx.py and the rope_1d kernels of model/decode_fused_metal.py:43 (one token, then a cache
- * append): for every new token, RMS norm of each query and key head (q_weight, k_weight [head_dim] in `dtype` or f32; NULL:
+/* Replaces model/norm_rope_mlx.py and the rope_1d kernels of model/decode_fused_metal.py:43, and the cache write after them:
+ * for every new token, RMS norm of each query and key head (q_weight, k_weight [head_dim] in `dtype` or f32; NULL:
  * no norm), rotation of the first rotary_dim elements by the token's position, rounding, and the write of keys and values
  * to slots[token] of the cache.  q [tokens, heads, head_dim], k and v [tokens, kv_heads, head_dim] in `dtype` (CACHALOT_F16
  * or CACHALOT_BF16), rows 16-byte aligned, strides in elements; inv_freq f64 [rotary_dim/2], radians per position;
  * interleaved: pairs (2i, 2i+1), else (i, i + rotary_dim/2); magnitude: factor of the rotated elements (1; more where
  * long-context scaling asks for it).  q_out [tokens, heads, head_dim] and, if not NULL, k_out [tokens, kv_heads, head_dim]
  * are contiguous and may not overlap an input.  cache NULL: v and slots are not read.  A negative slot (padding) is not stored, one past the
- * cache neither (CACHALOT_STATUS_SLOT_RANGE); two tokens of a call must not share one.  E4M3 caches get value / scale,
+ * cache neither (CACHALOT_STATUS_SLOT_RANGE); two tokens of a call must not share one.  E4M3 caches get value * (1 / scale),
  * saturated at +-448.  head_dim a multiple of 8 up to 256. */
 CACHALOT_API int cachalot_qk_norm_rope(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k,
                           int64_t k_token_stride, int64_t k_head_stride, const void* v, int64_t v_token_stride,
@@ -410,8 +410,8 @@ CACHALOT_API int cachalot_qk_norm_rope(const void* q, int64_t q_token_stride, in
                           const cachalot_paged_kv* cache /* host, or NULL */, const int32_t* slots, int* status,
                           cachalot_stream_t stream);
 
-/* Replaces minimax/gqa_decode.py:180-187 (grouped-query attention of one decode token over a contiguous cache): one new
- * token per request against the tokens of its pages,
+/* Replaces minimax/gqa_decode.py:180-187 (grouped-query attention of a decode token): one new token per request against the
+ * tokens of its pages,
  *   s_j = scale * q . k_j  (softcap > 0: softcap * tanh(s_j / softcap)),  out = softmax(s) V,  lse = log sum_j exp(s_j)
  * over j < lens[r], with window > 0 only the last `window` of them (the new token is one of them and already in the cache).
  * q [requests, heads, head_dim] F16 or BF16 (strides in elements, 4-byte aligned), out [requests, heads, head_dim]
@@ -430,7 +430,7 @@ CACHALOT_API int cachalot_paged_attention(const void* q, int64_t q_row_stride, i
                              void* workspace, size_t workspace_bytes, void* out, int out_dtype, float* lse, int* status,
                              cachalot_stream_t stream);
 
-/* No counterpart in the reference (its sampling reads the whole logits on the host).  For every row of logits
+/* No counterpart among the reference's operators.  For every row of logits
  * [rows, vocab] (dtype F32, BF16 or F16, rows row_stride elements apart): logprobs[r] = log softmax of tokens[r] (0 for a
  * negative id, and for one past the vocabulary: CACHALOT_STATUS_ID_RANGE), entropy[r] = -sum p log p (f32 [rows]), and the
  * `top` <= 32 most likely tokens, most likely first, ties to the lower index: top_ids i32, top_logprobs f32 [rows, top].
