@@ -10,7 +10,7 @@
 // heads: an output element is r (x A + p B), r the head's 1 / rms, p the partner element, A = m w cos, B = -/+ m w_p sin
 // in registers.  Interleaved partners are in the same lane; those of the half layout are a second 16-byte load that hits
 // L1 (fp32 values handed through shared memory instead: 365 instead of about 100 instructions per two heads, 124 us for
-// 4096 tokens of 64 + 16 + 16 heads of 128).  Pairs that straddle 16-byte pieces are fetched element by element.
+// 4096 tokens of 64 + 16 + 16 heads of 128; now 40 us).  Halves that are no whole 16-byte pieces go through shared memory as they are.
 // Angles are computed once per token: position * frequency in 64 bits, reduced to a fraction of a turn there (a float
 // product is off by 0.06 rad at position 10^6), then sincospif.
 #include <cuda_fp8.h>
@@ -38,8 +38,9 @@ struct RopeArgs {
   float eps, magnitude;
   const int32_t* positions;
   const double* inv_freq;
-  int half, interleaved;
-  int heads, kv_heads, dim;
+  int half;
+  int tokens, heads, kv_heads, dim;
+  int crew_log2;  // groups of a CTA on one token
   float inv_dim;
   void *q_out, *k_out;
   PagedView cache;  // cache.k null: none
@@ -108,53 +109,59 @@ __device__ __forceinline__ f32x2 swapped(f32x2 p) {
   return pair(v.y, v.x);
 }
 
-enum { PAIRS_ADJACENT, PAIRS_HALF, PAIRS_ANY };  // (2i, 2i+1) and (i, i+r/2) in whole 16-byte pieces; element by element
+enum { PAIRS_ADJACENT, PAIRS_HALF, PAIRS_ANY };  // (2i, 2i+1); (i, i+r/2) in whole 16-byte pieces; (i, i+r/2) in any place
 
 template <typename T, int L, int PAIRS>
 struct Lane {  // what a lane does to its 8 elements of a query or key head
   f32x2 a[4], b[4];
-  bool rotated;  // any of them
-  int partner;   // first element of the piece the partners are in
-  int half, at, adjacent;
+  int turns;     // the rotated ones: a bit per pair (adjacent) or per element
+  int partner;   // PAIRS_HALF: first element of the piece the partners are in
+  int half, at;
 
+  __device__ __forceinline__ int mate(int i) const { return i < half ? i + half : i - half; }
+  __device__ __forceinline__ void place(int first, int h) {
+    at = first, half = h, turns = 0;
+#pragma unroll
+    for (int e = 0; e < (PAIRS == PAIRS_ADJACENT ? 4 : 8); ++e) turns |= (PAIRS == PAIRS_ADJACENT ? at / 2 + e < half : at + e < 2 * half) << e;
+    partner = PAIRS == PAIRS_HALF && turns ? mate(at) : at;
+  }
   __device__ __forceinline__ void set(const void* w, int f32, const float* cs, const float* sn) {
     weights8<T>(w, f32, at, a);
 #pragma unroll
     for (int i = 0; i < 4; ++i) b[i] = pair(0.f, 0.f);
+    if (!turns) return;
     if constexpr (PAIRS == PAIRS_ANY) {
       float x[8], z[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const int i = at + e, k = adjacent ? i >> 1 : i < half ? i : i - half, j = mate(i);
-        const bool turns = i < 2 * half;
-        x[e] = weight<T>(w, f32, i) * (turns ? cs[k] : 1.f);
-        z[e] = turns ? weight<T>(w, f32, j) * (j > i ? -sn[k] : sn[k]) : 0.f;
+        const int i = at + e, k = i < half ? i : i - half;
+        const bool on = turns >> e & 1;
+        x[e] = weight<T>(w, f32, i) * (on ? cs[k] : 1.f);
+        z[e] = on ? weight<T>(w, f32, mate(i)) * (i < half ? -sn[k] : sn[k]) : 0.f;
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i) a[i] = pair(x[2 * i], x[2 * i + 1]), b[i] = pair(z[2 * i], z[2 * i + 1]);
-    } else if (rotated) {
-      if constexpr (PAIRS == PAIRS_ADJACENT) {
+    } else if constexpr (PAIRS == PAIRS_ADJACENT) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float c = cs[at / 2 + i], s = sn[at / 2 + i];
-          b[i] = mul2(swapped(a[i]), pair(-s, s)), a[i] = mul2(a[i], pair(c, c));
-        }
-      } else {
-        f32x2 other[4];
-        weights8<T>(w, f32, partner, other);
-        const int k = at < half ? at : partner;
-        const float sign = at < half ? -1.f : 1.f;
+      for (int i = 0; i < 4; ++i) {
+        if (!(turns >> i & 1)) continue;
+        const float c = cs[at / 2 + i], s = sn[at / 2 + i];
+        b[i] = mul2(swapped(a[i]), pair(-s, s)), a[i] = mul2(a[i], pair(c, c));
+      }
+    } else {
+      f32x2 other[4];
+      weights8<T>(w, f32, partner, other);
+      const int k = at < half ? at : partner;
+      const float sign = at < half ? -1.f : 1.f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float2 c = *reinterpret_cast<const float2*>(cs + k + 2 * i), s = *reinterpret_cast<const float2*>(sn + k + 2 * i);
-          a[i] = mul2(a[i], pair(c.x, c.y)), b[i] = mul2(other[i], pair(sign * s.x, sign * s.y));
-        }
+      for (int i = 0; i < 4; ++i) {
+        const float2 c = *reinterpret_cast<const float2*>(cs + k + 2 * i), s = *reinterpret_cast<const float2*>(sn + k + 2 * i);
+        a[i] = mul2(a[i], pair(c.x, c.y)), b[i] = mul2(other[i], pair(sign * s.x, sign * s.y));
       }
     }
   }
-  __device__ __forceinline__ int mate(int i) const { return adjacent ? i ^ 1 : i < half ? i + half : i - half; }
 
-  // y <- (y A + p B) / rms (or without the norm), `times` a factor on top; `piece`: the partner's, `row`: the head in memory
+  // y <- (y A + p B) / rms (or without the norm), `times` a factor on top; `piece`: the partner's, `row`: the head in shared memory
   __device__ __forceinline__ void apply(f32x2 (&y)[4], const uint4& piece, const T* row, bool normed, float eps, float inv_dim, float times) const {
     float r = times;
     if (normed) {
@@ -167,117 +174,139 @@ struct Lane {  // what a lane does to its 8 elements of a query or key head
       r *= rsqrtf(fmaf(ss, inv_dim, eps));
     }
     const f32x2 r2 = pair(r, r);
-    if (PAIRS != PAIRS_ANY && !rotated) {
+    if (!turns) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) y[i] = mul2(y[i], mul2(a[i], r2));
       return;
     }
+    // the partner of an element that stays is 0, not itself: 0 * inf is not 0
     f32x2 p[4];
     if constexpr (PAIRS == PAIRS_ADJACENT) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) p[i] = swapped(y[i]);
+      for (int i = 0; i < 4; ++i) p[i] = turns >> i & 1 ? swapped(y[i]) : 0;
     } else if constexpr (PAIRS == PAIRS_HALF) {
       widen8<T>(piece, p);
     } else {
-      float v[8];
+      if (half & 1) {
+        float v[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = row && at + e < 2 * half ? weight<T>(row, 0, mate(at + e)) : 0.f;
+        for (int e = 0; e < 8; ++e) v[e] = turns >> e & 1 ? weight<T>(row, 0, mate(at + e)) : 0.f;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) p[i] = pair(v[2 * i], v[2 * i + 1]);
+        for (int i = 0; i < 4; ++i) p[i] = pair(v[2 * i], v[2 * i + 1]);
+      } else {  // two neighbours have neighbours for partners
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = turns >> 2 * i & 1 ? *reinterpret_cast<const uint32_t*>(row + mate(at + 2 * i)) : 0u;
+        widen8<T>(make_uint4(w[0], w[1], w[2], w[3]), p);
+      }
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) y[i] = mul2(r2, fma2(p[i], b[i], mul2(y[i], a[i])));
   }
 };
 
-template <typename T, int L, int PAIRS>
+template <typename T, int L, int PAIRS, bool SEVERAL>  // SEVERAL: tokens of a CTA
 __global__ void __launch_bounds__(QR_THREADS) qk_norm_rope_kernel(const RopeArgs a) {
   constexpr int GROUPS = QR_THREADS / L;
   using std::integral_constant;
   wait_for_predecessor();
-  __shared__ __align__(16) float cs[QR_MAX_DIM / 2], sn[QR_MAX_DIM / 2];
-  const int token = blockIdx.x, group = threadIdx.x / L, half = a.half;
-  const int step = GROUPS * gridDim.y, first = blockIdx.y * GROUPS;  // heads first + group, + step, ..
+  __shared__ __align__(16) float cs[SEVERAL ? GROUPS : 1][L * 4], sn[SEVERAL ? GROUPS : 1][L * 4];  // per token of the CTA
+  __shared__ uint4 staged[PAIRS == PAIRS_ANY ? QR_BATCH : 1][PAIRS == PAIRS_ANY ? QR_THREADS : 1];
+  // a CTA's groups: `crew` of them on each of its tokens, which take the token's heads in turn
+  const int group = threadIdx.x / L, crew = SEVERAL ? 1 << a.crew_log2 : GROUPS, tokens = SEVERAL ? GROUPS >> a.crew_log2 : 1;
+  const int member = SEVERAL ? group & (crew - 1) : group, mine = SEVERAL ? group >> a.crew_log2 : 0, half = a.half;
+  const int token = blockIdx.x * tokens + mine;
+  const int step = crew * gridDim.y, first = blockIdx.y * crew;  // heads first + member, + step, ..
+  const bool exists = !SEVERAL || token < a.tokens, live = threadIdx.x % L * 8 < a.dim && exists;
+  const int at = threadIdx.x % L * 8 < a.dim ? threadIdx.x % L * 8 : 0;  // lanes past the head count as zeros
   Lane<T, L, PAIRS> ln;
-  ln.at = threadIdx.x % L * 8, ln.half = half, ln.adjacent = a.interleaved;
-  const bool live = ln.at < a.dim;
-  const int at = live ? ln.at : 0;  // lanes past the head count as zeros
-  ln.at = at, ln.rotated = at < 2 * half;
-  ln.partner = PAIRS != PAIRS_HALF || !ln.rotated ? at : at < half ? at + half : at - half;
-  for (int i = threadIdx.x; i < half; i += QR_THREADS) {
-    const double turns = (double)a.positions[token] * a.inv_freq[i] * 0.15915494309189533577;  // 1 / (2 pi)
+  ln.place(at, half);
+  for (int i = threadIdx.x; i < tokens * half; i += QR_THREADS) {
+    const int t = SEVERAL ? i / half : 0, f = i - t * half;
+    if (SEVERAL && blockIdx.x * tokens + t >= a.tokens) break;
+    const double turns = (double)a.positions[blockIdx.x * tokens + t] * a.inv_freq[f] * 0.15915494309189533577;  // 1 / (2 pi)
     float s, c;
     sincospif(2.0f * (float)(turns - rint(turns)), &s, &c);
-    cs[i] = c * a.magnitude, sn[i] = s * a.magnitude;
+    cs[t][f] = c * a.magnitude, sn[t][f] = s * a.magnitude;
   }
   __syncthreads();
   const uint4 zero = make_uint4(0, 0, 0, 0);
-  // heads h0 + group, + step, .. (N of them); CHECK: the last ones may not be there
-  auto loads = [&](auto n, auto check, const T* x, long long head, int heads, int h0, int from, uint4* v) {
-    const T* p = x + (long long)(h0 + group) * head + from;
+  // heads h0 + member, + step, .. (N of them); CHECK: the last ones may not be there
+  auto loads = [&](auto n, auto check, const T* x, long long head, int heads, int h0, int from, bool wanted, uint4* v) {
+    const T* p = x + (long long)(h0 + member) * head + from;
 #pragma unroll
     for (int i = 0; i < decltype(n)::value; ++i, p += step * head)
-      v[i] = live && (!decltype(check)::value || h0 + group + i * step < heads) ? *reinterpret_cast<const uint4*>(p) : zero;
+      v[i] = wanted && (!decltype(check)::value || h0 + member + i * step < heads) ? *reinterpret_cast<const uint4*>(p) : zero;
   };
   // as many whole batches as there are, then one by one
   auto over = [&](int heads, auto batch, auto&& work) {
     constexpr int N = decltype(batch)::value;
     int h = first;
-    for (; h + (N - 1) * step + GROUPS <= heads; h += N * step) work(batch, integral_constant<bool, false>{}, h);
+    for (; h + (N - 1) * step + crew <= heads; h += N * step) work(batch, integral_constant<bool, false>{}, h);
     for (; h < heads; h += step) work(integral_constant<int, 1>{}, integral_constant<bool, true>{}, h);
   };
+  // PAIRS_ANY: the heads of a batch as they are, for the lanes that have their partners
+  auto stage = [&](auto n, const uint4* v) {
+    if constexpr (PAIRS == PAIRS_ANY) {
+      __syncwarp();
+#pragma unroll
+      for (int i = 0; i < decltype(n)::value; ++i) staged[i][threadIdx.x] = v[i];
+      __syncwarp();
+    }
+  };
+  auto row = [&](int i) { return PAIRS == PAIRS_ANY ? reinterpret_cast<const T*>(&staged[i][group * L]) : nullptr; };
 
   const T* q = static_cast<const T*>(a.q.x) + token * a.q.token;
   T* q_out = static_cast<T*>(a.q_out) + (long long)token * a.heads * a.dim + at;
-  ln.set(a.q_weight, a.w_f32, cs, sn);
+  ln.set(a.q_weight, a.w_f32, cs[mine], sn[mine]);
   over(a.heads, integral_constant<int, QR_BATCH>{}, [&](auto n, auto check, int h0) {
     constexpr int N = decltype(n)::value;
     uint4 own[N], piece[N];
-    loads(n, check, q, a.q.head, a.heads, h0, at, own);
-    if (PAIRS == PAIRS_HALF) loads(n, check, q, a.q.head, a.heads, h0, ln.partner, piece);
-    T* out = q_out + (h0 + group) * a.dim;
+    loads(n, check, q, a.q.head, a.heads, h0, at, live, own);
+    if (PAIRS == PAIRS_HALF) loads(n, check, q, a.q.head, a.heads, h0, ln.partner, live, piece);
+    stage(n, own);
+    T* out = q_out + (h0 + member) * a.dim;
 #pragma unroll
     for (int i = 0; i < N; ++i, out += step * a.dim) {
-      const int h = h0 + group + i * step;
-      const bool there = live && (!decltype(check)::value || h < a.heads);
       f32x2 y[4];
       widen8<T>(own[i], y);
-      ln.apply(y, piece[i], there ? q + h * a.q.head : nullptr, a.q_weight != nullptr, a.eps, a.inv_dim, 1.f);
-      if (there) *reinterpret_cast<uint4*>(out) = round8<T>(y);
+      ln.apply(y, piece[i], row(i), a.q_weight != nullptr, a.eps, a.inv_dim, 1.f);
+      if (live && (!decltype(check)::value || h0 + member + i * step < a.heads)) *reinterpret_cast<uint4*>(out) = round8<T>(y);
     }
   });
 
   bool stored = false;
   uint8_t *k_row = nullptr, *v_row = nullptr;
-  if (a.cache.k) {
+  if (a.cache.k && exists) {
     const int slot = a.slots[token];
     const int n = a.cache.n_pages * a.cache.page_size;
     stored = slot >= 0 && slot < n;
-    if (slot >= n && a.status && threadIdx.x == 0 && blockIdx.y == 0) atomicOr(a.status, CACHALOT_STATUS_SLOT_RANGE);
+    if (slot >= n && a.status && member == 0 && threadIdx.x % L == 0 && blockIdx.y == 0) atomicOr(a.status, CACHALOT_STATUS_SLOT_RANGE);
     const int page = stored ? slot / a.cache.page_size : 0, off = stored ? slot - page * a.cache.page_size : 0;
     k_row = a.cache.k + page * a.cache.k_page + off * a.cache.k_token;
     v_row = a.cache.v + page * a.cache.v_page + off * a.cache.v_token;
   }
-  if (!stored && !a.k_out) return;
-  const bool f8 = a.cache.dtype == CACHALOT_E4M3;
+  if (!SEVERAL && !stored && !a.k_out) return;
+  const bool f8 = a.cache.dtype == CACHALOT_E4M3, wanted = live && (!SEVERAL || stored || a.k_out);
   const T* k = static_cast<const T*>(a.k.x) + token * a.k.token;
   const T* v = static_cast<const T*>(a.v.x) + token * a.v.token;
-  ln.set(a.k_weight, a.w_f32, cs, sn);
+  ln.set(a.k_weight, a.w_f32, cs[mine], sn[mine]);
   over(a.kv_heads, integral_constant<int, 2>{}, [&](auto n, auto check, int h0) {
     constexpr int N = decltype(n)::value;
     uint4 own[N], piece[N], value[N];
-    loads(n, check, k, a.k.head, a.kv_heads, h0, at, own);
-    if (PAIRS == PAIRS_HALF) loads(n, check, k, a.k.head, a.kv_heads, h0, ln.partner, piece);
-    if (stored) loads(n, check, v, a.v.head, a.kv_heads, h0, at, value);
+    loads(n, check, k, a.k.head, a.kv_heads, h0, at, wanted, own);
+    if (PAIRS == PAIRS_HALF) loads(n, check, k, a.k.head, a.kv_heads, h0, ln.partner, wanted, piece);
+    if (SEVERAL ? a.cache.k != nullptr : stored) loads(n, check, v, a.v.head, a.kv_heads, h0, at, wanted && (!SEVERAL || stored), value);
+    stage(n, own);
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int h = h0 + group + i * step;
-      const bool there = live && (!decltype(check)::value || h < a.kv_heads);
+      const int h = h0 + member + i * step;
+      const bool there = wanted && (!decltype(check)::value || h < a.kv_heads);
       f32x2 y[4];
       widen8<T>(own[i], y);
       // E4M3: times 1 / scale, one more rounding to fp32 than the division, instead of eight divisions
       const float k_times = f8 && a.cache.k_scale && there ? 1.f / a.cache.k_scale[h] : 1.f;
-      ln.apply(y, piece[i], there ? k + h * a.k.head : nullptr, a.k_weight != nullptr, a.eps, a.inv_dim, k_times);
+      ln.apply(y, piece[i], row(i), a.k_weight != nullptr, a.eps, a.inv_dim, k_times);
       if (!there) continue;
       if (a.k_out) *reinterpret_cast<uint4*>(static_cast<T*>(a.k_out) + ((long long)token * a.kv_heads + h) * a.dim + at) = round8<T>(y);
       if (!stored) continue;
@@ -339,21 +368,28 @@ extern "C" int cachalot_qk_norm_rope(const void* q, int64_t q_token_stride, int6
   }
   a.q = {q, q_token_stride, q_head_stride}, a.k = {k, k_token_stride, k_head_stride}, a.v = {v, v_token_stride, v_head_stride};
   a.q_weight = q_weight, a.k_weight = k_weight, a.w_f32 = w_dtype == CACHALOT_F32, a.eps = eps, a.magnitude = magnitude;
-  a.positions = positions, a.inv_freq = inv_freq, a.half = rotary_dim / 2, a.interleaved = interleaved != 0;
-  a.heads = heads, a.kv_heads = kv_heads, a.dim = head_dim, a.inv_dim = 1.f / (float)head_dim, a.q_out = q_out, a.k_out = k_out, a.slots = slots, a.status = status;
+  a.positions = positions, a.inv_freq = inv_freq, a.half = rotary_dim / 2;
+  a.tokens = tokens, a.heads = heads, a.kv_heads = kv_heads, a.dim = head_dim, a.inv_dim = 1.f / (float)head_dim, a.q_out = q_out, a.k_out = k_out, a.slots = slots, a.status = status;
   const int lanes = head_dim <= 64 ? 8 : head_dim <= 128 ? 16 : 32, groups = QR_THREADS / lanes;
-  const long long parts = ((long long)heads + groups - 1) / groups;         // CTAs of a token at most
-  const long long want = (600 + (long long)tokens - 1) / tokens;           // few tokens: their heads over more CTAs
-  const dim3 grid((unsigned)tokens, (unsigned)(parts < want ? parts : want));
+  // Many tokens of few heads: several tokens share a CTA, so that a group has eight heads per setting of its factors (18589
+  // tokens of 6 + 2 + 2 heads of 128: 22.6 us; 16384 of 16 + 2 + 2: 40 us, with four heads per setting 52).  Few tokens: their heads go over several CTAs.
+  int crew = groups;
+  while (crew > 1 && heads < 8 * crew && (long long)tokens * crew / groups >= 1200) crew /= 2;
+  for (a.crew_log2 = 0; 1 << a.crew_log2 < crew;) ++a.crew_log2;
+  const long long parts = ((long long)heads + groups - 1) / groups, want = (600 + (long long)tokens - 1) / tokens;
+  const dim3 grid((unsigned)((tokens + (long long)groups / crew - 1) / (groups / crew)), (unsigned)(parts < want ? parts : want));
   cudaStream_t s = (cudaStream_t)stream;
   cudaError_t e = cudaSuccess;
   auto run = [&](auto type, auto l) {
     using T = decltype(type);
     constexpr int L = decltype(l)::value;
-    const auto kern = rotary_dim % 8 == 0 && interleaved     ? qk_norm_rope_kernel<T, L, PAIRS_ADJACENT>
-                      : rotary_dim % 16 == 0 && !interleaved ? qk_norm_rope_kernel<T, L, PAIRS_HALF>
-                                                             : qk_norm_rope_kernel<T, L, PAIRS_ANY>;
-    e = launch_early(kern, grid, QR_THREADS, 0, s, 1, a);
+    auto pick = [&](auto several) {
+      constexpr bool SEVERAL = decltype(several)::value;
+      return interleaved       ? qk_norm_rope_kernel<T, L, PAIRS_ADJACENT, SEVERAL>
+             : rotary_dim % 16 ? qk_norm_rope_kernel<T, L, PAIRS_ANY, SEVERAL>
+                               : qk_norm_rope_kernel<T, L, PAIRS_HALF, SEVERAL>;
+    };
+    e = launch_early(crew < groups ? pick(std::true_type{}) : pick(std::false_type{}), grid, QR_THREADS, 0, s, 1, a);
   };
   auto go = [&](auto type) {
     if (lanes == 8) run(type, std::integral_constant<int, 8>{});

@@ -112,6 +112,14 @@ def test_caches(dim, page, dtype, cache, order):
     _case(19, 6, 2, dim, dim // 2, dtype, cache=cache, page=page, order=order, interleaved=dim == 96, seed=page)
 
 
+@pytest.mark.parametrize("cache", [None, torch.bfloat16, torch.float8_e4m3fn])
+@pytest.mark.parametrize("dim,heads,kv_heads,rotary,interleaved", [(64, 3, 1, 64, False), (128, 6, 2, 44, False), (128, 6, 2, 44, True), (192, 7, 1, 114, False),
+                                                                  (256, 1, 1, 256, False), (80, 17, 3, 6, True), (128, 20, 4, 128, False)])
+def test_many_tokens_of_few_heads(dim, heads, kv_heads, rotary, interleaved, cache):
+    """Several tokens share a CTA; their number is no multiple of what a CTA takes."""
+    _case(9607, heads, kv_heads, dim, rotary, torch.bfloat16, interleaved=interleaved, cache=cache, page=16, seed=dim)
+
+
 def test_options():
     _case(9, 4, 2, 128, 128, torch.bfloat16, norm=False)
     _case(9, 4, 2, 128, 128, torch.bfloat16, w_dtype=torch.float32)
@@ -148,6 +156,25 @@ def test_no_tokens_and_zero_heads():
     w = torch.ones(64, dtype=torch.bfloat16, device="cuda")
     y, k = cb.qk_norm_rope(z, z, torch.arange(2, dtype=torch.int32, device="cuda"), freq, q_weight=w, k_weight=w)
     assert not y.any() and not k.any()
+
+
+@pytest.mark.parametrize("rotary,interleaved", [(16, False), (20, False), (22, False), (20, True), (32, True)])
+def test_nan_and_inf_stay_in_their_pair_without_a_norm(rotary, interleaved):
+    import cachalot_b200 as cb
+
+    q = torch.randn((2, 3, 64), device="cuda").to(torch.bfloat16)
+    pos, freq = torch.arange(1, 3, dtype=torch.int32, device="cuda"), cb.rope_frequencies(rotary)[0]
+    clean = cb.qk_norm_rope(q, q, pos, freq, interleaved=interleaved)[0]
+    for at, value in ((1, float("nan")), (rotary - 1, float("inf")), (rotary, float("nan")), (rotary + 1, float("inf")), (63, float("nan"))):
+        bad = q.clone()
+        bad[1, 2, at] = value
+        y = cb.qk_norm_rope(bad, bad, pos, freq, interleaved=interleaved)[0]
+        mate = at if at >= rotary else at ^ 1 if interleaved else (at + rotary // 2) % rotary
+        same = torch.ones(64, dtype=torch.bool, device="cuda")
+        same[[at, mate]] = False
+        assert torch.equal(y[1, 2, same], clean[1, 2, same]) and torch.equal(y[0], clean[0]) and not torch.isfinite(y[1, 2, [at, mate]]).any()
+        if at >= rotary:
+            assert torch.equal(y[1, 2, at].isnan(), torch.tensor(value != value, device="cuda"))
 
 
 def test_nan_and_inf_stay_in_their_head():
