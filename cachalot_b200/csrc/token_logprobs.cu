@@ -8,7 +8,7 @@
 // worked on.  A row is split over a cluster of CTAs where there are few rows, joined through distributed shared memory:
 // one launch, no workspace.
 //
-// The alternatives.  The first round of a CTA finds the n-th largest of its 256 threads' own maxima, a lower bound ("bar")
+// The alternatives.  The first round of a CTA finds the n-th largest of its threads' own maxima, a lower bound ("bar")
 // of the n-th best that about n threads reach; from then on a thread whose maximum reaches the bar appends that maximum and
 // its place to a list in shared memory, and after 4, 8, 16 .. rounds the bar is raised to the list's n-th largest: about n
 // entries per doubling on logits in no particular order.  At the end the entries that reach the last bar, about n, are read again, an
@@ -28,9 +28,9 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int TL_THREADS = 256, TL_WARPS = TL_THREADS / 32, TL_MAX_TOP = 32, TL_LOADS = 4;
-constexpr int TL_CTAS = 4;     // per SM: up to 64 KB of loads in flight
-constexpr int TL_SEEN = 1024;
+constexpr int TL_WARPS = 8;    // of a CTA; 4 or 2 for many rows
+constexpr int TL_MAX_TOP = 32, TL_LOADS = 4;
+constexpr int TL_CTAS = 4;     // of 8 warps per SM: up to 64 KB of loads in flight
 constexpr int TL_LIST = 1088;  // 32 kept + 32 threads of 32 elements
 constexpr float TL_LOG2E = 1.4426950408889634f;
 constexpr float TL_FAR = -200.f;  // e^-200 is zero in fp32; stands for -inf, which would make 0 * -inf
@@ -124,7 +124,7 @@ __device__ __forceinline__ unsigned merge32(unsigned a, unsigned b, int lane) {
 
 // ... of the first `n` warps' sorted lists, in warp 0 and in lists[0]; the others' lists are empty
 template <typename K>
-__device__ __forceinline__ K merge_block(K x, K (*lists)[32], int warp, int lane, int n = TL_WARPS) {
+__device__ __forceinline__ K merge_block(K x, K (*lists)[32], int warp, int lane, int n) {
   lists[warp][lane] = x;
   for (int step = 1; step < n; step <<= 1) {
     __syncthreads();
@@ -133,8 +133,8 @@ __device__ __forceinline__ K merge_block(K x, K (*lists)[32], int warp, int lane
   __syncthreads();
   return x;
 }
-// warps that sort a list of this length, 32 at a time each
-__device__ __forceinline__ int warps_of(int length) { return min((length + 31) / 32, TL_WARPS); }
+// warps of `all` that sort a list of this length, 32 at a time each
+__device__ __forceinline__ int warps_of(int length, int all) { return min((length + 31) / 32, all); }
 
 // 16 bytes of logits
 template <typename T>
@@ -189,16 +189,17 @@ struct Vec {
 
 // A CTA's share of a row: 16-byte vectors (the first and the last of the row may reach over its ends), in rounds of
 // TL_LOADS per thread, upwards.
-template <typename T>
+template <typename T, int WARPS>
 struct Share {
+  static constexpr int THREADS = WARPS * 32;
   const T* row;
   int vocab, shift, ctas, rank, rounds;
   __device__ __forceinline__ Share(const T* r, int n, int c, int k) : row(r), vocab(n), ctas(c), rank(k) {
     shift = (int)(reinterpret_cast<uintptr_t>(r) % 16 / sizeof(T));
-    rounds = ((n + shift + Vec<T>::PER - 1) / Vec<T>::PER + c * TL_LOADS * TL_THREADS - 1) / (c * TL_LOADS * TL_THREADS);
+    rounds = ((n + shift + Vec<T>::PER - 1) / Vec<T>::PER + c * TL_LOADS * THREADS - 1) / (c * TL_LOADS * THREADS);
   }
   __device__ __forceinline__ int index(int round, int k, int thread) const {  // of the first element of a thread's k-th vector
-    return (((round * ctas + rank) * TL_LOADS + k) * TL_THREADS + thread) * Vec<T>::PER - shift;
+    return (((round * ctas + rank) * TL_LOADS + k) * THREADS + thread) * Vec<T>::PER - shift;
   }
   __device__ __forceinline__ int index(int round, int k) const { return index(round, k, (int)threadIdx.x); }
   __device__ __forceinline__ void fetch(Vec<T> (&v)[TL_LOADS], int round) const {
@@ -208,8 +209,8 @@ struct Share {
 };
 
 // The best n of a round in hand: the thread's own best, and its elements that reach a bar, appended to a list.
-template <typename T>
-__device__ __forceinline__ Key best_of(const Share<T>& sh, const Vec<T> (&v)[TL_LOADS], int round, float most) {
+template <typename T, int WARPS>
+__device__ __forceinline__ Key best_of(const Share<T, WARPS>& sh, const Vec<T> (&v)[TL_LOADS], int round, float most) {
   Key best = 0;
 #pragma unroll
   for (int k = TL_LOADS - 1; k >= 0; --k)
@@ -221,8 +222,8 @@ __device__ __forceinline__ Key best_of(const Share<T>& sh, const Vec<T> (&v)[TL_
   return best;
 }
 // A thread's elements of a round that reach the bar, appended to the list.
-template <typename T>
-__device__ __forceinline__ void offer(const Share<T>& sh, const Vec<T> (&v)[TL_LOADS], int round, Key bar, float bar_value, Key* list, int base, int* count) {
+template <typename T, int WARPS>
+__device__ __forceinline__ void offer(const Share<T, WARPS>& sh, const Vec<T> (&v)[TL_LOADS], int round, Key bar, float bar_value, Key* list, int base, int* count) {
 #pragma unroll
   for (int k = 0; k < TL_LOADS; ++k) {
     if (!(v[k].top() >= bar_value)) continue;
@@ -244,9 +245,9 @@ __device__ __forceinline__ void offer(const Share<T>& sh, const Vec<T> (&v)[TL_L
 // The careful selection, for rows where a list overflowed: over the share once more, the bar raised in every round that would
 // overflow the list, from the list and the threads' own best together (at most n threads reach it, so at most 32 n elements).
 // Returns the length of the list.  `added`: three counters for the rounds in turn (one counted, one still read, one cleared).
-template <typename T>
-__device__ __noinline__ int select_carefully(const Share<T> sh, int top, Key* list, Key (*lists)[32], int* added) {
-  constexpr int CHUNKS = (TL_LIST + TL_THREADS - 1) / TL_THREADS;
+template <typename T, int WARPS>
+__device__ __noinline__ int select_carefully(const Share<T, WARPS> sh, int top, Key* list, Key (*lists)[32], int* added) {
+  constexpr int THREADS = WARPS * 32, CHUNKS = (TL_LIST + THREADS - 1) / THREADS;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   int held = 0;
   Key bar = 0;
@@ -275,12 +276,12 @@ __device__ __noinline__ int select_carefully(const Share<T> sh, int top, Key* li
       }
     }
     Key mine = sort32(best_of(sh, v, round, most), lane);  // what the round has added to the list is given up
-    for (int at = warp * 32; at < held; at += TL_THREADS) mine = merge32(mine, sort32(at + lane < held ? list[at + lane] : 0, lane), lane);
-    merge_block(mine, lists, warp, lane);
+    for (int at = warp * 32; at < held; at += THREADS) mine = merge32(mine, sort32(at + lane < held ? list[at + lane] : 0, lane), lane);
+    merge_block(mine, lists, warp, lane, WARPS);
     bar = lists[0][top - 1], bar_value = value_of(bar);
     Key kept[CHUNKS];
 #pragma unroll
-    for (int c = 0; c < CHUNKS; ++c) kept[c] = c * TL_THREADS + tid < held ? list[c * TL_THREADS + tid] : 0;
+    for (int c = 0; c < CHUNKS; ++c) kept[c] = c * THREADS + tid < held ? list[c * THREADS + tid] : 0;
     if (tid == 0) *count = 0;
     __syncthreads();
 #pragma unroll
@@ -293,17 +294,17 @@ __device__ __noinline__ int select_carefully(const Share<T> sh, int top, Key* li
   return held;
 }
 
-template <typename T, bool TOP>
-__global__ void __launch_bounds__(TL_THREADS, TL_CTAS) token_logprobs_kernel(const T* logits, long long stride, int vocab,
+template <typename T, bool TOP, int WARPS>
+__global__ void __launch_bounds__(WARPS * 32, TL_CTAS * TL_WARPS / WARPS) token_logprobs_kernel(const T* logits, long long stride, int vocab,
                                                                              const int32_t* tokens, int top, float* logprobs,
                                                                              float* entropy, int32_t* top_ids,
                                                                              float* top_logprobs, int* status) {
   using V = Vec<T>;
-  constexpr int PER = V::PER;
-  __shared__ Sums parts[TL_WARPS];
-  __shared__ Key lists[TOP ? TL_WARPS : 1][32];
+  constexpr int PER = V::PER, THREADS = WARPS * 32, SEEN = 128 * WARPS;
+  __shared__ Sums parts[WARPS];
+  __shared__ Key lists[TOP ? WARPS : 1][32];
   __shared__ Key list[TOP ? TL_LIST : 1];
-  __shared__ uint2 seen[TOP ? TL_SEEN : 1];  // maxima that reached the bar: ordered value, round * threads + thread
+  __shared__ uint2 seen[TOP ? SEEN : 1];  // maxima that reached the bar: ordered value, round * threads + thread
   __shared__ int added[3], noted;
   unsigned(*bars)[32] = reinterpret_cast<unsigned(*)[32]>(lists);
   wait_for_predecessor();
@@ -311,7 +312,7 @@ __global__ void __launch_bounds__(TL_THREADS, TL_CTAS) token_logprobs_kernel(con
   const int ctas = cluster.num_blocks(), rank = cluster.block_rank();
   const int row = blockIdx.x / ctas, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const T* x = logits + row * stride;
-  const Share<T> sh(x, vocab, ctas, rank);
+  const Share<T, WARPS> sh(x, vocab, ctas, rank);
 
   Sums sum{-FLT_MAX, 0.f, 0.f};
   float bar = -INFINITY;  // nothing below it is among the best
@@ -327,10 +328,10 @@ __global__ void __launch_bounds__(TL_THREADS, TL_CTAS) token_logprobs_kernel(con
   auto raise = [&] {  // to the n-th largest of the maxima so far
     __syncthreads();
     const int n = noted;
-    if (n > TL_SEEN) return;
+    if (n > SEEN) return;
     unsigned mine = 0;
-    for (int at = warp * 32; at < n; at += TL_THREADS) mine = merge32(mine, sort32(at + lane < n ? seen[at + lane].x : 0u, lane), lane);
-    bar = fmaxf(bar, value_of(nth(mine, warps_of(n))));
+    for (int at = warp * 32; at < n; at += THREADS) mine = merge32(mine, sort32(at + lane < n ? seen[at + lane].x : 0u, lane), lane);
+    bar = fmaxf(bar, value_of(nth(mine, warps_of(n, WARPS))));
   };
   for (int round = 0; round < sh.rounds; ++round) {
     V now[TL_LOADS];
@@ -348,10 +349,10 @@ __global__ void __launch_bounds__(TL_THREADS, TL_CTAS) token_logprobs_kernel(con
     const float2 s2 = both(part.s), u2 = both(part.u);
     sum.s += s2.x + s2.y, sum.u += u2.x + u2.y;
     if constexpr (TOP) {
-      if (round == 0) bar = value_of(nth(sort32(order_of(most), lane), TL_WARPS));
-      if (most >= bar) {
+      if (round == 0) bar = value_of(nth(sort32(order_of(most), lane), WARPS));
+      if (most >= bar && sh.index(round, 0) < vocab) {  // a thread past the row has nothing to note
         const int at = atomicAdd(&noted, 1);
-        if (at < TL_SEEN) seen[at] = make_uint2(order_of(most), round * TL_THREADS + tid);
+        if (at < SEEN) seen[at] = make_uint2(order_of(most), round * THREADS + tid);
       }
       if (round > 2 && (round & (round + 1)) == 0 && round + 1 < sh.rounds) raise();
     }
@@ -372,11 +373,11 @@ __global__ void __launch_bounds__(TL_THREADS, TL_CTAS) token_logprobs_kernel(con
     raise();
     const int n = noted;
     int held = TL_LIST + 1;
-    if (n <= TL_SEEN) {  // the elements of the entries that reach the bar, a lane each
-      for (int at = warp; at < n; at += TL_WARPS) {
+    if (n <= SEEN) {  // the elements of the entries that reach the bar, a lane each
+      for (int at = warp; at < n; at += WARPS) {
         const uint2 entry = seen[at];
         if (!(value_of(entry.x) >= bar)) continue;
-        const int i = sh.index(entry.y / TL_THREADS, lane / PER % TL_LOADS, entry.y % TL_THREADS) + lane % PER;
+        const int i = sh.index(entry.y / THREADS, lane / PER % TL_LOADS, entry.y % THREADS) + lane % PER;
         const bool there = lane < PER * TL_LOADS && i >= 0 && i < vocab;
         const float v = there ? V::widen(x[i]) : 0.f;
         const unsigned hit = __ballot_sync(0xffffffffu, there && v >= bar);
@@ -389,14 +390,14 @@ __global__ void __launch_bounds__(TL_THREADS, TL_CTAS) token_logprobs_kernel(con
       held = added[0];
     }
     if (held > TL_LIST) held = select_carefully(sh, top, list, lists, added);
-    for (int at = warp * 32; at < held; at += TL_THREADS) best = merge32(best, sort32(at + lane < held ? list[at + lane] : 0, lane), lane);
-    best = merge_block(best, lists, warp, lane, warps_of(held));
+    for (int at = warp * 32; at < held; at += THREADS) best = merge32(best, sort32(at + lane < held ? list[at + lane] : 0, lane), lane);
+    best = merge_block(best, lists, warp, lane, warps_of(held, WARPS));
   }
   if (warp == 0) {
-    sum = parts[lane % TL_WARPS];
-    join_lanes(TL_WARPS / 2);
+    sum = parts[lane % WARPS];
+    join_lanes(WARPS / 2);
   }
-  if (ctas > 1) {  // ctas <= TL_WARPS: a warp for each CTA's list, lanes for their sums
+  if (ctas > 1) {  // ctas <= WARPS: a warp for each CTA's list, lanes for their sums
     __syncthreads();
     if (tid == 0) parts[0] = sum;
     cluster.sync();
@@ -429,10 +430,16 @@ __global__ void __launch_bounds__(TL_THREADS, TL_CTAS) token_logprobs_kernel(con
 }
 
 template <typename T>
-cudaError_t launch(bool with_top, int rows, int ctas, cudaStream_t stream, const void* logits, long long stride, int vocab, const int32_t* tokens, int top,
+cudaError_t launch(bool with_top, int warps, int rows, int ctas, cudaStream_t stream, const void* logits, long long stride, int vocab, const int32_t* tokens, int top,
                    float* logprobs, float* entropy, int32_t* top_ids, float* top_logprobs, int* status) {
-  const auto kern = with_top ? token_logprobs_kernel<T, true> : token_logprobs_kernel<T, false>;
-  return launch_early(kern, dim3((unsigned)rows * ctas), TL_THREADS, 0, stream, ctas, static_cast<const T*>(logits), stride, vocab, tokens, top, logprobs,
+  auto pick = [&](auto n) {
+    constexpr int WARPS = decltype(n)::value;
+    return with_top ? token_logprobs_kernel<T, true, WARPS> : token_logprobs_kernel<T, false, WARPS>;
+  };
+  using std::integral_constant;
+  const auto kern = warps == 2 ? pick(integral_constant<int, 2>{})
+                    : warps == 4 ? pick(integral_constant<int, 4>{}) : pick(integral_constant<int, TL_WARPS>{});
+  return launch_early(kern, dim3((unsigned)rows * ctas), warps * 32, 0, stream, ctas, static_cast<const T*>(logits), stride, vocab, tokens, top, logprobs,
                       entropy, top_ids, top_logprobs, status);
 }
 
@@ -454,17 +461,22 @@ extern "C" int cachalot_token_logprobs(const void* logits, int dtype, int64_t ro
   const int es = dtype == CACHALOT_F32 ? 4 : 2;
   if (!aligned(logits, es)) return fail(CACHALOT_EALIGN, "token_logprobs: logits are not aligned to their type");
   if (vocab > 0x7fffffff - 131072) return fail(CACHALOT_EUNSUPPORTED, "token_logprobs: vocabulary of %d", vocab);
-  // CTAs of a row: enough to fill the GPU with few rows, a power of two up to the portable cluster size
-  const double slots = 148.0 * TL_CTAS, row_us = (double)vocab * es / 16e3, fixed_us = top ? 3.0 : 1.0;  // a CTA: 16 GB/s, and its joins
+  // What ends a row costs its CTA the same for any number of warps, so many rows get small CTAs (us with 2, 4 and 8 warps):
+  // 600 rows of 4000 bf16 12.2, 8.4, 13.2; 600 of 129280 71.9, 52.2, 52.1; 1300 of 16000 26.2, 26.3, 27.4; 4096 of 4000 and the
+  // 32 largest 41, 42, 62; 16384 of 32000 240, 267, 312; 2048 of 129280 119, 113, 116.
+  const int warps = rows > 1184 && (long long)vocab * es <= 65536 ? 2 : rows > 592 ? 4 : TL_WARPS;
+  // CTAs of a row: what takes the least time with 16 GB/s and a fixed part each, and the cluster's meeting where there is
+  // more than one
+  const double slots = 148.0 * TL_CTAS, row_us = (double)vocab * es / 16e3, fixed_us = top ? 3.0 : 1.0, meet_us = top ? 3.0 : 1.5;
   int ctas = 1;
   double least = 1e30;
-  for (int c = 1; c <= TL_WARPS; c *= 2) {
-    const double us = ceil((double)rows * c / slots) * (row_us / c + fixed_us);
+  for (int c = 1; c <= 8 && warps == TL_WARPS; c *= 2) {
+    const double us = ceil((double)rows * c / slots) * (row_us / c + fixed_us) + (c > 1 ? meet_us : 0.0);
     if (us < least) least = us, ctas = c;
   }
   if ((long long)rows * ctas > 0x7fffffffLL) return fail(CACHALOT_EUNSUPPORTED, "token_logprobs: %d rows", rows);
   const auto go = dtype == CACHALOT_F32 ? launch<float> : dtype == CACHALOT_BF16 ? launch<__nv_bfloat16> : launch<__half>;
-  const cudaError_t e = go(top > 0, rows, ctas, (cudaStream_t)stream, logits, row_stride, vocab, tokens, top, logprobs, entropy, top_ids, top_logprobs, status);
+  const cudaError_t e = go(top > 0, warps, rows, ctas, (cudaStream_t)stream, logits, row_stride, vocab, tokens, top, logprobs, entropy, top_ids, top_logprobs, status);
   if (e != cudaSuccess) return fail(CACHALOT_ECUDA, "token_logprobs: %s", cudaGetErrorString(e));
   return check_launch("token_logprobs");
 }

@@ -2,7 +2,8 @@
 
 Tolerance: the sum of weights is off by at most one part in 2^24 per dependent addition (a thread adds vocab / 256 terms, then 64
 covers the joins, the approximate exp2 and its argument's rounding for terms that matter); that goes into ln S as it is,
-and into U / S times U / S + 1 <= entropy + ln S + 1.  On top, the log probability itself is rounded (2^-23 of it)."""
+and into U / S times U / S + 1 <= entropy + ln S + 1.  On top, the log probability itself is rounded (2^-23 of it).  (256: at
+least 128 threads with two sums each.  The 64 threads that a row gets where there are more than 1184 add vocab / 128.)"""
 import numpy as np
 import pytest
 
@@ -18,7 +19,7 @@ def _gen(seed):
     return torch.Generator(device="cuda").manual_seed(seed)
 
 
-def _check(x, tokens, top, status=0):
+def _check(x, tokens, top, status=0, sums=256):
     import cachalot_b200 as cb
 
     word = torch.zeros(1, dtype=torch.int32, device="cuda")
@@ -29,7 +30,7 @@ def _check(x, tokens, top, status=0):
     rows, vocab = h.shape
     assert r.logprobs.shape == r.entropy.shape == (rows,) and r.top_ids.shape == r.top_logprobs.shape == (rows, top)
     assert np.array_equal(r.top_ids.cpu().numpy(), ids)
-    step = (vocab / 256 + 64) * 2.0 ** -24
+    step = (vocab / sums + 64) * 2.0 ** -24
     for got, want in ((r.logprobs, lp), (r.top_logprobs, best)):
         got = got.double().cpu().numpy()
         assert np.array_equal(np.isnan(got), np.isnan(want)) and np.array_equal(got == -np.inf, want == -np.inf)
@@ -72,6 +73,18 @@ def test_orders_and_ties(order, dtype):
     i = torch.arange(v, device="cuda", dtype=torch.float32)
     x = {"up": i / 1000, "down": -i / 1000, "equal": torch.zeros_like(i), "two": (i.to(torch.int32) % 97 == 96).float(), "late": (i >= v - 5).float() * 3}[order]
     _check(x.to(dtype)[None].repeat(2, 1), [3, v - 1], 32)
+
+
+@pytest.mark.parametrize("rows", [600, 1200])
+@pytest.mark.parametrize("vocab,dtype", [(1, F32), (37, BF16), (1001, F16), (1023, F32), (2049, BF16), (4100, F16), (9001, F32), (30001, BF16)])
+def test_many_rows(rows, vocab, dtype):
+    """Each of the orders above and rows of random logits, masked ones among them."""
+    g, i = _gen(vocab), torch.arange(vocab, device="cuda", dtype=torch.float32)
+    x = torch.randn((rows, vocab), device="cuda", generator=g) * 3
+    x[0::7], x[1::7], x[2::7], x[3::7] = i / 100, -i / 100, 0.0, (i.to(torch.int32) % 97 == 96).float()
+    x[4::7, vocab // 3:] = -float("inf")
+    x[5::7, vocab // 2:] = torch.finfo(dtype).min
+    _check(x.to(dtype), [(k * 977) % vocab for k in range(rows)], min(vocab, 32), sums=256 if rows == 600 else 128)
 
 
 @pytest.mark.parametrize("offset", range(1, 9))
