@@ -654,15 +654,18 @@ AttendLaunch attend_shape(int group) {
   return l;
 }
 // Column tiles of 8 query heads per warp: as few warps as possible read the same keys, up to three tiles where the registers hold
-// their sums (heads of up to 128).  24 heads to a key-value head: 121 us with three tiles, 178 with two tiles in two warps.
+// their sums; wider heads have fewer.  64 requests over up to 8192 tokens of E4M3, 24 heads to a key-value head: heads of 128 121 us
+// with three tiles, 178 with two in two warps; of 192 321, 405, and 604 with one in four warps; of 256 720, 471, 691.  16 heads to
+// one: of 192 225 with two tiles, 323 with one; of 256 244, 356.  bf16, 32 requests: of 192 181 with two, 205 with one; of 256 390, 268.
 template <bool F8, typename Fn>
 bool attend_dispatch(int dim, int group, Fn&& fn) {
   auto go = [&](auto d, auto nt) { fn(d, nt, attend_shape<F8, decltype(d)::value, decltype(nt)::value>(group)); };
   using std::integral_constant;
   auto nt = [&](auto d) {
-    if constexpr (decltype(d)::value <= 128) {
+    if constexpr (decltype(d)::value <= 192 || F8) {
       const int two = (group + 15) / 16, three = (group + 23) / 24;  // warps
-      if (group > 16 && (three == 1 || (two > 2 && three == 2))) return go(d, integral_constant<int, 3>{});
+      if constexpr (decltype(d)::value <= (F8 ? 192 : 128))
+        if (group > 16 && (three == 1 || (two > 2 && three == 2))) return go(d, integral_constant<int, 3>{});
       if (group > 8) return go(d, integral_constant<int, 2>{});
     }
     go(d, integral_constant<int, 1>{});

@@ -124,6 +124,13 @@ def test_groups(group, dim, cache):
     Case([1, 40, 200, 0], 2 * group, 2, dim, 8, BF16, cache, seed=group).check()
 
 
+@pytest.mark.parametrize("cache", [BF16, E4M3])
+@pytest.mark.parametrize("dim", [96, 192])
+@pytest.mark.parametrize("group", [9, 16, 17, 24, 48, 56, 70])
+def test_groups_of_other_head_sizes(group, dim, cache):
+    Case([1, 40, 200, 0], 2 * group, 2, dim, 16, BF16, cache, seed=group).check()
+
+
 @pytest.mark.parametrize("page", [1, 3, 8, 16, 24, 32, 40, 64, 100, 256])
 @pytest.mark.parametrize("order", ["heads", "tokens"])
 def test_pages(page, order):
