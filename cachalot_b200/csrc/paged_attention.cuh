@@ -176,6 +176,19 @@ __device__ __forceinline__ void store_out(void* out, int dtype, long long at, fl
   else if (dtype == CACHALOT_BF16) static_cast<__nv_bfloat16*>(out)[at] = __float2bfloat16_rn(v);
   else static_cast<__half*>(out)[at] = __float2half_rn(v);
 }
+// ... of elements at .. at + 3, at a multiple of 4
+__device__ __forceinline__ void store_out4(void* out, int dtype, long long at, float4 v) {
+  const bool whole = ((uintptr_t)out & (dtype == CACHALOT_F32 ? 15 : 7)) == 0;
+  if (!whole) {
+    store_out(out, dtype, at, v.x), store_out(out, dtype, at + 1, v.y), store_out(out, dtype, at + 2, v.z), store_out(out, dtype, at + 3, v.w);
+  } else if (dtype == CACHALOT_F32) {
+    *reinterpret_cast<float4*>(static_cast<float*>(out) + at) = v;
+  } else {
+    const uint2 w = dtype == CACHALOT_BF16 ? make_uint2(pack2<__nv_bfloat16>(v.x, v.y), pack2<__nv_bfloat16>(v.z, v.w))
+                                           : make_uint2(pack2<__half>(v.x, v.y), pack2<__half>(v.z, v.w));
+    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(out) + at) = w;
+  }
+}
 
 template <typename M, bool F8, int D, int NT, bool PAGE8, bool KEEP>
 __global__ void __launch_bounds__(PA_THREADS, AttendShape<F8, D, NT>::CTAS) attend_kernel(const AttendArgs a) {
@@ -394,32 +407,61 @@ __global__ void __launch_bounds__(PA_THREADS, AttendShape<F8, D, NT>::CTAS) atte
 
     // ---- the query heads as MMA fragments ----
     if constexpr (F8) {  // f16 from here on: a bf16 head is brought into range by a power of two
-      for (int i = warp; i < unit_heads; i += PA_WARPS) {
-        float top = 0.f;
-        if (i < heads && a.q_bf16) {
-          const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(a.q) + r * a.q_row + (long long)(h * a.group + head0 + i) * a.q_head;
-          for (int d = lane; d < D; d += 32) top = fmaxf(top, fabsf(__bfloat162float(q[d])));
-          top = warp_max(top);
+      for (int i0 = warp; i0 < unit_heads; i0 += 4 * PA_WARPS) {  // four heads' loads at a time
+        float top[4] = {};
+        if (a.q_bf16) {
+          uint32_t x[4][(D + 63) / 64];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int i = min(i0 + j * PA_WARPS, heads - 1);
+            const uint16_t* q = static_cast<const uint16_t*>(a.q) + r * a.q_row + (long long)(h * a.group + head0 + i) * a.q_head;
+#pragma unroll
+            for (int c = 0; c < (D + 63) / 64; ++c) {
+              const int d = c * 64 + 2 * lane;
+              x[j][c] = d < D ? *reinterpret_cast<const uint32_t*>(q + d) : 0;
+            }
+          }
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+#pragma unroll
+            for (int c = 0; c < (D + 63) / 64; ++c)
+              top[j] = fmaxf(top[j], fmaxf(fabsf(__uint_as_float(x[j][c] << 16)), fabsf(__uint_as_float(x[j][c] & 0xffff0000u))));
+            top[j] = warp_max(top[j]);
+          }
         }
-        const int e = (int)((__float_as_uint(top) >> 23) & 255) - 127;
-        if (lane == 0) sexp[i] = top > 0.f ? pow2f(max(-126, min(126, e))) : 1.f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int e = (int)((__float_as_uint(top[j]) >> 23) & 255) - 127;
+          if (lane == 0 && i0 + j * PA_WARPS < unit_heads) sexp[i0 + j * PA_WARPS] = top[j] > 0.f ? pow2f(max(-126, min(126, e))) : 1.f;
+        }
       }
       __syncthreads();
     }
-    for (int i = tid; i < a.tiles * NT * S::KSTEPS * 32; i += PA_THREADS) {
-      const int l = i & 31, ks = (i >> 5) % S::KSTEPS, head = (i >> 5) / S::KSTEPS * 8 + (l >> 2);
-      const int d0 = F8 ? S::k_dim(ks, l & 3) : S::k_dim(2 * ks, l & 3), d1 = F8 ? d0 + 2 : S::k_dim(2 * ks + 1, l & 3);
-      uint2 f = make_uint2(0, 0);
-      if (head < heads) {
-        const uint16_t* q = static_cast<const uint16_t*>(a.q) + r * a.q_row + (long long)(h * a.group + head0 + head) * a.q_head;
-        f.x = *reinterpret_cast<const uint32_t*>(q + d0), f.y = *reinterpret_cast<const uint32_t*>(q + d1);
-        if (F8 && a.q_bf16) {
-          const float inv = 1.f / sexp[head];  // a power of two
-          f.x = pack2<__half>(__uint_as_float(f.x << 16) * inv, __uint_as_float(f.x & 0xffff0000u) * inv);
-          f.y = pack2<__half>(__uint_as_float(f.y << 16) * inv, __uint_as_float(f.y & 0xffff0000u) * inv);
+    // Several loads of a thread in flight: one at a time, 161 requests of 2 tokens with 52 heads took 25.8 us, not 20.8.
+    constexpr int BATCH = NT * S::KSTEPS >= 16 ? 8 : (NT * S::KSTEPS + 1) / 2;
+    for (int i0 = tid; i0 < a.tiles * NT * S::KSTEPS * 32; i0 += BATCH * PA_THREADS) {
+      uint2 f[BATCH];
+#pragma unroll
+      for (int j = 0; j < BATCH; ++j) {
+        const int i = i0 + j * PA_THREADS, l = i & 31, ks = (i >> 5) % S::KSTEPS, head = (i >> 5) / S::KSTEPS * 8 + (l >> 2);
+        const int d0 = F8 ? S::k_dim(ks, l & 3) : S::k_dim(2 * ks, l & 3), d1 = F8 ? d0 + 2 : S::k_dim(2 * ks + 1, l & 3);
+        f[j] = make_uint2(0, 0);
+        if (head < heads) {
+          const uint16_t* q = static_cast<const uint16_t*>(a.q) + r * a.q_row + (long long)(h * a.group + head0 + head) * a.q_head;
+          f[j].x = *reinterpret_cast<const uint32_t*>(q + d0), f[j].y = *reinterpret_cast<const uint32_t*>(q + d1);
         }
       }
-      sq[i] = f;
+#pragma unroll
+      for (int j = 0; j < BATCH; ++j) {
+        const int i = i0 + j * PA_THREADS, head = (i >> 5) / S::KSTEPS * 8 + ((i & 31) >> 2);
+        if (i >= a.tiles * NT * S::KSTEPS * 32) break;
+        if (F8 && a.q_bf16) {
+          const float inv = 1.f / sexp[head];  // a power of two
+          f[j].x = pack2<__half>(__uint_as_float(f[j].x << 16) * inv, __uint_as_float(f[j].x & 0xffff0000u) * inv);
+          f[j].y = pack2<__half>(__uint_as_float(f[j].y << 16) * inv, __uint_as_float(f[j].y & 0xffff0000u) * inv);
+        }
+        sq[i] = f[j];
+      }
     }
     __syncthreads();
 
@@ -617,8 +659,7 @@ __global__ void __launch_bounds__(PA_THREADS, AttendShape<F8, D, NT>::CTAS) atte
       if (whole) {
         const float inv = sum == 0.f ? 0.f : v_scale / sum;
         const long long to = (row0 + head) * D + d;
-        store_out(a.out, a.out_dtype, to, v.x * inv), store_out(a.out, a.out_dtype, to + 1, v.y * inv);
-        store_out(a.out, a.out_dtype, to + 2, v.z * inv), store_out(a.out, a.out_dtype, to + 3, v.w * inv);
+        store_out4(a.out, a.out_dtype, to, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
         if (d == 0 && a.lse) a.lse[row0 + head] = sum == 0.f ? -INFINITY : (top - SHIFT + log2f(sum)) * PA_LN2;
       } else {
         *reinterpret_cast<float4*>(a.part_o + (slot * unit_heads + head) * D + d) = v;
@@ -654,9 +695,11 @@ AttendLaunch attend_shape(int group) {
   return l;
 }
 // Column tiles of 8 query heads per warp: as few warps as possible read the same keys, up to three tiles where the registers hold
-// their sums; wider heads have fewer.  64 requests over up to 8192 tokens of E4M3, 24 heads to a key-value head: heads of 128 121 us
-// with three tiles, 178 with two in two warps; of 192 321, 405, and 604 with one in four warps; of 256 720, 471, 691.  16 heads to
-// one: of 192 225 with two tiles, 323 with one; of 256 244, 356.  bf16, 32 requests: of 192 181 with two, 205 with one; of 256 390, 268.
+// their sums; wider heads have fewer.  Each with both sides measured when it was chosen (loads of the queries have since been
+// batched, which took 5 to 17 % off), E4M3, 64 requests of up to 8192 tokens, 8 key-value heads: 24 heads to each, of 192: 321 us with three
+// tiles, 405 with two, 604 with one; of 256: 720, 471, 691.  16 heads to each, of 192: 225 with two, 323 with one; of 256: 244, 356.
+// bf16, 32 requests, 16 heads to each, of 192: 181 with two, 205 with one; of 256: 390, 268.  24 heads of 128 to each of 2, up to 16384
+// tokens: 121 with three in one warp, 178 with two in two.
 template <bool F8, typename Fn>
 bool attend_dispatch(int dim, int group, Fn&& fn) {
   auto go = [&](auto d, auto nt) { fn(d, nt, attend_shape<F8, decltype(d)::value, decltype(nt)::value>(group)); };
