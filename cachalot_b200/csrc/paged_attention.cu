@@ -193,7 +193,7 @@ extern "C" int cachalot_paged_attention(const void* q, int64_t q_row_stride, int
   const int step_bytes = l.step * 2 * a.c.head_dim * paged_elem_bytes(a.c.dtype);
   // 48 KB: two steps of 128-element heads (a batch of very different lengths 44.7 us, with three 46.2); with two CTAs per SM, each
   // of which gets more of the bandwidth, 96 KB (16 heads to a key-value head 105 us, with 48 KB 113); over an E4M3 cache,
-  // where instructions count for more than bytes, 384 tokens: three steps (batch of 64: 100 us, with two 107)
+  // where instructions count for more than bytes, 384 tokens: three steps (batch of 64: 7 us less than with two)
   const int cost_bytes = l.ctas_per_sm > 2 ? 48 * 1024 : 96 * 1024;
   a.unit_cost = f8 ? (384 + l.step - 1) / l.step : (cost_bytes + step_bytes - 1) / step_bytes;
   a.scale = scale, a.softcap = softcap, a.window = window, a.out = out, a.out_dtype = out_dtype, a.lse = lse, a.status = status;

@@ -22,4 +22,6 @@ Parity status per module:
   mxfp4.py    parity unpinned beyond the reference's rounding table
               (MLX only).
   prefill.py  parity unpinned beyond the reference's ordering rules.
+  paged.py    formulas in float64 of the decode step around the experts (page
+              plan, norm and rotation, attention, log probabilities).
 """
