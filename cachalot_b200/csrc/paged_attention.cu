@@ -137,6 +137,9 @@ int sm_count() {  // of the current device; an attribute of the device, asked fo
 
 size_t up(size_t v) { return (v + 255) / 256 * 256; }
 
+// CTAs of one warp: as many warps as in CTAs of four
+void make_one_warp(AttendLaunch* l) { l->ctas_per_sm *= PA_WARPS, l->step /= PA_WARPS; }
+
 size_t workspace_of(const AttendLaunch& l, int dim, int ctas) {
   return up((size_t)ctas * 2 * sizeof(int4)) + up((size_t)ctas * 2 * l.unit_heads * sizeof(float2)) + (size_t)ctas * 2 * l.unit_heads * dim * sizeof(float);
 }
@@ -149,6 +152,7 @@ using namespace cachalot;
 extern "C" size_t cachalot_paged_attention_workspace_bytes(int heads, int kv_heads, int head_dim, int cache_dtype) {
   AttendLaunch l;
   if (heads <= 0 || kv_heads <= 0 || heads % kv_heads || !shape_of(cache_dtype == CACHALOT_E4M3, head_dim, heads / kv_heads, &l)) return 0;
+  if (l.tiles == 1 && l.unit_heads <= 16) make_one_warp(&l);  // whichever form a call takes
   return workspace_of(l, head_dim, sm_count() * l.ctas_per_sm);
 }
 
@@ -177,13 +181,23 @@ extern "C" int cachalot_paged_attention(const void* q, int64_t q_row_stride, int
   if (!aligned(q, 4) || q_row_stride % 2 || q_head_stride % 2) return fail(CACHALOT_EALIGN, "paged_attention: query heads need 4-byte alignment");
   if (requests > 1 && table_stride < width) return fail(CACHALOT_EINVAL, "paged_attention: block table rows overlap");
   if (!aligned(workspace, 256)) return fail(CACHALOT_EALIGN, "paged_attention: workspace needs 256-byte alignment");
+  // CTAs of one warp where every CTA of four would begin more than one unit and no request is long: the four warps meet three
+  // times for every unit, and what a unit costs besides its tokens (7 us) is then paid by one warp, not by four.  Heads of
+  // 128, 8 heads to each of 8 key-value heads, one against four warps (us), bf16 and E4M3: 500 requests of up to 60 tokens 27
+  // and 48, 35 and 56; 2000 86 and 182, 113 and 218; 160 of up to 400 22 and 29, 24 and 30; of up to 800 55 and 57, 45 and 52;
+  // of up to 3000 57 and 54, 44 and 50; of up to 16000 188 and 170, 108 and 105 (more parts to join); with fewer units, 40
+  // requests of up to 200, 12.8 and 11.4, 13.7 and 11.8.
+  const long long units = (long long)requests * a.c.kv_heads * l.head_blocks, table_room = (long long)width * a.c.page_size;
+  const long long reach = window > 0 && window < table_room ? window : table_room;
+  a.one_warp = l.tiles == 1 && l.unit_heads <= 16 && a.c.page_size % 8 == 0 && units > sm_count() * l.ctas_per_sm && reach <= (f8 ? 4096 : 1024);
+  const int cost_share = a.one_warp ? PA_WARPS : 1;
+  if (a.one_warp) make_one_warp(&l);
   const int most = sm_count() * l.ctas_per_sm;
   if (workspace_bytes < workspace_of(l, a.c.head_dim, most))
     return fail(CACHALOT_ESCRATCH, "paged_attention: workspace of %zu bytes, %zu needed", workspace_bytes, workspace_of(l, a.c.head_dim, most));
   a.q = q, a.q_row = q_row_stride, a.q_head = q_head_stride, a.q_bf16 = q_dtype == CACHALOT_BF16;
   a.table = block_table, a.table_stride = table_stride, a.lens = lens;
-  const long long room = (long long)width * a.c.page_size;
-  a.room = room < 0x7fffff00LL ? (int)room : 0x7fffff00;
+  a.room = table_room < 0x7fffff00LL ? (int)table_room : 0x7fffff00;
   a.requests = requests, a.heads = heads, a.group = heads / a.c.kv_heads, a.tiles = l.tiles, a.head_blocks = l.head_blocks;
   a.page_shift = -1;
   for (int s = 0; s < 28; ++s)
@@ -194,8 +208,8 @@ extern "C" int cachalot_paged_attention(const void* q, int64_t q_row_stride, int
   // 48 KB: two steps of 128-element heads (a batch of very different lengths 44.7 us, with three 46.2); with two CTAs per SM, each
   // of which gets more of the bandwidth, 96 KB (16 heads to a key-value head 105 us, with 48 KB 113); over an E4M3 cache,
   // where instructions count for more than bytes, 384 tokens: three steps (batch of 64: 7 us less than with two)
-  const int cost_bytes = l.ctas_per_sm > 2 ? 48 * 1024 : 96 * 1024;
-  a.unit_cost = f8 ? (384 + l.step - 1) / l.step : (cost_bytes + step_bytes - 1) / step_bytes;
+  const int cost_bytes = (l.ctas_per_sm / cost_share > 2 ? 48 * 1024 : 96 * 1024) / cost_share;
+  a.unit_cost = f8 ? (384 / cost_share + l.step - 1) / l.step : (cost_bytes + step_bytes - 1) / step_bytes;
   a.scale = scale, a.softcap = softcap, a.window = window, a.out = out, a.out_dtype = out_dtype, a.lse = lse, a.status = status;
   uint8_t* w = static_cast<uint8_t*>(workspace);
   a.parts = reinterpret_cast<int4*>(w), w += up((size_t)most * 2 * sizeof(int4));

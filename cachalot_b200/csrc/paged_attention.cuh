@@ -16,7 +16,7 @@
 //   * S^T fragments become P^T fragments by one movmatrix each.
 //   * the running maximum moves only when a score exceeds it by more than 2^8 (one vote per tile instead of six shuffles
 //     and a rescaling); P stays below 2^8 in bf16, and is shifted by 2^7 in f16 to use that type's range.
-// Work is cut on the device, where the lengths are: the steps (a tile for each warp, of one request and key-value head) of the whole
+// Work is cut on the device, where the lengths are: the steps (a tile for each of a CTA's warps, of one request and key-value head) of the whole
 // batch are laid on a line and every CTA takes an equal run of it, so a batch of very different lengths is balanced
 // and one long request fills the GPU.  A unit (request, head) also occupies what it costs to begin one (query, first
 // page, empty pipeline, merge: as long as 48 or 96 KB of keys and values, or 384 tokens of E4M3; without that, CTAs with many short requests
@@ -28,7 +28,7 @@
 
 namespace cachalot {
 
-constexpr int PA_THREADS = 128, PA_WARPS = 4;
+constexpr int PA_THREADS = 128, PA_WARPS = 4;  // of a CTA; of one warp where short requests are many
 
 struct AttendArgs {
   const void* q;
@@ -43,6 +43,7 @@ struct AttendArgs {
   int tiles, head_blocks;          // head tiles (of 8 NT heads) a CTA's warps are split over; units per key-value head
   int page_shift;                  // log2(page_size / 8) or -1; tokens one by one where the page size is no multiple of 8
   uint64_t page_magic;             // ceil(2^35 / (page_size / 8)) for page sizes below 1024, else 0
+  int one_warp;                    // CTAs of one warp (one head tile, pages of 8 k tokens)
   int unit_cost;                   // what beginning a unit costs, in steps
   float scale, softcap;
   int window;
@@ -123,7 +124,7 @@ __device__ __forceinline__ void load_words(uint32_t (&r)[W], const uint8_t* p) {
 }
 
 // Geometry of one instantiation: what a lane holds of a key row (a quarter of it) and of a value row (an eighth).
-template <bool F8, int D, int NT>
+template <bool F8, int D, int NT, int W>
 struct AttendShape {
   static constexpr int ES = F8 ? 1 : 2;
   static constexpr int KBYTES = D * ES / 4, VBYTES = D * ES / 8;
@@ -133,7 +134,7 @@ struct AttendShape {
   // MMA tiles of 16 tokens that a warp works on at a time.  (E4M3 with several column tiles: one tile and three CTAs per SM 141 us,
   // two and two 168 us, batch of 64 with 16 heads of 128 to a key-value head.)
   static constexpr int U = D * ES <= 128 && !(F8 && NT > 1 && D > 64) ? 2 : 1;
-  static constexpr int TILE = 16 * U, STEP = PA_WARPS * TILE;
+  static constexpr int TILE = 16 * U, STEP = W * TILE;
   static constexpr int KSTEPS = D / 16;                 // MMAs over the head's elements = MMA row tiles of O^T
   static constexpr int TILE_HEADS = 8 * NT;
   static constexpr int O_PITCH = D + 4;
@@ -141,24 +142,27 @@ struct AttendShape {
   static constexpr __host__ __device__ int k_dim(int w, int t) { return (w / (KB / 4) * (4 * KB) + t * KB + w % (KB / 4) * 4) / ES; }
   static constexpr __host__ __device__ int v_dim(int w, int g) { return (w / (VB / 4) * (8 * VB) + g * VB + w % (VB / 4) * 4) / ES; }
   static constexpr int Q_BYTES(int tiles) { return tiles * NT * KSTEPS * 32 * 8; }
-  static constexpr int SMEM(int tiles) { return Q_BYTES(tiles) + PA_WARPS * TILE_HEADS * (O_PITCH * 4 + 8) + 4 * TILE_HEADS * 4; }
+  static constexpr int SMEM(int tiles) { return Q_BYTES(tiles) + W * TILE_HEADS * (O_PITCH * 4 + 8) + 4 * TILE_HEADS * 4; }
   static constexpr int MAX_TILES = 4;
   // CTAs per SM that the registers are cut for
-  static constexpr int CTAS = D * NT <= 64 ? 4 : D * NT <= 128 || (F8 && NT > 1 && D * NT <= 256) ? 3 : 2;
+  static constexpr int CTAS = PA_WARPS / W * (D * NT <= 64 ? 4 : D * NT <= 128 || (F8 && NT > 1 && D * NT <= 256) ? 3 : 2);
 };
 
 struct Span {  // what is visible of a request
   int lo, len, first_tile, steps;
 };
 template <typename S>
-__device__ __forceinline__ Span span_of(const AttendArgs& a, int r) {
+__device__ __forceinline__ Span span_of_length(const AttendArgs& a, int length) {
   Span s;
-  s.len = min(max(a.lens[r], 0), a.room);
+  s.len = min(max(length, 0), a.room);
   s.lo = a.window > 0 ? max(0, s.len - a.window) : 0;
   s.first_tile = s.lo / S::TILE;
   s.steps = s.len > 0 ? (s.len - s.first_tile * S::TILE + S::STEP - 1) / S::STEP : 0;
   return s;
 }
+
+template <typename S>
+__device__ __forceinline__ Span span_of(const AttendArgs& a, int r) { return span_of_length<S>(a, a.lens[r]); }
 
 // Division by a number that stays the same, of dividends below 2^53 (a 64-bit division takes a thousand cycles).
 struct Divisor {
@@ -190,18 +194,18 @@ __device__ __forceinline__ void store_out4(void* out, int dtype, long long at, f
   }
 }
 
-template <typename M, bool F8, int D, int NT, bool PAGE8, bool KEEP>
-__global__ void __launch_bounds__(PA_THREADS, AttendShape<F8, D, NT>::CTAS) attend_kernel(const AttendArgs a) {
-  using S = AttendShape<F8, D, NT>;
+template <typename M, bool F8, int D, int NT, bool PAGE8, bool KEEP, int W>
+__global__ void __launch_bounds__(W * 32, AttendShape<F8, D, NT, W>::CTAS) attend_kernel(const AttendArgs a) {
+  using S = AttendShape<F8, D, NT, W>;
   constexpr bool HALF = std::is_same<M, __half>::value;
   constexpr float SHIFT = HALF ? 7.f : 0.f, SLACK = 8.f;
   constexpr int TERMS = F8 ? 1 : 2;  // of P
   extern __shared__ __align__(16) uint8_t smem[];
   uint2* sq = reinterpret_cast<uint2*>(smem);                                        // [tiles * NT][KSTEPS][32]
   float* so = reinterpret_cast<float*>(smem + S::Q_BYTES(a.tiles));                  // [warps][TILE_HEADS][O_PITCH]
-  float2* sml = reinterpret_cast<float2*>(so + PA_WARPS * S::TILE_HEADS * S::O_PITCH);  // [warps][TILE_HEADS]
-  float* sexp = reinterpret_cast<float*>(sml + PA_WARPS * S::TILE_HEADS);            // [tiles * TILE_HEADS] scale of the query
-  __shared__ long long sums[PA_WARPS];
+  float2* sml = reinterpret_cast<float2*>(so + W * S::TILE_HEADS * S::O_PITCH);  // [warps][TILE_HEADS]
+  float* sexp = reinterpret_cast<float*>(sml + W * S::TILE_HEADS);            // [tiles * TILE_HEADS] scale of the query
+  __shared__ long long sums[W];
   __shared__ long long shared_found_at;
   __shared__ int shared_found;
 
@@ -211,11 +215,9 @@ __global__ void __launch_bounds__(PA_THREADS, AttendShape<F8, D, NT>::CTAS) atte
   int flags = 0;
 
   // ---- which part of the line is this CTA's ----
-  auto cost_of = [&](int r) {
-    if (r >= a.requests) return 0LL;
-    const int n = a.lens[r];
+  auto cost_of = [&](int n) {  // of a request of n tokens
     if (n < 0 || n > a.room) flags |= CACHALOT_STATUS_LENGTH;
-    const int steps = span_of<S>(a, r).steps;
+    const int steps = span_of_length<S>(a, n).steps;
     return steps ? (long long)(steps + a.unit_cost) * per_request : 0LL;
   };
   auto scan = [&](long long v) {  // inclusive, over the warp
@@ -233,35 +235,34 @@ __global__ void __launch_bounds__(PA_THREADS, AttendShape<F8, D, NT>::CTAS) atte
     begin = per * blockIdx.x;
   };
   if (a.requests <= 32) {  // every warp for itself
-    const long long own = cost_of(lane), end = scan(own);
+    const long long own = cost_of(lane < a.requests ? a.lens[lane] : 0), end = scan(own);
     total = __shfl_sync(0xffffffffu, end, 31);
     cut();
     const unsigned here = __ballot_sync(0xffffffffu, begin >= end - own && begin < end);
     if (here) found = __ffs(here) - 1, found_at = __shfl_sync(0xffffffffu, end - own, found);
   } else {
-    for (int r = tid; r < a.requests; r += PA_THREADS) total += cost_of(r);
-    total = __shfl_sync(0xffffffffu, scan(total), 31);
-    if (lane == 0) sums[warp] = total;
+    // a thread has `each` requests in a row; eight loads at a time
+    const int each = (a.requests + W * 32 - 1) / (W * 32), r0 = tid * each;
+    long long own = 0;
+    for (int i0 = 0; i0 < each; i0 += 8) {
+      int n[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) n[i] = i0 + i < each && r0 + i0 + i < a.requests ? a.lens[r0 + i0 + i] : 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) own += cost_of(n[i]);
+    }
+    long long end = scan(own);
+    if (lane == 31) sums[warp] = end;
     if (tid == 0) shared_found = -1;
     __syncthreads();
-    total = 0;
 #pragma unroll
-    for (int w = 0; w < PA_WARPS; ++w) total += sums[w];
+    for (int w = 0; w < W; ++w) total += sums[w], end += w < warp ? sums[w] : 0;
     cut();
-    long long before = 0;
-    for (int r0 = 0; r0 < a.requests && begin < total; r0 += PA_THREADS) {
-      const long long own = cost_of(r0 + tid);
-      long long end = scan(own);
-      __syncthreads();
-      if (lane == 31) sums[warp] = end;
-      __syncthreads();
-#pragma unroll
-      for (int w = 0; w < PA_WARPS; ++w) end += w < warp ? sums[w] : 0;
-      end += before;
-      if (begin >= end - own && begin < end) shared_found = r0 + tid, shared_found_at = end - own;
-#pragma unroll
-      for (int w = 0; w < PA_WARPS; ++w) before += sums[w];
-      if (before > begin) break;
+    if (begin >= end - own && begin < end) {
+      int r = r0;
+      long long from = end - own;
+      for (long long c; begin >= from + (c = cost_of(a.lens[r])); ++r) from += c;
+      shared_found = r, shared_found_at = from;
     }
     __syncthreads();
     found = shared_found, found_at = shared_found_at;
@@ -271,7 +272,7 @@ __global__ void __launch_bounds__(PA_THREADS, AttendShape<F8, D, NT>::CTAS) atte
   const Divisor by_per(per);
   const int near_end = (int)max(min((long long)a.unit_cost, per / 4), 1LL);  // a cut is at least that many steps inside a unit
 
-  const int mt = warp % a.tiles, slice = warp / a.tiles, slices = PA_WARPS / a.tiles;
+  const int mt = W == 1 ? 0 : warp % a.tiles, slice = W == 1 ? 0 : warp / a.tiles, slices = W == 1 ? 1 : W / a.tiles;
   const int unit_heads = a.tiles * S::TILE_HEADS;
   int r = max(found, 0);
   Span sp = span_of<S>(a, r);
@@ -304,7 +305,7 @@ __global__ void __launch_bounds__(PA_THREADS, AttendShape<F8, D, NT>::CTAS) atte
     const uint32_t k_page = (uint32_t)a.c.k_page, k_token = (uint32_t)a.c.k_token, v_page = (uint32_t)a.c.v_page, v_token = (uint32_t)a.c.v_token;
     const uint8_t *klane = kbase + (uint64_t)(uint32_t)g * k_token, *vlane = vbase + (uint64_t)(uint32_t)(2 * t4) * v_token;
     const int32_t* pages = a.table + r * a.table_stride;
-    const int tile_end = min(sp.first_tile + (step0 + steps) * PA_WARPS, (sp.len + S::TILE - 1) / S::TILE);
+    const int tile_end = min(sp.first_tile + (step0 + steps) * W, (sp.len + S::TILE - 1) / S::TILE);
     uint32_t kr[S::U][2][S::KW], vr[S::U][4][S::VW];
 
     // page of a token, -1 where the table names none of the cache's
@@ -397,7 +398,7 @@ __global__ void __launch_bounds__(PA_THREADS, AttendShape<F8, D, NT>::CTAS) atte
       }
     };
 
-    int tile = sp.first_tile + step0 * PA_WARPS + slice;
+    int tile = sp.first_tile + step0 * W + slice;
     Place next;
     if (tile < tile_end) {  // on their way while the queries are laid out
       const Place p = locate(tile);
@@ -407,13 +408,13 @@ __global__ void __launch_bounds__(PA_THREADS, AttendShape<F8, D, NT>::CTAS) atte
 
     // ---- the query heads as MMA fragments ----
     if constexpr (F8) {  // f16 from here on: a bf16 head is brought into range by a power of two
-      for (int i0 = warp; i0 < unit_heads; i0 += 4 * PA_WARPS) {  // four heads' loads at a time
+      for (int i0 = warp; i0 < unit_heads; i0 += 4 * W) {  // four heads' loads at a time
         float top[4] = {};
         if (a.q_bf16) {
           uint32_t x[4][(D + 63) / 64];
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            const int i = min(i0 + j * PA_WARPS, heads - 1);
+            const int i = min(i0 + j * W, heads - 1);
             const uint16_t* q = static_cast<const uint16_t*>(a.q) + r * a.q_row + (long long)(h * a.group + head0 + i) * a.q_head;
 #pragma unroll
             for (int c = 0; c < (D + 63) / 64; ++c) {
@@ -432,18 +433,18 @@ __global__ void __launch_bounds__(PA_THREADS, AttendShape<F8, D, NT>::CTAS) atte
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const int e = (int)((__float_as_uint(top[j]) >> 23) & 255) - 127;
-          if (lane == 0 && i0 + j * PA_WARPS < unit_heads) sexp[i0 + j * PA_WARPS] = top[j] > 0.f ? pow2f(max(-126, min(126, e))) : 1.f;
+          if (lane == 0 && i0 + j * W < unit_heads) sexp[i0 + j * W] = top[j] > 0.f ? pow2f(max(-126, min(126, e))) : 1.f;
         }
       }
       __syncthreads();
     }
     // Several loads of a thread in flight: one at a time, 161 requests of 2 tokens with 52 heads took 25.8 us, not 20.8.
-    constexpr int BATCH = NT * S::KSTEPS >= 16 ? 8 : (NT * S::KSTEPS + 1) / 2;
-    for (int i0 = tid; i0 < a.tiles * NT * S::KSTEPS * 32; i0 += BATCH * PA_THREADS) {
+    constexpr int BATCH = NT * S::KSTEPS * PA_WARPS / W >= 16 ? 8 : (NT * S::KSTEPS + 1) / 2;
+    for (int i0 = tid; i0 < a.tiles * NT * S::KSTEPS * 32; i0 += BATCH * W * 32) {
       uint2 f[BATCH];
 #pragma unroll
       for (int j = 0; j < BATCH; ++j) {
-        const int i = i0 + j * PA_THREADS, l = i & 31, ks = (i >> 5) % S::KSTEPS, head = (i >> 5) / S::KSTEPS * 8 + (l >> 2);
+        const int i = i0 + j * W * 32, l = i & 31, ks = (i >> 5) % S::KSTEPS, head = (i >> 5) / S::KSTEPS * 8 + (l >> 2);
         const int d0 = F8 ? S::k_dim(ks, l & 3) : S::k_dim(2 * ks, l & 3), d1 = F8 ? d0 + 2 : S::k_dim(2 * ks + 1, l & 3);
         f[j] = make_uint2(0, 0);
         if (head < heads) {
@@ -453,7 +454,7 @@ __global__ void __launch_bounds__(PA_THREADS, AttendShape<F8, D, NT>::CTAS) atte
       }
 #pragma unroll
       for (int j = 0; j < BATCH; ++j) {
-        const int i = i0 + j * PA_THREADS, head = (i >> 5) / S::KSTEPS * 8 + ((i & 31) >> 2);
+        const int i = i0 + j * W * 32, head = (i >> 5) / S::KSTEPS * 8 + ((i & 31) >> 2);
         if (i >= a.tiles * NT * S::KSTEPS * 32) break;
         if (F8 && a.q_bf16) {
           const float inv = 1.f / sexp[head];  // a power of two
@@ -627,7 +628,7 @@ __global__ void __launch_bounds__(PA_THREADS, AttendShape<F8, D, NT>::CTAS) atte
       for (int c = 0; c < 2; ++c) {
         const int row = n * 8 + 2 * t4 + c;
         float top = -INFINITY;
-        for (int w = mt; w < PA_WARPS; w += a.tiles) top = fmaxf(top, sml[w * S::TILE_HEADS + row].x);
+        for (int w = mt; w < W; w += a.tiles) top = fmaxf(top, sml[w * S::TILE_HEADS + row].x);
         const float f = m[n][c] == -INFINITY ? 0.f : ex2(m[n][c] - top);
         float* dst = so + (warp * S::TILE_HEADS + row) * S::O_PITCH;
 #pragma unroll
@@ -644,13 +645,13 @@ __global__ void __launch_bounds__(PA_THREADS, AttendShape<F8, D, NT>::CTAS) atte
     const int which = cta == c0 ? 1 : 0;
     const long long slot = (long long)blockIdx.x * 2 + which;
     const float v_scale = F8 && a.c.v_scale ? a.c.v_scale[h] : 1.f;
-    for (int i = tid; i < heads * (D / 4); i += PA_THREADS) {
+    for (int i = tid; i < heads * (D / 4); i += W * 32) {
       const int head = i / (D / 4), d = i % (D / 4) * 4;
       const int row = head % S::TILE_HEADS, from = head / S::TILE_HEADS;
       float top = -INFINITY, sum = 0.f;
-      for (int w = from; w < PA_WARPS; w += a.tiles) top = fmaxf(top, sml[w * S::TILE_HEADS + row].x);
+      for (int w = from; w < W; w += a.tiles) top = fmaxf(top, sml[w * S::TILE_HEADS + row].x);
       float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-      for (int w = from; w < PA_WARPS; w += a.tiles) {
+      for (int w = from; w < W; w += a.tiles) {
         const float2 ml = sml[w * S::TILE_HEADS + row];
         sum += ml.x == -INFINITY ? 0.f : ml.y * ex2(ml.x - top);
         const float4 x = *reinterpret_cast<const float4*>(so + (w * S::TILE_HEADS + row) * S::O_PITCH + d);
@@ -673,9 +674,9 @@ __global__ void __launch_bounds__(PA_THREADS, AttendShape<F8, D, NT>::CTAS) atte
   // ---- rows without a visible key ----
   for (int r = blockIdx.x; r < a.requests; r += gridDim.x) {
     if (span_of<S>(a, r).steps) continue;
-    for (int i = tid; i < a.heads * D; i += PA_THREADS) store_out(a.out, a.out_dtype, (long long)r * a.heads * D + i, 0.f);
+    for (int i = tid; i < a.heads * D; i += W * 32) store_out(a.out, a.out_dtype, (long long)r * a.heads * D + i, 0.f);
     if (a.lse)
-      for (int i = tid; i < a.heads; i += PA_THREADS) a.lse[(long long)r * a.heads + i] = -INFINITY;
+      for (int i = tid; i < a.heads; i += W * 32) a.lse[(long long)r * a.heads + i] = -INFINITY;
   }
   if (a.status && flags) atomicOr(a.status, flags);
 }
@@ -691,7 +692,7 @@ AttendLaunch attend_shape(int group) {
   l.tiles = need >= 3 ? 4 : need;
   l.unit_heads = l.tiles * 8 * NT;
   l.head_blocks = (group + l.unit_heads - 1) / l.unit_heads;
-  l.ctas_per_sm = AttendShape<F8, D, NT>::CTAS, l.step = AttendShape<F8, D, NT>::STEP;
+  l.ctas_per_sm = AttendShape<F8, D, NT, PA_WARPS>::CTAS, l.step = AttendShape<F8, D, NT, PA_WARPS>::STEP;
   return l;
 }
 // Column tiles of 8 query heads per warp: as few warps as possible read the same keys, up to three tiles where the registers hold
@@ -728,15 +729,20 @@ int launch_attend(AttendArgs& a, int dim, int ctas, cudaStream_t stream) {
   cudaError_t e = cudaSuccess;
   attend_dispatch<F8>(dim, a.group, [&](auto d, auto nt, const AttendLaunch& l) {
     constexpr int D = decltype(d)::value, NT = decltype(nt)::value;
-    using S = AttendShape<F8, D, NT>;
-    auto run = [&](auto kern) {
-      e = smem_optin_once(kern, S::SMEM(S::MAX_TILES));
-      if (e == cudaSuccess) e = launch_early(kern, dim3(ctas), PA_THREADS, S::SMEM(l.tiles), stream, 1, a);
+    auto run = [&](auto kern, auto warps) {
+      constexpr int W = decltype(warps)::value;
+      using S = AttendShape<F8, D, NT, W>;
+      e = smem_optin_once(kern, S::SMEM(W == 1 ? 1 : S::MAX_TILES));
+      if (e == cudaSuccess) e = launch_early(kern, dim3(ctas), W * 32, S::SMEM(l.tiles), stream, 1, a);
     };
+    using std::integral_constant;
+    constexpr auto all = integral_constant<int, PA_WARPS>{};
     const bool page8 = a.c.page_size % 8 == 0;
-    if (page8 && l.tiles == 1) run(attend_kernel<M, F8, D, NT, true, false>);
-    else if (page8) run(attend_kernel<M, F8, D, NT, true, true>);
-    else run(attend_kernel<M, F8, D, NT, false, true>);
+    if constexpr (NT <= 2)
+      if (a.one_warp) return run(attend_kernel<M, F8, D, NT, true, false, 1>, integral_constant<int, 1>{});
+    if (page8 && l.tiles == 1) run(attend_kernel<M, F8, D, NT, true, false, PA_WARPS>, all);
+    else if (page8) run(attend_kernel<M, F8, D, NT, true, true, PA_WARPS>, all);
+    else run(attend_kernel<M, F8, D, NT, false, true, PA_WARPS>, all);
   });
   if (e != cudaSuccess) return fail(CACHALOT_ECUDA, "paged_attention: %s", cudaGetErrorString(e));
   return check_launch("paged_attention");

@@ -131,6 +131,21 @@ def test_groups_of_other_head_sizes(group, dim, cache):
     Case([1, 40, 200, 0], 2 * group, 2, dim, 16, BF16, cache, seed=group).check()
 
 
+@pytest.mark.parametrize("dtype,cache", [(BF16, BF16), (F16, F16), (BF16, E4M3), (F16, E4M3)])
+@pytest.mark.parametrize("dim,group", [(64, 8), (96, 3), (128, 1), (128, 13), (192, 9), (256, 16)])
+def test_many_short_requests(dim, group, dtype, cache):
+    lens = (EDGES * 6)[:80]
+    Case(lens, 8 * group, 8, dim, 16, dtype, cache, seed=dim).check()
+    Case(lens, 8 * group, 8, dim, 24, dtype, cache, seed=dim).check(window=33, softcap=20.0)
+
+
+def test_more_requests_than_a_warp_adds_up_at_once():
+    lens = [(i * 37) % 23 for i in range(700)]
+    Case(lens, 8, 2, 64, 8, BF16, BF16, seed=3).check()
+    Case([0] * 600 + [5] + [0] * 99 + [300], 8, 2, 64, 8, BF16, E4M3, seed=3).check()
+    Case([0, 1, 2] * 800, 2, 2, 64, 8, F16, F16, seed=3).check()
+
+
 @pytest.mark.parametrize("page", [1, 3, 8, 16, 24, 32, 40, 64, 100, 256])
 @pytest.mark.parametrize("order", ["heads", "tokens"])
 def test_pages(page, order):
