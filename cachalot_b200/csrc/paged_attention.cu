@@ -189,7 +189,8 @@ extern "C" int cachalot_paged_attention(const void* q, int64_t q_row_stride, int
   // requests of up to 200, 12.8 and 11.4, 13.7 and 11.8.
   const long long units = (long long)requests * a.c.kv_heads * l.head_blocks, table_room = (long long)width * a.c.page_size;
   const long long reach = window > 0 && window < table_room ? window : table_room;
-  a.one_warp = l.tiles == 1 && l.unit_heads <= 16 && a.c.page_size % 8 == 0 && units > sm_count() * l.ctas_per_sm && reach <= (f8 ? 4096 : 1024);
+  a.one_warp = l.tiles == 1 && l.unit_heads <= 16 && a.c.page_size % 8 == 0 && units > sm_count() * l.ctas_per_sm &&
+               reach <= (f8 ? 4096 : 1024);
   const int cost_share = a.one_warp ? PA_WARPS : 1;
   if (a.one_warp) make_one_warp(&l);
   const int most = sm_count() * l.ctas_per_sm;

@@ -304,6 +304,20 @@ def test_same_bits_every_time():
         assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
 
 
+def test_many_requests_replayed_with_other_lengths():
+    """The form of the call is chosen by what the table holds; the lengths may become anything up to that."""
+    c = Case([160] * 90, 32, 8, 64, 16, seed=9)
+    c.run()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out, lse = c.run(want_lse=True)
+    for lens in ([160] * 90, [0] * 90, [(7 * i) % 161 for i in range(90)], [0] * 89 + [160]):
+        c.lens.copy_(_int(lens))
+        g.replay()
+        torch.cuda.synchronize()
+        c.compare(out, lse, c.want())
+
+
 def test_graphs_and_streams():
     """Two captured calls replayed at the same time on two streams, with lengths that changed after the capture."""
     a, b = Case([3000, 100], 16, 2, 128, 16, seed=1), Case([10, 4000], 16, 2, 128, 16, BF16, E4M3, seed=2)
