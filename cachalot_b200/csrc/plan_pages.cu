@@ -145,7 +145,7 @@ extern "C" int cachalot_plan_pages(const int32_t* context_lens, const int32_t* n
   PlanArgs a{context_lens, new_lens, block_table, table_stride, free_pages, free_count, requests, width, n_free, page_size, tokens,
              starts, request_of, positions, slots, lens, free_count_out, status};
   const size_t smem = (2 * (size_t)requests + 1) * sizeof(int);
-  if (smem > 48 * 1024) {
+  if (smem > 40 * 1024) {  // without it 48 KB is the limit, of these and of the kernel's static arrays together
     const cudaError_t e = smem_optin_once(plan_pages_kernel, (2 * PP_MAX_REQUESTS + 1) * (int)sizeof(int));
     if (e != cudaSuccess) return fail(CACHALOT_ECUDA, "plan_pages: %s", cudaGetErrorString(e));
   }

@@ -1,4 +1,8 @@
 """GPU parity: the page plan against its definition in Python integers."""
+import pathlib
+import subprocess
+import sys
+
 import numpy as np
 import pytest
 
@@ -121,3 +125,12 @@ def test_refusals():
     with pytest.raises(NotImplementedError, match="8193 requests"):
         many = torch.zeros(8193, dtype=torch.int32, device="cuda")
         cb.plan_pages(many, many, torch.zeros((8193, 1), dtype=torch.int32, device="cuda"), free, count, **ok)
+
+
+def test_requests_around_the_default_shared_memory_limit():
+    """Each in a process of its own: a larger call before it would have raised the kernel's limit for good."""
+    root = pathlib.Path(__file__).resolve().parents[1]
+    code = "import sys; sys.path[:0] = ['.', 'tests']; import test_gpu_plan_pages as t; n = int(sys.argv[1]); t._check([i % 40 for i in range(n)], [i % 3 for i in range(n)], 16, n + 9, 4, n)"
+    for n in (6135, 6136, 6143, 6144):
+        run = subprocess.run([sys.executable, "-c", code, str(n)], cwd=root, capture_output=True, text=True, timeout=300)
+        assert run.returncode == 0, (n, run.stderr[-2000:])
