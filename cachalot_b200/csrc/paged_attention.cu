@@ -25,6 +25,7 @@ struct JoinArgs {
 template <int E>
 struct Joined {
   float m = -INFINITY, l = 0.f, v[E] = {};
+  // (a part without a maximum has a sum of 0, or of NaN, which 0 * NaN carries on)
   __device__ __forceinline__ void add(float om, float ol, const float (&o)[E]) {
     const float top = fmaxf(m, om), f = m == -INFINITY ? 0.f : ex2(m - top), g = om == -INFINITY ? 0.f : ex2(om - top);
     m = top, l = l * f + ol * g;

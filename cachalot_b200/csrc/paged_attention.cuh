@@ -653,7 +653,7 @@ __global__ void __launch_bounds__(W * 32, AttendShape<F8, D, NT, W>::CTAS) atten
       float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
       for (int w = from; w < W; w += a.tiles) {
         const float2 ml = sml[w * S::TILE_HEADS + row];
-        sum += ml.x == -INFINITY ? 0.f : ml.y * ex2(ml.x - top);
+        sum += ml.x == -INFINITY ? ml.y : ml.y * ex2(ml.x - top);  // no maximum: 0, or NaN where all its scores are
         const float4 x = *reinterpret_cast<const float4*>(so + (w * S::TILE_HEADS + row) * S::O_PITCH + d);
         v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
       }

@@ -418,7 +418,8 @@ CACHALOT_API int cachalot_qk_norm_rope(const void* q, int64_t q_token_stride, in
  * contiguous in out_dtype, lse f32 [requests, heads] or NULL; query head i reads key-value head i / (heads / kv_heads).
  * The cache holds q's type or E4M3.  Everything between the products is fp32; softmax weights enter the second one with 16
  * bits (bf16 cache), 22 (f16) or 11 (E4M3).  What lies behind a length or on hidden pages may be anything, NaN too; a visible
- * value that is not finite makes its element NaN or infinite for the heads that see it.  block_table i32 [requests, width], rows table_stride apart; lens i32 [requests].  A request without a visible
+ * value that is not finite makes its element NaN or infinite for the heads that see it; a score that is NaN (a NaN in the query or
+ * in a visible key) makes its head's elements and lse NaN.  block_table i32 [requests, width], rows table_stride apart; lens i32 [requests].  A request without a visible
  * key gets zeros and -inf.  A length past its table is cut, a negative one counts as 0 (CACHALOT_STATUS_LENGTH); tokens on
  * a page outside [0, n_pages) are hidden (CACHALOT_STATUS_SLOT_RANGE); pages that no visible token lies on are not looked at.
  * head_dim 64, 96, 128, 192 or 256.  workspace: cachalot_paged_attention_workspace_bytes() bytes, 256-byte aligned, not

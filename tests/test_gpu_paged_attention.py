@@ -369,3 +369,57 @@ def test_refusals():
     n = torch.zeros((2, 2, 16, 48), dtype=BF16, device="cuda")
     with pytest.raises(NotImplementedError, match="head size 48"):
         cb.paged_attention(torch.zeros((2, 4, 48), dtype=BF16, device="cuda"), n, n.clone(), c.table, c.lens)
+
+
+NAN_CACHES = [(BF16, BF16), (F16, F16), (BF16, E4M3), (F16, E4M3)]
+
+
+def _set_keys(c, request, tokens, head, value):
+    """Element 5 of these keys of one key-value head."""
+    at = c.table[request].long()
+    raw = c.caches[0].view(torch.uint8) if c.caches[0].dtype == E4M3 else c.caches[0]
+    raw[at[tokens // c.page], head, tokens % c.page, 5] = (0x7F if c.caches[0].dtype == E4M3 else value)
+
+
+def _nan_where(c, hit, **kw):
+    """NaN for these (request, head) pairs, in every element and in the log sum exp; returns what the call gave."""
+    out, lse = c.run(want_lse=True, **kw)
+    assert out[hit].isnan().all() and lse[hit].isnan().all()
+    return out, lse
+
+
+# a unit of a CTA, of several, of CTAs of one warp; a last tile of one token
+NAN_LENS = {"whole": [40, 1, 65, 0], "joined": [20001, 33], "one warp": [i % 50 for i in range(90)]}
+
+
+@pytest.mark.parametrize("lens", NAN_LENS)
+@pytest.mark.parametrize("dtype,cache", NAN_CACHES)
+def test_nan_in_a_query_makes_its_head_nan(dtype, cache, lens):
+    c = Case(NAN_LENS[lens], 16, 8, 64, 16, dtype, cache, hidden="")
+    for kw in ({}, dict(softcap=5.0)):
+        clean, want, keep = c.run(want_lse=True, **kw), c.want(**kw), c.q.clone()
+        c.q[0, 3, 7] = c.q[1, 9, 63] = float("nan")
+        hit = torch.zeros(c.q.shape[:2], dtype=torch.bool, device="cuda")
+        hit[0, 3], hit[1, 9] = c.lens[0] > 0, c.lens[1] > 0
+        got = _nan_where(c, hit, **kw)
+        c.q = keep
+        for a, b in zip(got, clean):  # the others are right, though not the clean call's bits: heads of a unit move their maxima together
+            a[hit] = b[hit]
+        c.compare(*got, want, kw.get("softcap", 0.0))
+
+
+@pytest.mark.parametrize("which", ["first", "last", "many", "whole tiles", "all"])
+@pytest.mark.parametrize("lens", NAN_LENS)
+@pytest.mark.parametrize("dtype,cache", NAN_CACHES)
+def test_nan_in_keys_reaches_the_log_sum_exp(dtype, cache, lens, which):
+    c = Case(NAN_LENS[lens], 16, 8, 64, 16, dtype, cache, hidden="")
+    clean = c.run(want_lse=True)
+    hit = torch.zeros(c.q.shape[:2], dtype=torch.bool, device="cuda")
+    for r, n in enumerate(NAN_LENS[lens]):
+        if r % 3 == 2 and lens == "one warp" or n == 0:
+            continue
+        tokens = torch.arange(*{"first": (0, 1), "last": (n - 1, n), "many": (n // 2, n), "whole tiles": (n // 2 // 128 * 128, n), "all": (0, n)}[which], device="cuda")
+        _set_keys(c, r, tokens, 2, float("nan"))
+        hit[r, 4:6] = True
+    got = _nan_where(c, hit)
+    assert all(torch.equal(a[~hit], b[~hit]) for a, b in zip(got, clean))
