@@ -1,6 +1,7 @@
 // Paged attention: argument checks, workspace, and the join of units that lie in several CTAs (the kernel itself:
 // paged_attention.cuh).
 #include <atomic>
+#include <cmath>
 
 #include "paged_attention.cuh"
 
@@ -170,7 +171,7 @@ extern "C" int cachalot_paged_attention(const void* q, int64_t q_row_stride, int
   if (const int rc = paged_view("paged_attention", cache, &a.c)) return rc;
   if (heads % a.c.kv_heads) return fail(CACHALOT_EINVAL, "paged_attention: %d query heads over %d key-value heads", heads, a.c.kv_heads);
   if (a.c.dtype != CACHALOT_E4M3 && a.c.dtype != q_dtype) return fail(CACHALOT_EINVAL, "paged_attention: cache and queries differ in type");
-  if (window < 0 || !(softcap >= 0.f)) return fail(CACHALOT_EINVAL, "paged_attention: window and softcap must not be negative");
+  if (window < 0 || !(softcap >= 0.f) || std::isinf(softcap)) return fail(CACHALOT_EINVAL, "paged_attention: window and softcap must be finite and not negative");
   for (long long stride : {a.c.k_page, a.c.k_token, a.c.v_page, a.c.v_token})
     if (stride > 0xffffffffLL) return fail(CACHALOT_EUNSUPPORTED, "paged_attention: pages or tokens %lld bytes apart", stride);
   const bool f8 = a.c.dtype == CACHALOT_E4M3;

@@ -412,7 +412,7 @@ CACHALOT_API int cachalot_qk_norm_rope(const void* q, int64_t q_token_stride, in
 
 /* Replaces minimax/gqa_decode.py:180-187 (grouped-query attention of a decode token): one new token per request against the
  * tokens of its pages,
- *   s_j = scale * q . k_j  (softcap > 0: softcap * tanh(s_j / softcap)),  out = softmax(s) V,  lse = log sum_j exp(s_j)
+ *   s_j = scale * q . k_j  (softcap > 0, finite: softcap * tanh(s_j / softcap)),  out = softmax(s) V,  lse = log sum_j exp(s_j)
  * over j < lens[r], with window > 0 only the last `window` of them (the new token is one of them and already in the cache).
  * q [requests, heads, head_dim] F16 or BF16 (strides in elements, 4-byte aligned), out [requests, heads, head_dim]
  * contiguous in out_dtype, lse f32 [requests, heads] or NULL; query head i reads key-value head i / (heads / kv_heads).

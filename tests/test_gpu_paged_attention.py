@@ -423,3 +423,13 @@ def test_nan_in_keys_reaches_the_log_sum_exp(dtype, cache, lens, which):
         hit[r, 4:6] = True
     got = _nan_where(c, hit)
     assert all(torch.equal(a[~hit], b[~hit]) for a, b in zip(got, clean))
+
+
+def test_an_infinite_softcap_is_refused():
+    import cachalot_b200 as cb
+
+    c = Case([5, 9], 4, 2, 64, 16)
+    for lens in (c.lens, c.lens.long()):  # the native call path and the general form
+        for cap in (float("inf"), 1e39):
+            with pytest.raises(ValueError, match="softcap"):
+                cb.paged_attention(c.q, *c.caches, c.table, lens, softcap=cap)

@@ -131,3 +131,20 @@ def test_token_logprobs_refusals():
                          (dict(x=C.c_void_p(p.value + 2)), _lib.EALIGN, "aligned")):
         assert call(**kw) == rc and word in _lib.last_error(), (kw, _lib.last_error())
     assert call(rows=0, x=None) == _lib.OK
+
+
+def test_paged_attention_refuses_an_infinite_softcap():
+    from cachalot_b200 import _lib
+
+    buf = (C.c_int32 * 4096)()
+    base = C.addressof(buf) + (-C.addressof(buf)) % 256
+    p, d = C.c_void_p(base), _lib.PagedKV()
+    d.k = d.v = base
+    d.k_page_stride = d.v_page_stride = 16 * 64
+    d.k_head_stride = d.v_head_stride = 16 * 64
+    d.k_token_stride = d.v_token_stride = 64
+    d.n_pages, d.page_size, d.kv_heads, d.head_dim, d.dtype = 2, 16, 1, 64, _lib.BF16
+    # room for no workspace: the call ends before its launch whatever it thinks of the cap
+    call = lambda cap: _lib.lib.cachalot_paged_attention(p, 64, 64, _lib.BF16, 1, 1, C.byref(d), p, 2, 2, p, 0.125, 0, cap, p, 0, p, _lib.BF16, None, None, None)  # noqa: E731
+    assert call(float("inf")) == _lib.EINVAL and "softcap" in _lib.last_error()
+    assert call(1e39) == _lib.EINVAL and call(3e38) == _lib.ESCRATCH and call(0.0) == _lib.ESCRATCH
