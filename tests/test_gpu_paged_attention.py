@@ -433,3 +433,34 @@ def test_an_infinite_softcap_is_refused():
         for cap in (float("inf"), 1e39):
             with pytest.raises(ValueError, match="softcap"):
                 cb.paged_attention(c.q, *c.caches, c.table, lens, softcap=cap)
+
+
+@pytest.mark.parametrize("softcap", [1e-3, 0.5, 8.0, 50.0, 1e3, 1e4, 1e5, 1e30, 3e38])
+@pytest.mark.parametrize("dtype,cache", [(BF16, BF16), (F16, F16), (F16, E4M3)])
+def test_softcap_is_as_accurate_as_the_scores(dtype, cache, softcap):
+    """The error that the cap adds is relative to the capped score, whatever the cap.  Up to 0.4 of the cap a series of five
+    terms: what is left out is 0.009 z^10 < 2^-19.9, its roundings (in terms of z^2 / 3 and less) below 2^-22.  Above, with x = |z|, 1 - 2 / (1 +
+    e^2x): the exponential's 2^-22 times the slope, at most 1/2; its argument, 2^-23 times x / cosh^2 x < 0.45; the sum's 2^-24 and the
+    reciprocal's 2^-23 of at most 1; the last rounding 2^-25: 2^-21.3 of the cap, which is less than 2^-19 of a score that is capped to
+    0.37 of it or more.  A capped score is below `reach`, and the derivative of the cap at most 1: reach * 2^-18 on top of what an
+    uncapped score carries."""
+    for q_scale in (2.0, 0.02):
+        c = Case([1, 2, 40, 300, 0], 6, 2, 64, 16, dtype, cache, q_scale=q_scale, seed=5)
+        for scale in (None, -0.2):
+            out, lse = c.run(want_lse=True, softcap=softcap, out_dtype=F32, scale=scale)
+            want = c.want(softcap=softcap, scale=scale)
+            c.compare(out, lse, want, want[3])
+
+
+def test_softcap_keeps_the_order_of_scores_around_the_border():
+    """Where the two forms meet, z = 0.4: one key each, so the log sum exp is the capped score itself."""
+    c = Case([1] * 64, 1, 1, 64, 16, F16)
+    c.q.zero_()
+    c.q[:, 0, 0] = torch.linspace(0.3, 0.5, 64, device="cuda").to(F16)
+    for sign in (1.0, -1.0):
+        c.caches[0].zero_()
+        c.caches[0][..., 0] = sign
+        _, lse = c.run(want_lse=True, softcap=1.0, scale=1.0)
+        want = torch.tanh(c.q[:, 0, 0].double() * sign)
+        assert ((lse[:, 0].double() - want).abs() <= 2.0 ** -18 * want.abs() + 2.0 ** -22).all()
+        assert (lse[1:, 0] * sign >= lse[:-1, 0] * sign).all()
