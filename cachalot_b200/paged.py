@@ -6,6 +6,8 @@ float8_e4m3fn (with one float32 scale per head: value = code * scale); other ord
 their own storage (`.transpose(1, 2)` of [pages, page_size, kv_heads, head_dim]).  A request's row of the block table
 names its pages in order; slot = page * page_size + place within the page.
 
+Lengths, positions, slots and ids are int32; int64 ones are narrowed (values beyond int32 become its largest or smallest).
+
 Every function here calls the C ABI; as in `ops`, calls whose arguments already have the dtype and layout the kernels take
 go through the native call path, and none has a PyTorch or CPU fallback.
 """
@@ -35,12 +37,13 @@ def _same_device(*ts) -> torch.device:
 
 
 def _ints(t: torch.Tensor, name: str, shape: tuple) -> torch.Tensor:
-    """An int32 contiguous tensor of this shape (int64 is narrowed)."""
+    """An int32 contiguous tensor of this shape.  int64 is narrowed, with values beyond int32 held at its ends: too long, past the
+    cache or past the vocabulary as before, which wrapped they might not be."""
     if t.dtype not in (torch.int32, torch.int64):
         raise ValueError(f"{name} must be int32, got {t.dtype}")
     if tuple(t.shape) != shape:
         raise ValueError(f"{name} must be {list(shape)}, got {tuple(t.shape)}")
-    return t.to(torch.int32).contiguous()
+    return (t.clamp(-2 ** 31, 2 ** 31 - 1) if t.dtype == torch.int64 else t).to(torch.int32).contiguous()
 
 
 def _status(t: torch.Tensor | None) -> None:

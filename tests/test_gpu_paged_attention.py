@@ -464,3 +464,13 @@ def test_softcap_keeps_the_order_of_scores_around_the_border():
         want = torch.tanh(c.q[:, 0, 0].double() * sign)
         assert ((lse[:, 0].double() - want).abs() <= 2.0 ** -18 * want.abs() + 2.0 ** -22).all()
         assert (lse[1:, 0] * sign >= lse[:-1, 0] * sign).all()
+
+
+def test_int64_lengths_beyond_int32():
+    import cachalot_b200 as cb
+
+    c = Case([64, 30], 4, 2, 64, 16)
+    word = _int([0])
+    out = cb.paged_attention(c.q, *c.caches, c.table, torch.tensor([2 ** 32 + 5, -2 ** 32 - 3], device="cuda"), status=word)
+    want = cb.paged_attention(c.q, *c.caches, c.table, _int([64, 0]))
+    assert torch.equal(out, want) and int(word.item()) == 32

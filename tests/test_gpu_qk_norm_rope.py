@@ -257,3 +257,14 @@ def test_refusals():
         cb.qk_norm_rope(wide, wide, pos[:1], freq)
     with pytest.raises(NotImplementedError, match="20"):
         cb.qk_norm_rope(x[..., :20].contiguous(), x[..., :20].contiguous(), pos, cb.rope_frequencies(20)[0])
+
+
+def test_int64_slots_beyond_int32():
+    import cachalot_b200 as cb
+
+    x = torch.randn((3, 2, 64), device="cuda").to(torch.bfloat16)
+    cache = [torch.zeros((2, 2, 4, 64), dtype=torch.bfloat16, device="cuda") for _ in "kv"]
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    cb.qk_norm_rope(x, x, torch.arange(3, device="cuda"), cb.rope_frequencies(64)[0], v=x, k_cache=cache[0], v_cache=cache[1],
+                    slots=torch.tensor([2 ** 32 + 1, -2 ** 32 + 2, 2 ** 31], device="cuda"), status=status)
+    assert int(status.item()) == 1 and not cache[0].any() and not cache[1].any()

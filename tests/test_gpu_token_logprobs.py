@@ -182,3 +182,11 @@ def test_refusals():
     with pytest.raises(NotImplementedError, match="33 alternatives"):
         cb.token_logprobs(x, t, top=33)
     assert cb.token_logprobs(x[:0], t[:0], top=2).top_ids.shape == (0, 2)
+
+
+def test_int64_tokens_beyond_int32():
+    import cachalot_b200 as cb
+
+    x, word = torch.randn((3, 300), device="cuda", generator=_gen(8)), torch.zeros(1, dtype=torch.int32, device="cuda")
+    r = cb.token_logprobs(x, torch.tensor([2 ** 32 + 5, -2 ** 33 + 5, 5], device="cuda"), status=word)
+    assert r.logprobs[:2].tolist() == [0.0, 0.0] and int(word.item()) == 2 and float(r.logprobs[2]) < 0

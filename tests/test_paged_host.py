@@ -148,3 +148,13 @@ def test_paged_attention_refuses_an_infinite_softcap():
     call = lambda cap: _lib.lib.cachalot_paged_attention(p, 64, 64, _lib.BF16, 1, 1, C.byref(d), p, 2, 2, p, 0.125, 0, cap, p, 0, p, _lib.BF16, None, None, None)  # noqa: E731
     assert call(float("inf")) == _lib.EINVAL and "softcap" in _lib.last_error()
     assert call(1e39) == _lib.EINVAL and call(3e38) == _lib.ESCRATCH and call(0.0) == _lib.ESCRATCH
+
+
+def test_int64_values_beyond_int32_are_not_wrapped():
+    from cachalot_b200 import paged
+
+    wide = torch.tensor([2 ** 32 + 5, -2 ** 40, 7, 2 ** 31 - 1, -2 ** 31, 2 ** 31, 2 ** 63 - 1], dtype=torch.int64)
+    got = paged._ints(wide, "lens", (7,))
+    assert got.dtype == torch.int32 and got.tolist() == [2 ** 31 - 1, -2 ** 31, 7, 2 ** 31 - 1, -2 ** 31, 2 ** 31 - 1, 2 ** 31 - 1]
+    same = torch.tensor([1, 2], dtype=torch.int32)
+    assert paged._ints(same, "lens", (2,)) is same
