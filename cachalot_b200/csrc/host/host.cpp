@@ -114,7 +114,7 @@ int unlocked(F&& launch) {
 }
 #define UNLOCKED(call) unlocked([&] { return call; })
 
-// numeric arguments
+// numeric arguments and flags
 struct Args {
   PyObject* const* a;
   bool bad = false;
@@ -123,6 +123,11 @@ struct Args {
     if (v == -1 && PyErr_Occurred()) PyErr_Clear(), bad = true;
     if (v != (int)v) bad = true;
     return (int)v;
+  }
+  int truth(int n) {
+    const int v = PyObject_IsTrue(a[n]);
+    if (v < 0) PyErr_Clear(), bad = true;
+    return v;
   }
   double f(int n) {
     const double v = PyFloat_AsDouble(a[n]);
@@ -507,8 +512,8 @@ PyObject* qk_norm_rope(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   const int dev = current_device();
   const ScalarType dt = q->scalar_type();
   const double eps = p.f(6), magnitude = p.f(8);
-  const int interleaved = PyObject_IsTrue(a[7]);
-  PLAIN_OR_NONE(!p.bad && interleaved >= 0 && (dt == ScalarType::Half || dt == ScalarType::BFloat16) && head_rows(q, dt, dev) && head_rows(k, dt, dev));
+  const int interleaved = p.truth(7);
+  PLAIN_OR_NONE(!p.bad && (dt == ScalarType::Half || dt == ScalarType::BFloat16) && head_rows(q, dt, dev) && head_rows(k, dt, dev));
   const int64_t tokens = q->size(0), heads = q->size(1), dim = q->size(2), kv_heads = k->size(1);
   PLAIN_OR_NONE(tokens > 0 && tokens < (1LL << 31) && heads > 0 && heads < (1 << 20) && kv_heads > 0 && kv_heads < (1 << 20) && dim > 0 && dim <= 4096);
   PLAIN_OR_NONE(k->size(0) == tokens && k->size(2) == dim && plain_ints(pos, tokens, dev) && plain(freq, ScalarType::Double, dev) && freq->dim() == 1 && freq->size(0) <= dim);
@@ -556,8 +561,8 @@ PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   const int dev = current_device();
   const ScalarType dt = q->scalar_type();
   const double softcap = p.f(7);
-  const int window = (int)p.i(6), odt = a[10] == Py_None ? element_code(dt) : (int)p.i(10), want = PyObject_IsTrue(a[11]);
-  PLAIN_OR_NONE(!p.bad && want >= 0 && (dt == ScalarType::Half || dt == ScalarType::BFloat16) && q->get_device() == dev && q->dim() == 3 && q->stride(2) == 1);
+  const int window = (int)p.i(6), odt = a[10] == Py_None ? element_code(dt) : (int)p.i(10), want = p.truth(11);
+  PLAIN_OR_NONE(!p.bad && (dt == ScalarType::Half || dt == ScalarType::BFloat16) && q->get_device() == dev && q->dim() == 3 && q->stride(2) == 1);
   PLAIN_OR_NONE(q->stride(0) % 2 == 0 && q->stride(1) % 2 == 0 && reinterpret_cast<uintptr_t>(q->data_ptr()) % 4 == 0);
   const int64_t requests = q->size(0), heads = q->size(1), dim = q->size(2);
   PLAIN_OR_NONE(requests > 0 && requests < (1LL << 30) && heads > 0 && heads < (1 << 20) && odt >= CACHALOT_F16 && odt <= CACHALOT_F32 && window >= 0);

@@ -474,3 +474,10 @@ def test_int64_lengths_beyond_int32():
     out = cb.paged_attention(c.q, *c.caches, c.table, torch.tensor([2 ** 32 + 5, -2 ** 32 - 3], device="cuda"), status=word)
     want = cb.paged_attention(c.q, *c.caches, c.table, _int([64, 0]))
     assert torch.equal(out, want) and int(word.item()) == 32
+
+
+def test_want_lse_that_has_no_truth_value():
+    c = Case([5], 4, 2, 64, 16)
+    with pytest.raises(RuntimeError, match="ambiguous"):
+        c.run(want_lse=torch.ones(2))
+    assert torch.isfinite(c.run().float()).all()

@@ -268,3 +268,12 @@ def test_int64_slots_beyond_int32():
     cb.qk_norm_rope(x, x, torch.arange(3, device="cuda"), cb.rope_frequencies(64)[0], v=x, k_cache=cache[0], v_cache=cache[1],
                     slots=torch.tensor([2 ** 32 + 1, -2 ** 32 + 2, 2 ** 31], device="cuda"), status=status)
     assert int(status.item()) == 1 and not cache[0].any() and not cache[1].any()
+
+
+def test_interleaved_that_has_no_truth_value():
+    import cachalot_b200 as cb
+
+    x, pos, freq = torch.zeros((3, 2, 64), dtype=torch.bfloat16, device="cuda"), torch.arange(3, dtype=torch.int32, device="cuda"), cb.rope_frequencies(64)[0]
+    with pytest.raises((RuntimeError, ValueError)):  # int() of two elements; not an error of the interpreter itself
+        cb.qk_norm_rope(x, x, pos, freq, interleaved=torch.ones(2))
+    assert not cb.qk_norm_rope(x, x, pos, freq)[0].any()
