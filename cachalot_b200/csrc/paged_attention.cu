@@ -223,8 +223,9 @@ extern "C" int cachalot_paged_attention(const void* q, int64_t q_row_stride, int
   const long long bound = steps * requests * a.c.kv_heads * l.head_blocks;
   const int ctas = (int)(bound < most ? bound : most);
   cudaStream_t s = (cudaStream_t)stream;
-  const int rc = f8 ? launch_attend_e4m3(a, a.c.head_dim, ctas, s) : q_dtype == CACHALOT_BF16 ? launch_attend_bf16(a, a.c.head_dim, ctas, s)
-                                                                                            : launch_attend_f16(a, a.c.head_dim, ctas, s);
+  const auto launch = f8                        ? (out_dtype == CACHALOT_F32 ? launch_attend_e4m3_f32 : launch_attend_e4m3)
+                      : q_dtype == CACHALOT_BF16 ? launch_attend_bf16 : launch_attend_f16;
+  const int rc = launch(a, a.c.head_dim, ctas, s);
   if (rc) return rc;
   JoinArgs j{a.part_o, a.part_ml, a.parts, l.unit_heads, l.head_blocks, heads, a.group, a.c.head_dim,
              f8 || q_dtype == CACHALOT_F16 ? 7.f : 0.f, f8 ? a.c.v_scale : nullptr, out, out_dtype, lse};

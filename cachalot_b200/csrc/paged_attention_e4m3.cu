@@ -2,5 +2,5 @@
 #include "paged_attention.cuh"
 
 namespace cachalot {
-int launch_attend_e4m3(AttendArgs& a, int dim, int ctas, cudaStream_t stream) { return launch_attend<__half, true>(a, dim, ctas, stream); }
+int launch_attend_e4m3(AttendArgs& a, int dim, int ctas, cudaStream_t stream) { return launch_attend<__half, true, 1>(a, dim, ctas, stream); }
 }  // namespace cachalot

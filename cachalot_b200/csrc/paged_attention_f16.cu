@@ -2,5 +2,5 @@
 #include "paged_attention.cuh"
 
 namespace cachalot {
-int launch_attend_f16(AttendArgs& a, int dim, int ctas, cudaStream_t stream) { return launch_attend<__half, false>(a, dim, ctas, stream); }
+int launch_attend_f16(AttendArgs& a, int dim, int ctas, cudaStream_t stream) { return launch_attend<__half, false, 2>(a, dim, ctas, stream); }
 }  // namespace cachalot

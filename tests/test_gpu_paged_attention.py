@@ -481,3 +481,23 @@ def test_want_lse_that_has_no_truth_value():
     with pytest.raises(RuntimeError, match="ambiguous"):
         c.run(want_lse=torch.ones(2))
     assert torch.isfinite(c.run().float()).all()
+
+
+@pytest.mark.parametrize("dim,group,page", [(64, 3, 16), (128, 9, 16), (128, 20, 8), (96, 1, 7), (192, 24, 16), (256, 5, 24)])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_float32_results_over_an_e4m3_cache(dtype, dim, group, page):
+    """Two f16 terms of every weight, as over an f16 cache: 2^-22 of spread instead of 2^-11.  Small scores and few tokens, so that
+    what the scores carry does not cover the difference."""
+    for lens in ([2, 3, 5, 6, 40, 0, 1], [i % 7 for i in range(90)], [20000]):
+        heads = 2 if len(lens) == 7 else 8 if len(lens) > 7 else 1
+        if len(lens) == 1 and dim != 64:
+            continue
+        c = Case(lens, group * heads, heads, dim, page, dtype, E4M3, q_scale=0.02, seed=dim + group)
+        out, lse = c.run(want_lse=True, out_dtype=F32)
+        wout, wlse, spread, reach, floor = c.want()
+        d = dim * (2.0 ** -22 + 2.0 ** -24) * reach
+        tol = (4 * d[..., None] + 2.0 ** -16 + 2.0 ** -22) * spread + 2.0 ** -32 * floor
+        tol = tol + HALF[F32] * (np.abs(wout) + tol)
+        assert (np.abs(out.double().cpu().numpy() - wout) <= tol).all(), (np.abs(out.double().cpu().numpy() - wout) / np.maximum(tol, 1e-30)).max()
+        live = wlse > -np.inf
+        assert (np.abs(lse.double().cpu().numpy()[live] - wlse[live]) <= d[live] + 2.0 ** -16 + 2.0 ** -22 * np.abs(wlse[live])).all()
