@@ -141,3 +141,74 @@ def test_prompt_chunk_then_decode():
             o = paged.attend(q[i, h].double().cpu().numpy(), keys[:, h // 4], values[:, h // 4], DIM ** -0.5)
             assert (np.abs(out[i, h] - o[0]) <= (2.0 ** -14 + 4 * DIM * 2.0 ** -22 * o[3]) * o[2]).all()
     assert int(layer.status.item()) == 0 and plan.free_count.tolist() == [layer.pages - 3 - 1 - 1]
+
+
+@pytest.mark.parametrize("last", ["kernel", "copy", "operator"])
+def test_captured_forks_that_meet_in_front_of_the_operators(last):
+    """Two captured streams join right before each operator (which is launched early): it has to wait for both."""
+    import cachalot_b200 as cb
+
+    page, dim = 16, 64
+    base = {k: torch.zeros(n, dtype=torch.int32, device="cuda") for k, n in dict(ctx=2, new=2, count=1).items()}
+    ctx, new, count = base["ctx"], base["new"], base["count"]
+    table, free = torch.full((2, 8), -1, dtype=torch.int32, device="cuda"), torch.arange(16, dtype=torch.int32, device="cuda")
+    x = torch.zeros((8, 4, dim), dtype=torch.bfloat16, device="cuda")
+    src = {k: torch.zeros_like(v) for k, v in dict(ctx=ctx, new=new, x=x).items()}
+    kc, vc = (torch.zeros((16, 1, page, dim), dtype=torch.bfloat16, device="cuda") for _ in "kv")
+    freq = cb.rope_frequencies(dim)[0]
+    filler = torch.zeros(1 << 22, device="cuda")
+    logits, ids = torch.zeros((2, 4000), device="cuda"), torch.zeros(2, dtype=torch.int32, device="cuda")
+    noise = torch.randn((2, 4000), device="cuda")
+
+    def slow(dst, source):  # a write that comes late
+        filler.add_(1.0), filler.mul_(0.5)
+        if last == "copy":
+            dst.copy_(source)
+        elif last == "kernel":
+            torch.add(source, 0, out=dst)
+        else:
+            dst.copy_(source)
+            cb.token_logprobs(noise, ids)
+
+    def forked(side, pairs):
+        here = torch.cuda.current_stream()
+        side.wait_stream(here)
+        with torch.cuda.stream(side):
+            slow(*pairs[0])
+        slow(*pairs[1])
+        here.wait_stream(side)
+
+    def step(side):
+        forked(side, [(ctx, src["ctx"]), (new, src["new"])])
+        plan = cb.plan_pages(ctx, new, table, free, count, page_size=page, tokens=8)
+        forked(side, [(x[:4], src["x"][:4]), (x[4:], src["x"][4:])])
+        y, _ = cb.qk_norm_rope(x[:, :2], x[:, 2:3], plan.positions, freq, v=x[:, 3:], k_cache=kc, v_cache=vc, slots=plan.slots)
+        q = torch.zeros((2, 2, dim), dtype=torch.bfloat16, device="cuda")
+        forked(side, [(q[:1], y[:1]), (q[1:], y[4:5])])
+        att = cb.paged_attention(q, kc, vc, table, plan.lens)
+        forked(side, [(logits[:1], noise[:1] * 2), (logits[1:], noise[1:] * 3)])
+        return (*plan, y, att, *cb.token_logprobs(logits, ids, top=4))
+
+    side = torch.cuda.Stream()
+
+    def fresh(seed):
+        g = torch.Generator(device="cuda").manual_seed(seed)
+        src["ctx"].zero_(), src["new"].copy_(torch.tensor([4, 4], device="cuda"))
+        src["x"].copy_(torch.randn(x.shape, device="cuda", generator=g)), noise.copy_(torch.randn(noise.shape, device="cuda", generator=g))
+        for t in (ctx, new, x, kc, vc, logits):
+            t.zero_()
+        table.fill_(-1), count.fill_(16)
+
+    fresh(1), step(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step(side)
+    for seed in (2, 3, 4):
+        fresh(seed)
+        want = [t.clone() for t in step(side)]
+        torch.cuda.synchronize()
+        fresh(seed), graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        assert want[3].tolist()[:8] == [240 + i for i in range(4)] + [224 + i for i in range(4)] and want[7].float().abs().max() > 0
