@@ -87,7 +87,10 @@ def _cache(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale, v_scale) -> _l
 
 class PagePlan(NamedTuple):
     """Where a step's new tokens go: `starts` int32 [requests+1], per token `requests`, `positions`, `slots` int32 [tokens]
-    (past the last one: -1, 0, -1), `lens` int32 [requests] with the new tokens, `free_count` int32 [1] pages left."""
+    (past the last one: -1, 0, -1), `lens` int32 [requests] with the new tokens, `free_count` int32 [1] pages left.
+
+    They may be views of one allocation that do not overlap, as those of `torch.split`: any of them keeps all of it alive (clone
+    what is kept longer than the step), and none may be resized, which would grow it over its neighbours."""
 
     starts: torch.Tensor
     requests: torch.Tensor
@@ -277,7 +280,8 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
 # ---- log probabilities ------------------------------------------------------------------------
 
 class TokenLogprobs(NamedTuple):
-    """float32 `logprobs` and `entropy` [rows], `top_ids` int32 and `top_logprobs` float32 [rows, top]."""
+    """float32 `logprobs` and `entropy` [rows], `top_ids` int32 and `top_logprobs` float32 [rows, top]; views of one allocation as those
+    of `PagePlan`."""
 
     logprobs: torch.Tensor
     entropy: torch.Tensor

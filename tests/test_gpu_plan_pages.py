@@ -134,3 +134,14 @@ def test_requests_around_the_default_shared_memory_limit():
     for n in (6135, 6136, 6143, 6144):
         run = subprocess.run([sys.executable, "-c", code, str(n)], cwd=root, capture_output=True, text=True, timeout=300)
         assert run.returncode == 0, (n, run.stderr[-2000:])
+
+
+def test_outputs_of_one_call_do_not_overlap():
+    """They may be pieces of one allocation: writing into one leaves the others as they are."""
+    import cachalot_b200 as cb
+
+    p = cb.plan_pages(_cuda([3, 20]), _cuda([1, 14]), _cuda([[1, -1, -1], [2, 3, -1]]), _cuda(list(range(100, 110))), _cuda([10]), page_size=16, tokens=16)
+    for i, t in enumerate(p):
+        before = [u.clone() for u in p]
+        t.fill_(-77)
+        assert all(torch.equal(a, b) for j, (a, b) in enumerate(zip(before, p)) if j != i) and (t == -77).all()

@@ -190,3 +190,14 @@ def test_int64_tokens_beyond_int32():
     x, word = torch.randn((3, 300), device="cuda", generator=_gen(8)), torch.zeros(1, dtype=torch.int32, device="cuda")
     r = cb.token_logprobs(x, torch.tensor([2 ** 32 + 5, -2 ** 33 + 5, 5], device="cuda"), status=word)
     assert r.logprobs[:2].tolist() == [0.0, 0.0] and int(word.item()) == 2 and float(r.logprobs[2]) < 0
+
+
+def test_outputs_of_one_call_do_not_overlap():
+    """They may be pieces of one allocation: writing into one leaves the others as they are."""
+    import cachalot_b200 as cb
+
+    r = cb.token_logprobs(torch.randn((3, 300), device="cuda"), torch.tensor([1, 2, 3], dtype=torch.int32, device="cuda"), top=7)
+    for i, t in enumerate(r):
+        before = [u.clone() for u in r]
+        t.fill_(-77)
+        assert all(torch.equal(a, b) for j, (a, b) in enumerate(zip(before, r)) if j != i) and (t == -77).all()
