@@ -7,6 +7,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
 #include <cstdarg>
 #include <cstdio>
 #include <mutex>
@@ -171,6 +172,19 @@ inline cudaError_t smem_optin_once(K kern, int bytes) {
   e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
   if (e == cudaSuccess) done.insert({(const void*)kern, dev});
   return e;
+}
+
+// SMs of the current device, asked for once per device; `otherwise` where there is none.
+inline int device_sms(int otherwise) {
+  static std::atomic<int> known[16];
+  int dev = 0, sms = 0;
+  if (cudaGetDevice(&dev) == cudaSuccess && dev >= 0 && dev < 16 && (sms = known[dev].load(std::memory_order_relaxed)) > 0) return sms;
+  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || sms <= 0) {
+    (void)cudaGetLastError();
+    return otherwise;
+  }
+  if (dev < 16) known[dev].store(sms, std::memory_order_relaxed);
+  return sms;
 }
 
 // Streaming loads of memory that the kernel before may have written (no .nc).

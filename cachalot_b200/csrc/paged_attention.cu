@@ -1,6 +1,6 @@
 // Paged attention: argument checks, workspace, and the join of units that lie in several CTAs (the kernel itself:
 // paged_attention.cuh).
-#include <atomic>
+#include <algorithm>
 #include <cmath>
 
 #include "paged_attention.cuh"
@@ -14,7 +14,7 @@ struct JoinArgs {
   const float* part_o;
   const float2* part_ml;
   const int4* parts;
-  int unit_heads, head_blocks, heads, group, dim;
+  int unit_heads, head_blocks, heads, group;
   float shift;
   const float* v_scale;
   void* out;
@@ -124,18 +124,7 @@ bool shape_of(bool f8, int dim, int group, AttendLaunch* l) {
   return f8 ? attend_dispatch<true>(dim, group, take) : attend_dispatch<false>(dim, group, take);
 }
 
-int sm_count() {  // of the current device; an attribute of the device, asked for once
-  static std::atomic<int> known[16];
-  int dev = 0, sms = 0;
-  if (cudaGetDevice(&dev) == cudaSuccess && dev >= 0 && dev < 16 && (sms = known[dev].load(std::memory_order_relaxed)) > 0) return sms;
-  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || sms <= 0) {
-    (void)cudaGetLastError();
-    return PA_MAX_SMS;  // no device: sizes only
-  }
-  sms = sms < PA_MAX_SMS ? sms : PA_MAX_SMS;
-  if (dev < 16) known[dev].store(sms, std::memory_order_relaxed);
-  return sms;
-}
+int sm_count() { return std::min(device_sms(PA_MAX_SMS), PA_MAX_SMS); }  // no device: sizes only
 
 size_t up(size_t v) { return (v + 255) / 256 * 256; }
 
@@ -227,7 +216,7 @@ extern "C" int cachalot_paged_attention(const void* q, int64_t q_row_stride, int
                       : q_dtype == CACHALOT_BF16 ? launch_attend_bf16 : launch_attend_f16;
   const int rc = launch(a, a.c.head_dim, ctas, s);
   if (rc) return rc;
-  JoinArgs j{a.part_o, a.part_ml, a.parts, l.unit_heads, l.head_blocks, heads, a.group, a.c.head_dim,
+  JoinArgs j{a.part_o, a.part_ml, a.parts, l.unit_heads, l.head_blocks, heads, a.group,
              f8 || q_dtype == CACHALOT_F16 ? 7.f : 0.f, f8 ? a.c.v_scale : nullptr, out, out_dtype, lse};
   cudaError_t e = cudaSuccess;
   auto join = [&](auto kern) { e = launch_early(kern, dim3(ctas), PA_THREADS, 0, s, 1, j); };

@@ -373,10 +373,11 @@ extern "C" int cachalot_qk_norm_rope(const void* q, int64_t q_token_stride, int6
   const int lanes = head_dim <= 64 ? 8 : head_dim <= 128 ? 16 : 32, groups = QR_THREADS / lanes;
   // Many tokens of few heads: several tokens share a CTA, so that a group has eight heads per setting of its factors (18589
   // tokens of 6 + 2 + 2 heads of 128: 22.6 us; 16384 of 16 + 2 + 2: 40 us, with four heads per setting 52).  Few tokens: their heads go over several CTAs.
+  const int sms = device_sms(148);
   int crew = groups;
-  while (crew > 1 && heads < 8 * crew && (long long)tokens * crew / groups >= 1200) crew /= 2;
+  while (crew > 1 && heads < 8 * crew && (long long)tokens * crew / groups >= 8 * sms) crew /= 2;
   for (a.crew_log2 = 0; 1 << a.crew_log2 < crew;) ++a.crew_log2;
-  const long long parts = ((long long)heads + groups - 1) / groups, want = (600 + (long long)tokens - 1) / tokens;
+  const long long parts = ((long long)heads + groups - 1) / groups, want = (4 * sms + (long long)tokens - 1) / tokens;
   const dim3 grid((unsigned)((tokens + (long long)groups / crew - 1) / (groups / crew)), (unsigned)(parts < want ? parts : want));
   cudaStream_t s = (cudaStream_t)stream;
   cudaError_t e = cudaSuccess;

@@ -464,14 +464,15 @@ extern "C" int cachalot_token_logprobs(const void* logits, int dtype, int64_t ro
   // What ends a row costs its CTA the same for any number of warps, so many rows get small CTAs (us with 2, 4 and 8 warps):
   // 600 rows of 4000 bf16 12.2, 8.4, 13.2; 600 of 129280 71.9, 52.2, 52.1; 1300 of 16000 26.2, 26.3, 27.4; 4096 of 4000 and the
   // 32 largest 41, 42, 62; 16384 of 32000 240, 267, 312; 2048 of 129280 119, 113, 116.
-  const int warps = rows > 1184 && (long long)vocab * es <= 65536 ? 2 : rows > 592 ? 4 : TL_WARPS;
+  const int places = device_sms(148) * TL_CTAS;  // 592 on a B200
+  const int warps = rows > 2 * places && (long long)vocab * es <= 65536 ? 2 : rows > places ? 4 : TL_WARPS;
   // CTAs of a row: what takes the least time with 16 GB/s and a fixed part each, and the cluster's meeting where there is
   // more than one
-  const double slots = 148.0 * TL_CTAS, row_us = (double)vocab * es / 16e3, fixed_us = top ? 3.0 : 1.0, meet_us = top ? 3.0 : 1.5;
+  const double row_us = (double)vocab * es / 16e3, fixed_us = top ? 3.0 : 1.0, meet_us = top ? 3.0 : 1.5;
   int ctas = 1;
   double least = 1e30;
   for (int c = 1; c <= 8 && warps == TL_WARPS; c *= 2) {
-    const double us = ceil((double)rows * c / slots) * (row_us / c + fixed_us) + (c > 1 ? meet_us : 0.0);
+    const double us = ceil((double)rows * c / places) * (row_us / c + fixed_us) + (c > 1 ? meet_us : 0.0);
     if (us < least) least = us, ctas = c;
   }
   if ((long long)rows * ctas > 0x7fffffffLL) return fail(CACHALOT_EUNSUPPORTED, "token_logprobs: %d rows", rows);
