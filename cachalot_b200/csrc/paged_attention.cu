@@ -212,7 +212,7 @@ extern "C" int cachalot_paged_attention(const void* q, int64_t q_row_stride, int
   const long long bound = steps * requests * a.c.kv_heads * l.head_blocks;
   const int ctas = (int)(bound < most ? bound : most);
   cudaStream_t s = (cudaStream_t)stream;
-  const auto launch = f8                        ? (out_dtype == CACHALOT_F32 ? launch_attend_e4m3_f32 : launch_attend_e4m3)
+  const auto launch = f8                        ? (out_dtype == CACHALOT_BF16 ? launch_attend_e4m3 : launch_attend_e4m3_two)
                       : q_dtype == CACHALOT_BF16 ? launch_attend_bf16 : launch_attend_f16;
   const int rc = launch(a, a.c.head_dim, ctas, s);
   if (rc) return rc;

@@ -1,5 +1,5 @@
 // Attention of one new token per request over a paged key-value cache: the kernel, instantiated per cache type in
-// paged_attention_{bf16,f16,e4m3,e4m3_f32}.cu.
+// paged_attention_{bf16,f16,e4m3,e4m3_two}.cu.
 //
 //   s_j = scale * q . k_j   (cap * tanh(s / cap) with a soft cap),  j in [max(0, len - window), len)
 //   out = sum_j 2^(s_j log2 e - m) v_j / sum_j 2^(s_j log2 e - m),  m a running maximum
@@ -220,8 +220,9 @@ __device__ __forceinline__ void store_out4(void* out, int dtype, long long at, f
   }
 }
 
-// TERMS of P, of the matrix type: two keep 16 bits of a weight (bf16) or 22 (f16); one f16 term, 11 bits, over an E4M3 cache whose
-// result is rounded to 16 bits anyway (two cost 64 requests of up to 8192 tokens, 8, 16 and 24 query heads of 128, 128 and 192 to a
+// TERMS of P, of the matrix type: two keep 16 bits of a weight (bf16) or 22 (f16); one f16 term, 11 bits, over an E4M3 cache where
+// the result is rounded to bf16 (error against 64 bits 1.67e-3 with one term, 1.66e-3 of the rounding alone; rounded to f16 2.8e-4 and 2.1e-4, so
+// that takes two; they cost 64 requests of up to 8192 tokens, 8, 16 and 24 query heads of 128, 128 and 192 to a
 // key-value head, 101 us instead of 97, 146 instead of 131, 299 instead of 271).
 template <typename M, bool F8, int D, int NT, bool PAGE8, bool KEEP, int W, int TERMS>
 __global__ void __launch_bounds__(W * 32, AttendShape<F8, D, NT, W>::CTAS) attend_kernel(const AttendArgs a) {
@@ -805,6 +806,6 @@ int launch_attend(AttendArgs& a, int dim, int ctas, cudaStream_t stream) {
 int launch_attend_bf16(AttendArgs& a, int dim, int ctas, cudaStream_t stream);
 int launch_attend_f16(AttendArgs& a, int dim, int ctas, cudaStream_t stream);
 int launch_attend_e4m3(AttendArgs& a, int dim, int ctas, cudaStream_t stream);
-int launch_attend_e4m3_f32(AttendArgs& a, int dim, int ctas, cudaStream_t stream);
+int launch_attend_e4m3_two(AttendArgs& a, int dim, int ctas, cudaStream_t stream);
 
 }  // namespace cachalot

@@ -1,4 +1,4 @@
-// Paged attention over E4M3 caches (kernel and reasons: paged_attention.cuh).
+// Paged attention over E4M3 caches, bfloat16 results (kernel and reasons: paged_attention.cuh).
 #include "paged_attention.cuh"
 
 namespace cachalot {

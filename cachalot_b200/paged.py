@@ -239,7 +239,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     i // (heads // kv_heads); `scale` defaults to dim ** -0.5; softcap > 0: scores softcap * tanh(s / softcap); window > 0:
     only the last `window` tokens.  Returns out [requests, heads, dim] in `out_dtype` (default: q's), with `want_lse` also
     float32 [requests, heads] log sum exp of the scores.  Scores and sums are float32; softmax weights meet the values with 16
-    bits over a bfloat16 cache, 22 over a float16 one, and over an E4M3 one 11, or 22 with out_dtype float32.  A request of length 0
+    bits over a bfloat16 cache, 22 over a float16 one, and over an E4M3 one 11 for bfloat16 results, 22 for others.  A request of length 0
     gives zeros and -inf; tokens whose table entry is no page of the cache are hidden, lengths past the table cut (bits in
     `status`).  The lengths are read on the device: nothing waits for them, and a captured call replays with new ones."""
     r = _host.paged_attention(q, k_cache, v_cache, block_table, lens, scale, window, softcap, k_scale, v_scale,

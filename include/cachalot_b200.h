@@ -417,7 +417,7 @@ CACHALOT_API int cachalot_qk_norm_rope(const void* q, int64_t q_token_stride, in
  * q [requests, heads, head_dim] F16 or BF16 (strides in elements, 4-byte aligned), out [requests, heads, head_dim]
  * contiguous in out_dtype, lse f32 [requests, heads] or NULL; query head i reads key-value head i / (heads / kv_heads).
  * The cache holds q's type or E4M3.  Everything between the products is fp32 (a soft cap adds at most 2^-18 of the capped score); softmax weights enter the second one with 16
- * bits (bf16 cache), 22 (f16; E4M3 with out_dtype F32) or 11 (E4M3 otherwise), and a bf16 query enters the first one over an E4M3 cache as f16
+ * bits (bf16 cache), 22 (f16; E4M3 where out_dtype is not BF16) or 11 (E4M3 otherwise), and a bf16 query enters the first one over an E4M3 cache as f16
  * relative to its head's largest element (elements below 2^-17 of that lose bits, 2^-25 of the largest at most).  What lies behind a length or on hidden pages may be anything, NaN too; a visible
  * value that is not finite makes its element NaN or infinite for the heads that see it; a score that is NaN (a NaN in the query or
  * in a visible key) makes its head's elements and lse NaN.  block_table i32 [requests, width], rows table_stride apart; lens i32 [requests].  A request without a visible

@@ -501,3 +501,18 @@ def test_float32_results_over_an_e4m3_cache(dtype, dim, group, page):
         assert (np.abs(out.double().cpu().numpy() - wout) <= tol).all(), (np.abs(out.double().cpu().numpy() - wout) / np.maximum(tol, 1e-30)).max()
         live = wlse > -np.inf
         assert (np.abs(lse.double().cpu().numpy()[live] - wlse[live]) <= d[live] + 2.0 ** -16 + 2.0 ** -22 * np.abs(wlse[live])).all()
+
+
+@pytest.mark.parametrize("dim,group", [(64, 3), (128, 9), (192, 24)])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_float16_results_over_an_e4m3_cache(dtype, dim, group):
+    """As float32 ones (test_float32_results_over_an_e4m3_cache), then rounded: the weights' part is far below that rounding."""
+    for lens in ([2, 3, 5, 6, 40, 0, 1], [i % 7 for i in range(90)]):
+        heads = 2 if len(lens) == 7 else 8
+        c = Case(lens, group * heads, heads, dim, 16, dtype, E4M3, q_scale=0.02, seed=dim + group)
+        out = c.run(out_dtype=F16).double().cpu().numpy()
+        wout, _, spread, reach, floor = c.want()
+        d = dim * (2.0 ** -22 + 2.0 ** -24) * reach
+        tol = (4 * d[..., None] + 2.0 ** -16 + 2.0 ** -22) * spread + 2.0 ** -32 * floor
+        tol = tol + HALF[F16] * (np.abs(wout) + tol) + 2.0 ** -25
+        assert (np.abs(out - wout) <= tol).all(), (np.abs(out - wout) / tol).max()
