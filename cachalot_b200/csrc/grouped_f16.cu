@@ -23,7 +23,7 @@
 // codes); the MMAs of a unit of 64 rows take 128.  So the unpacked operand goes registers -> TMEM (tcgen05.st, 32 cycles a
 // tile), not through shared memory, where writing and reading it again would take 256 cycles.  Sixteen warps unpack, four
 // per scheduler: a tile's step takes 455 to 476 cycles in a loop of eight warps by themselves, and sixteen instead of
-// eight took 2048 tokens from 4.85 to 4.28 ms.  In the kernel (64 experts, 3072 rows, gate/up) the schedulers issue in 65 %
+// eight took 2048 tokens from 4.85 to 4.28 ms.  In the kernel (64 experts, gate/up) the schedulers issue in 65 %
 // of the cycles, 1080 instructions per tile with scales, waits and addresses: issue slots bound it, not DRAM (18 %).
 //
 // Warp roles (768 threads): warp 0 TMA (weight tiles through a 3-D map {K/4 bytes, rows, slot}, activation rows

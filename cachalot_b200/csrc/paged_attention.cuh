@@ -7,21 +7,22 @@
 // HBM-bound: every visible key and value is read once for the G query heads that share it, 2 G FLOP per byte of a 16-bit
 // cache.  On CUDA cores G = 8 would already need the whole fp32 rate; the legacy warp MMA (m16n8k16) has ten times the
 // arithmetic this needs and, unlike tcgen05, takes its operands from registers, so nothing is staged:
-//   * a warp works on tiles of 16 tokens, 32 where a row is 128 bytes or less.  S^T = K Q^T has the tokens as MMA rows and 8 query heads as columns, O^T = V^T P^T
-//     the head's elements as rows and the 8 heads as columns: no row of an MMA is spent on padding for G = 8.
+//   * a warp works on tiles of 16 tokens, 32 where a row is 128 bytes or less.  S^T = K Q^T has the tokens as MMA rows and 8 query
+//     heads as columns, O^T = V^T P^T the head's elements as rows and the 8 heads as columns: no row of an MMA is spent on
+//     padding for G = 8.
 //   * the order of the reduction index is free, so a lane's 16-byte loads of a key row ARE its operand fragments; for the
 //     values, whose fragments pair two tokens, one byte permute per register pairs the words of two rows.
 //   * keys of the next tile are requested when the scores are done, its values when the products are: 4 to 8 KB in
-//     flight per warp, 12 to 16 warps per SM.
+//     flight per warp, 8 to 16 warps per SM.
 //   * S^T fragments become P^T fragments by one movmatrix each.
 //   * the running maximum moves only when a score exceeds it by more than 2^8 (one vote per tile instead of six shuffles
 //     and a rescaling); P stays below 2^8 in bf16, and is shifted by 2^7 in f16 to use that type's range.
-// Work is cut on the device, where the lengths are: the steps (a tile for each of a CTA's warps, of one request and key-value head) of the whole
-// batch are laid on a line and every CTA takes an equal run of it, so a batch of very different lengths is balanced
+// Work is cut on the device, where the lengths are: the steps (a tile for each of a CTA's warps, of one request and key-value head)
+// of the whole batch are laid on a line and every CTA takes an equal run of it, so a batch of very different lengths is balanced
 // and one long request fills the GPU.  A unit (request, head) also occupies what it costs to begin one (query, first
-// page, empty pipeline, merge: as long as 48 or 96 KB of keys and values, or 384 tokens of E4M3; without that, CTAs with many short requests
-// took twice the average and 32 requests of 1 to 8192 tokens 79 us), and a cut that falls near a unit's end is moved there.
-// A CTA merges its four warps in shared memory; a unit that lies in one CTA is finished there, a unit that crosses
+// page, empty pipeline, merge: as long as 48 or 96 KB of keys and values, or 384 tokens of E4M3; without that, CTAs with many
+// short requests took twice the average and 32 requests of 1 to 8192 tokens 79 us), and a cut that falls near a unit's end is moved there.
+// A CTA's warps (four, or one where short requests are many) are merged in shared memory; a unit that lies in one CTA is finished there, a unit that crosses
 // CTAs leaves (m, l, O) of each part for the join kernel.
 #pragma once
 #include <cfloat>

@@ -208,7 +208,7 @@ struct Share {
   }
 };
 
-// The best n of a round in hand: the thread's own best, and its elements that reach a bar, appended to a list.
+// A thread's best element of a round, the first of equal ones.
 template <typename T, int WARPS>
 __device__ __forceinline__ Key best_of(const Share<T, WARPS>& sh, const Vec<T> (&v)[TL_LOADS], int round, float most) {
   Key best = 0;

@@ -241,7 +241,9 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     float32 [requests, heads] log sum exp of the scores.  Scores and sums are float32; softmax weights meet the values with 16
     bits over a bfloat16 cache, 22 over a float16 one, and over an E4M3 one 11 for bfloat16 results, 22 for others.  A request of length 0
     gives zeros and -inf; tokens whose table entry is no page of the cache are hidden, lengths past the table cut (bits in
-    `status`).  The lengths are read on the device: nothing waits for them, and a captured call replays with new ones."""
+    `status`).  The lengths are read on the device: nothing waits for them, and a captured call replays with new ones.  What
+    suits many short requests (up to 1024 tokens, 4096 over E4M3) is chosen by how many tokens a row of `block_table` holds, or by the
+    window: a view of the table's first columns that the batch needs makes such a batch up to twice as fast."""
     r = _host.paged_attention(q, k_cache, v_cache, block_table, lens, scale, window, softcap, k_scale, v_scale,
                               None if out_dtype is None else _DT.get(out_dtype, -1), want_lse, status)
     if r is not None:

@@ -415,16 +415,20 @@ CACHALOT_API int cachalot_qk_norm_rope(const void* q, int64_t q_token_stride, in
  *   s_j = scale * q . k_j  (softcap > 0, finite: softcap * tanh(s_j / softcap)),  out = softmax(s) V,  lse = log sum_j exp(s_j)
  * over j < lens[r], with window > 0 only the last `window` of them (the new token is one of them and already in the cache).
  * q [requests, heads, head_dim] F16 or BF16 (strides in elements, 4-byte aligned), out [requests, heads, head_dim]
- * contiguous in out_dtype, lse f32 [requests, heads] or NULL; query head i reads key-value head i / (heads / kv_heads).
- * The cache holds q's type or E4M3.  Everything between the products is fp32 (a soft cap adds at most 2^-18 of the capped score); softmax weights enter the second one with 16
- * bits (bf16 cache), 22 (f16; E4M3 where out_dtype is not BF16) or 11 (E4M3 otherwise), and a bf16 query enters the first one over an E4M3 cache as f16
- * relative to its head's largest element (elements below 2^-17 of that lose bits, 2^-25 of the largest at most).  What lies behind a length or on hidden pages may be anything, NaN too; a visible
- * value that is not finite makes its element NaN or infinite for the heads that see it; a score that is NaN (a NaN in the query or
- * in a visible key) makes its head's elements and lse NaN.  block_table i32 [requests, width], rows table_stride apart; lens i32 [requests].  A request without a visible
- * key gets zeros and -inf.  A length past its table is cut, a negative one counts as 0 (CACHALOT_STATUS_LENGTH); tokens on
- * a page outside [0, n_pages) are hidden (CACHALOT_STATUS_SLOT_RANGE); pages that no visible token lies on are not looked at.
- * head_dim 64, 96, 128, 192 or 256.  workspace: cachalot_paged_attention_workspace_bytes() bytes, 256-byte aligned, not
- * shared by calls that may overlap; its content does not matter. */
+ * contiguous in out_dtype, lse f32 [requests, heads] or NULL; query head i reads key-value head i / (heads / kv_heads). The
+ * cache holds q's type or E4M3.  Everything between the products is fp32 (a soft cap adds at most 2^-18 of the capped
+ * score); softmax weights enter the second one with 16 bits (bf16 cache), 22 (f16; E4M3 where out_dtype is not BF16) or 11
+ * (E4M3 otherwise), and a bf16 query enters the first one over an E4M3 cache as f16 relative to its head's largest element
+ * (elements below 2^-17 of that lose bits, 2^-25 of the largest at most).  What lies behind a length or on hidden pages may
+ * be anything, NaN too; a visible value that is not finite makes its element NaN or infinite for the heads that see it; a
+ * score that is NaN (a NaN in the query or in a visible key) makes its head's elements and lse NaN.  block_table i32
+ * [requests, width], rows table_stride apart; lens i32 [requests].  A request without a visible key gets zeros and -inf.  A
+ * length past its table is cut, a negative one counts as 0 (CACHALOT_STATUS_LENGTH); tokens on a page outside [0, n_pages)
+ * are hidden (CACHALOT_STATUS_SLOT_RANGE); pages that no visible token lies on are not looked at. head_dim 64, 96, 128, 192
+ * or 256; pages and tokens less than 4 GB apart.  Many requests of which none can hold more than 1024 tokens (4096 over
+ * E4M3) by width * page_size, or see more by the window, take a form made for short ones: width need not be more than the
+ * batch needs.  workspace: cachalot_paged_attention_workspace_bytes() bytes, 256-byte aligned, not shared by calls that may
+ * overlap; its content does not matter. */
 CACHALOT_API size_t cachalot_paged_attention_workspace_bytes(int heads, int kv_heads, int head_dim, int cache_dtype);
 CACHALOT_API int cachalot_paged_attention(const void* q, int64_t q_row_stride, int64_t q_head_stride, int q_dtype, int requests,
                              int heads, const cachalot_paged_kv* cache /* host */, const int32_t* block_table,
